@@ -11,6 +11,7 @@
 #include "common.cuh"
 
 #include "kernels.cuh"
+#include "linear.cuh"
 #include "prefill_kernels.cuh"
 
 namespace {
@@ -185,6 +186,91 @@ int gdn_prefill_fwd(const void* q, const void* k, const void* v, const float* st
     p.qpp = reinterpret_cast<uint16_t*>(ws + lay.off_qpp);
     p.oipp = reinterpret_cast<uint16_t*>(ws + lay.off_oipp);
     if (gdn::launch_prefill(p, bv, static_cast<cudaStream_t>(stream)) != 0) return GDN_ERR_CUDA;
+    return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
+}
+
+int gdn_linear_decode_fwd(const void* q, const void* k, const void* v, const float* state, const float* log_decay,
+                          int decay_per_token, float scale, void* out, float* new_state, int B, int H, int HV, int K,
+                          int V, void* stream, unsigned flags) {
+    if (!shape_ok(H, HV, K, V)) return GDN_ERR_SHAPE;
+    if (B < 0 || (long long)B * HV * 8 > 0x7fffffffll || (decay_per_token != 0 && decay_per_token != 1) || flags != 0)
+        return GDN_ERR_SIZE;
+    if (B == 0) return GDN_OK;
+    if (!q || !k || !v || !log_decay || !out || !new_state) return GDN_ERR_NULL;
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(new_state) ||
+        (state && !aligned16(state)) || (reinterpret_cast<uintptr_t>(log_decay) & 3u))
+        return GDN_ERR_ALIGN;
+    const int rc = check_device();
+    if (rc != GDN_OK) return rc;
+    gdn::LinearDecodeArgs p;
+    p.q = static_cast<const uint16_t*>(q);
+    p.k = static_cast<const uint16_t*>(k);
+    p.v = static_cast<const uint16_t*>(v);
+    p.state = state;
+    p.decay = log_decay;
+    p.per_token = decay_per_token;
+    p.scale = scale;
+    p.out = static_cast<uint16_t*>(out);
+    p.new_state = new_state;
+    p.B = B;
+    p.H = H;
+    p.HV = HV;
+    if (gdn::launch_linear_decode(p, static_cast<cudaStream_t>(stream)) != 0) return GDN_ERR_CUDA;
+    return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
+}
+
+size_t gdn_linear_prefill_workspace_bytes(int N, int T, int H, int HV, int K, int V) {
+    if (!shape_ok(H, HV, K, V) || N < 0 || T < 0) return 0;
+    return gdn::linear_prefill_layout(N, T, HV).total;
+}
+
+int gdn_linear_prefill_fwd(const void* q, const void* k, const void* v, const float* state, const float* log_decay,
+                           int decay_per_token, const void* cu_seqlens, int cu_is_int64, int N, int T, float scale,
+                           void* out, float* new_state, void* workspace, size_t workspace_bytes, int H, int HV, int K,
+                           int V, void* stream, unsigned flags) {
+    if (!shape_ok(H, HV, K, V)) return GDN_ERR_SHAPE;
+    if (N < 0 || T < 0 || (decay_per_token != 0 && decay_per_token != 1) || (cu_is_int64 != 0 && cu_is_int64 != 1) ||
+        (flags & ~GDN_FLAG_ZERO_UNOWNED))
+        return GDN_ERR_SIZE;
+    if (N == 0) return GDN_OK;
+    if (!cu_seqlens || !new_state) return GDN_ERR_NULL;
+    if (T > 0 && (!q || !k || !v || !log_decay || !out)) return GDN_ERR_NULL;
+    if ((T > 0 && (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))) || !aligned16(new_state) ||
+        (state && !aligned16(state)) || (reinterpret_cast<uintptr_t>(log_decay) & 3u) ||
+        (reinterpret_cast<uintptr_t>(cu_seqlens) & (cu_is_int64 ? 7u : 3u)))
+        return GDN_ERR_ALIGN;
+    const gdn::LinearPrefillLayout lay = gdn::linear_prefill_layout(N, T, HV);
+    if (((long long)lay.slots + lay.states) * HV > 0x7fffffffll) return GDN_ERR_SIZE;
+    if (!workspace || workspace_bytes < lay.total || (reinterpret_cast<uintptr_t>(workspace) & 255u))
+        return GDN_ERR_WORKSPACE;
+    const int rc = check_device();
+    if (rc != GDN_OK) return rc;
+    unsigned char* ws = static_cast<unsigned char*>(workspace);
+    gdn::LinearPrefillArgs p;
+    p.q = static_cast<const uint16_t*>(q);
+    p.k = static_cast<const uint16_t*>(k);
+    p.v = static_cast<const uint16_t*>(v);
+    p.state = state;
+    p.decay = log_decay;
+    p.per_token = decay_per_token;
+    p.cu = cu_seqlens;
+    p.cu64 = cu_is_int64;
+    p.N = N;
+    p.T = T;
+    p.H = H;
+    p.HV = HV;
+    p.zero_unowned = (flags & GDN_FLAG_ZERO_UNOWNED) ? 1 : 0;
+    p.scale = scale;
+    p.out = static_cast<uint16_t*>(out);
+    p.new_state = new_state;
+    p.m = lay.m;
+    p.slots = lay.slots;
+    p.states = lay.states;
+    p.cut = lay.cut;
+    p.status = reinterpret_cast<int*>(ws + lay.off_status);
+    p.gamma = reinterpret_cast<float*>(ws + lay.off_gamma);
+    p.seg = reinterpret_cast<float*>(ws + lay.off_seg);
+    if (gdn::launch_linear_prefill(p, static_cast<cudaStream_t>(stream)) != 0) return GDN_ERR_CUDA;
     return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
 }
 

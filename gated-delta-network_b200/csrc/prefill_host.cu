@@ -135,6 +135,11 @@ bool map2d(CUtensorMap* m, const void* base, CUtensorMapDataType dt, uint64_t d0
 
 }  // namespace
 
+bool map_bf16_rows(CUtensorMap* m, const void* base, int heads, int T) {
+    return map3d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 128, (uint64_t)heads, (uint64_t)T, 256, 256ull * heads, 64,
+                 1, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 bool build_prefill_maps(const PrefillArgs& p, PrefillMaps* m) {
     const uint64_t T = (uint64_t)p.T, R = (uint64_t)p.S * kChunk;
     const auto BF = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;

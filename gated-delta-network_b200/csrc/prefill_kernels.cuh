@@ -118,6 +118,8 @@ __device__ __forceinline__ int clamp_chunks(const PrefillArgs& p, int slot0, int
     return room > 0 ? room : 0;
 }
 
+// Map of [T][heads][128] bf16 rows: one box = 64 columns x 1 head x 64 tokens, SWIZZLE_128B.
+bool map_bf16_rows(CUtensorMap* m, const void* base, int heads, int T);
 bool build_prefill_maps(const PrefillArgs& p, PrefillMaps* m);
 
 // Workspace element offset of column group cg (8 state columns) of chunk slot `slot`, v-head hv,

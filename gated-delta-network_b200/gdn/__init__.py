@@ -11,10 +11,13 @@ Drop-in entry points with the reference's signatures:
 * ``gdn.prefill.kernel(..., cu_seqlens, scale, output, new_state)``
   (destination passing; solutions/gdn_prefill_qk4_v8_d128_k_last/solution/triton/fla_kernels.py:1049)
 
+Beside them, with the same tensors and state, linear attention with a decay for each head (no counterpart in
+the reference): ``gdn.linear_decode`` and ``gdn.linear_prefill``, ``run`` and ``kernel`` each.
+
 All compute runs in hand-written sm_100a CUDA behind the C ABI of
 ``include/gdn_b200.h`` (libgdn_b200.so); there is no CPU or Triton fallback.
 """
-from . import decode, prefill  # noqa: F401
+from . import decode, linear_decode, linear_prefill, prefill  # noqa: F401
 from ._lib import GDNError  # noqa: F401
 
-__all__ = ["decode", "prefill", "GDNError"]
+__all__ = ["decode", "linear_decode", "linear_prefill", "prefill", "GDNError"]

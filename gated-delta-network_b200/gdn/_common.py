@@ -80,3 +80,38 @@ def on_device(device: torch.device):
 def out_ok(t, device: torch.device, dtype: torch.dtype, numel: int) -> bool:
     return (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == device.index and t.dtype is dtype
             and t.is_contiguous() and t.numel() == numel)
+
+
+def decay_rows(log_decay, rows: int, HV: int, device: torch.device):
+    """(fp32 log decays on `device`, 1 if they hold a row for each token else 0): [HV] or [rows, (1,) HV]."""
+    if not isinstance(log_decay, torch.Tensor):
+        raise TypeError("log_decay must be a torch.Tensor")
+    shape = tuple(log_decay.shape)
+    if shape == (HV,):
+        per_token = 0
+    elif len(shape) in (2, 3) and shape[0] == rows and shape[-1] == HV and log_decay.numel() == rows * HV:
+        per_token = 1
+    else:
+        raise ValueError(f"log_decay must hold [{HV}] or [{rows}, {HV}] values (got {shape})")
+    return as_dev(log_decay, torch.float32, device), per_token
+
+
+def cu_on_device(cu_seqlens, device: torch.device):
+    """(contiguous cu_seqlens on `device`, 1 if int64 else 0, number of sequences)."""
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+        raise ValueError("cu_seqlens must be a tensor of at least one element")
+    if cu_seqlens.dtype not in (torch.int32, torch.int64):
+        raise ValueError("cu_seqlens must be int32 or int64")
+    cu = cu_seqlens if (cu_seqlens.is_cuda and cu_seqlens.get_device() == device.index) else cu_seqlens.to(device)
+    return cu.contiguous(), 1 if cu.dtype == torch.int64 else 0, cu_seqlens.shape[0] - 1
+
+
+def workspace_for(workspace, need: int, device: torch.device) -> torch.Tensor:
+    """The caller's workspace after its checks, or one from the caching allocator (for the current stream)."""
+    if workspace is None:
+        return torch.empty(max(need, 1), dtype=torch.uint8, device=device)
+    if (not isinstance(workspace, torch.Tensor) or not workspace.is_cuda or workspace.get_device() != device.index
+            or not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need
+            or workspace.data_ptr() % 256):
+        raise ValueError(f"workspace must be a contiguous, 256-byte aligned CUDA buffer of at least {need} bytes")
+    return workspace

@@ -16,6 +16,7 @@ _lib = None
 
 GDN_OK = 0
 GDN_FLAG_QK_L2NORM = 0x4  # include/gdn_b200.h
+GDN_FLAG_ZERO_UNOWNED = 0x20
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
@@ -53,6 +54,13 @@ def load():
             lib.gdn_prefill_fwd.argtypes = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _P, _P, _P, _SZ,
                                             _I, _I, _I, _I, _P, _U]
             lib.gdn_prefill_fwd.restype = _I
+            lib.gdn_linear_decode_fwd.argtypes = [_P, _P, _P, _P, _P, _I, _F, _P, _P, _I, _I, _I, _I, _I, _P, _U]
+            lib.gdn_linear_decode_fwd.restype = _I
+            lib.gdn_linear_prefill_workspace_bytes.argtypes = [_I, _I, _I, _I, _I, _I]
+            lib.gdn_linear_prefill_workspace_bytes.restype = _SZ
+            lib.gdn_linear_prefill_fwd.argtypes = [_P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _F, _P, _P, _P, _SZ, _I, _I,
+                                                   _I, _I, _P, _U]
+            lib.gdn_linear_prefill_fwd.restype = _I
             lib.gdn_status_string.argtypes = [_I]
             lib.gdn_status_string.restype = ctypes.c_char_p
             lib.gdn_version.restype = _I

@@ -65,6 +65,10 @@ enum gdn_status {
 #define GDN_FLAG_NO_SEGMENTS 0x8u
 #define GDN_FLAG_SEGMENTS 0x10u
 
+/* gdn_linear_prefill_fwd: write zeros to the output rows of tokens that no sequence owns (without it
+ * they are left as they were). */
+#define GDN_FLAG_ZERO_UNOWNED 0x20u
+
 /* Device-side status codes written to the first int of the prefill workspace. */
 #define GDN_DEVSTATUS_OK 0
 #define GDN_DEVSTATUS_SCAN_TMA_TIMEOUT 1
@@ -184,6 +188,35 @@ int gdn_prefill_fwd_noalloc(const void* q, const void* k, const void* v, const f
                             const void* a, const float* dt_bias, const void* b, const void* cu_seqlens,
                             int cu_is_int64, int N, int T, float scale, void* out, float* new_state, int H, int HV,
                             int K, int V, void* stream, unsigned flags);
+
+/*
+ * Linear attention with a decay for each head: the recurrence of the entry points above without beta
+ * and without the delta correction,
+ *   S <- e^a S + v k^T,   out = scale S q        (S is [V][K], fp32, k-last)
+ * with the log decay a <= 0 given for each head (decay_per_token = 0: log_decay [HV]) or for each token and
+ * head (decay_per_token = 1: log_decay [B, HV] or [T, HV]), f32.  -infinity forgets the state.  Neither
+ * entry point has a counterpart in the reference.
+ *
+ * gdn_linear_decode_fwd: one token for each of B sequences.  Tensors as for gdn_decode_fwd; new_state may
+ * be state itself; state NULL means zeros.  flags must be 0.
+ */
+int gdn_linear_decode_fwd(const void* q, const void* k, const void* v, const float* state, const float* log_decay,
+                          int decay_per_token, float scale, void* out, float* new_state, int B, int H, int HV, int K,
+                          int V, void* stream, unsigned flags);
+
+/*
+ * gdn_linear_prefill_fwd: N packed sequences of any lengths, tensors and cu_seqlens as for gdn_prefill_fwd.
+ * Two things differ from it: a zero-length sequence keeps its state (new_state = state, or zeros for a NULL
+ * state), and output rows of tokens outside every sequence are left as they were unless
+ * GDN_FLAG_ZERO_UNOWNED (the only flag) is given.  new_state may be state itself.  The workspace
+ * (256-byte aligned, at least gdn_linear_prefill_workspace_bytes) carries nothing between calls; its first
+ * int receives 0 or the code of a bounded device-side wait that gave up.
+ */
+size_t gdn_linear_prefill_workspace_bytes(int N, int T, int H, int HV, int K, int V);
+int gdn_linear_prefill_fwd(const void* q, const void* k, const void* v, const float* state, const float* log_decay,
+                           int decay_per_token, const void* cu_seqlens, int cu_is_int64, int N, int T, float scale,
+                           void* out, float* new_state, void* workspace, size_t workspace_bytes, int H, int HV, int K,
+                           int V, void* stream, unsigned flags);
 
 /* Human-readable name of a status code (static storage). */
 const char* gdn_status_string(int status);
