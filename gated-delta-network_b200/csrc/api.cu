@@ -274,6 +274,115 @@ int gdn_linear_prefill_fwd(const void* q, const void* k, const void* v, const fl
     return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
 }
 
+}  // extern "C"
+
+namespace {
+
+// Checks shared by the cache entry points; fills `c`.
+int cache_args(void* k_cache, void* v_cache, float* k_scale, float* v_scale, int code, const int* block_table,
+               const void* seq_lens, int len_is_int64, int num_pages, int page_size, int max_pages, int B, int Hkv, int D,
+               gdn::CacheArgs* c) {
+    if (D != GDN_HEAD_DIM || Hkv < 1 || Hkv > 65535) return GDN_ERR_SHAPE;
+    if (code != GDN_CODE_INT8 && code != GDN_CODE_E4M3) return GDN_ERR_SIZE;
+    int shift = 4;
+    while (shift < 7 && (1 << shift) != page_size) ++shift;
+    if ((1 << shift) != page_size) return GDN_ERR_SIZE;
+    if (num_pages < 0 || max_pages < 0 || ((long long)max_pages << shift) > 0x7fffffffll || B < 0 ||
+        (len_is_int64 != 0 && len_is_int64 != 1))
+        return GDN_ERR_SIZE;
+    if (B == 0) return GDN_OK;
+    if (!seq_lens || (max_pages > 0 && !block_table) || (num_pages > 0 && (!k_cache || !v_cache || !k_scale || !v_scale)))
+        return GDN_ERR_NULL;
+    if (!aligned16(k_cache) || !aligned16(v_cache) || (reinterpret_cast<uintptr_t>(k_scale) & 3u) ||
+        (reinterpret_cast<uintptr_t>(v_scale) & 3u) || (reinterpret_cast<uintptr_t>(block_table) & 3u) ||
+        (reinterpret_cast<uintptr_t>(seq_lens) & (len_is_int64 ? 7u : 3u)))
+        return GDN_ERR_ALIGN;
+    c->k_cache = k_cache;
+    c->v_cache = v_cache;
+    c->k_scale = k_scale;
+    c->v_scale = v_scale;
+    c->int8 = code == GDN_CODE_INT8 ? 1 : 0;
+    c->pages = num_pages;
+    c->Hkv = Hkv;
+    c->page_shift = shift;
+    c->table = block_table;
+    c->max_pages = max_pages;
+    c->seq_lens = seq_lens;
+    c->len64 = len_is_int64;
+    c->B = B;
+    return GDN_OK;
+}
+
+size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+constexpr size_t kAttendPieces = 256;  // byte offsets in the workspace: status, pieces, maxima and sums, results
+const size_t kAttendMl = up256(kAttendPieces + gdn::kAttendCtas * sizeof(int4));
+const size_t kAttendAcc = up256(kAttendMl + (size_t)gdn::kAttendCtas * 2 * 16 * 2 * sizeof(float));
+
+}  // namespace
+
+extern "C" {
+
+int gdn_cache_append(const void* k, const void* v, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                     int code, const int* block_table, const void* seq_lens, int len_is_int64, const void* cu_seqlens,
+                     int cu_is_int64, int num_pages, int page_size, int max_pages, int B, int T, int Hkv, int D,
+                     void* stream, unsigned flags) {
+    gdn::CacheAppendArgs p;
+    int rc = cache_args(k_cache, v_cache, k_scale, v_scale, code, block_table, seq_lens, len_is_int64, num_pages, page_size,
+                        max_pages, B, Hkv, D, &p.c);
+    if (rc != GDN_OK) return rc;
+    if (T < 0 || (long long)B * 2 + T > 0x7fffffffll || (cu_is_int64 != 0 && cu_is_int64 != 1) || flags != 0) return GDN_ERR_SIZE;
+    if (B == 0 || T == 0) return GDN_OK;
+    if (!cu_seqlens || !k || !v) return GDN_ERR_NULL;
+    if (!aligned16(k) || !aligned16(v) || (reinterpret_cast<uintptr_t>(cu_seqlens) & (cu_is_int64 ? 7u : 3u))) return GDN_ERR_ALIGN;
+    if (num_pages == 0 || max_pages == 0) return GDN_OK;  // no page to write to
+    rc = check_device();
+    if (rc != GDN_OK) return rc;
+    p.k = static_cast<const uint16_t*>(k);
+    p.v = static_cast<const uint16_t*>(v);
+    p.cu = cu_seqlens;
+    p.cu64 = cu_is_int64;
+    p.T = T;
+    if (gdn::launch_cache_append(p, static_cast<cudaStream_t>(stream)) != 0) return GDN_ERR_CUDA;
+    return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
+}
+
+size_t gdn_cache_attend_workspace_bytes(void) {
+    return kAttendAcc + (size_t)gdn::kAttendCtas * 2 * 16 * GDN_HEAD_DIM * sizeof(float);
+}
+
+int gdn_cache_attend(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                     int code, const int* block_table, const void* seq_lens, int len_is_int64, int num_pages,
+                     int page_size, int max_pages, int B, int Q, int Hq, int Hkv, int D, float scale, void* out,
+                     void* workspace, size_t workspace_bytes, void* stream, unsigned flags) {
+    gdn::CacheAttendArgs p;
+    int rc = cache_args(const_cast<void*>(k_cache), const_cast<void*>(v_cache), const_cast<float*>(k_scale),
+                        const_cast<float*>(v_scale), code, block_table, seq_lens, len_is_int64, num_pages, page_size,
+                        max_pages, B, Hkv, D, &p.c);
+    if (rc != GDN_OK) return rc;
+    if (Hq < Hkv || Hq % Hkv != 0) return GDN_ERR_SHAPE;
+    if (Q < 0 || flags != 0 || (long long)B * Hkv * (((long long)Q * (Hq / Hkv) + 15) / 16) > 0x7fffffffll) return GDN_ERR_SIZE;
+    if (B == 0 || Q == 0) return GDN_OK;
+    if (!q || !out) return GDN_ERR_NULL;
+    if (!aligned16(q) || !aligned16(out)) return GDN_ERR_ALIGN;
+    if (!workspace || workspace_bytes < gdn_cache_attend_workspace_bytes() || (reinterpret_cast<uintptr_t>(workspace) & 255u))
+        return GDN_ERR_WORKSPACE;
+    rc = check_device();
+    if (rc != GDN_OK) return rc;
+    if (num_pages == 0) p.c.max_pages = 0;  // an empty cache: every row sees nothing
+    unsigned char* ws = static_cast<unsigned char*>(workspace);
+    p.q = static_cast<const uint16_t*>(q);
+    p.Q = Q;
+    p.Hq = Hq;
+    p.scale = scale;
+    p.out = static_cast<uint16_t*>(out);
+    p.status = reinterpret_cast<int*>(ws);
+    p.piece = reinterpret_cast<int4*>(ws + kAttendPieces);
+    p.ml = reinterpret_cast<float*>(ws + kAttendMl);
+    p.acc = reinterpret_cast<float*>(ws + kAttendAcc);
+    if (gdn::launch_cache_attend(p, static_cast<cudaStream_t>(stream)) != 0) return GDN_ERR_CUDA;
+    return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
+}
+
 const char* gdn_status_string(int status) {
     switch (status) {
         case GDN_OK: return "ok";

@@ -50,6 +50,52 @@ struct LinearPrefillLayout {
 };
 LinearPrefillLayout linear_prefill_layout(int N, int T, int HV);
 
+// Paged key/value cache of 8-bit codes: x = code * scale[page][head].
+struct CacheArgs {
+    void* k_cache;         // [pages][Hkv][P][128] int8 or e4m3
+    void* v_cache;
+    float* k_scale;        // [pages][Hkv]
+    float* v_scale;
+    int int8;              // int8 codes, else e4m3
+    int pages, Hkv;
+    int page_shift;        // log2(P), 4 .. 7
+    const int* table;      // [B][max_pages] page of each P tokens of a sequence
+    int max_pages;
+    const void* seq_lens;  // [B] tokens of each sequence, the call's new ones included
+    int len64;
+    int B;
+};
+
+// Tokens of sequence b; a length that is not an int counts as 0.
+__device__ __forceinline__ int cache_length(const CacheArgs& c, int b) {
+    const long long n = c.len64 ? reinterpret_cast<const long long*>(c.seq_lens)[b] : reinterpret_cast<const int*>(c.seq_lens)[b];
+    return n < 0 || n > 0x7fffffffll ? 0 : (int)n;
+}
+
+struct CacheAppendArgs {
+    CacheArgs c;
+    const uint16_t* k;     // [T, Hkv, 128] bf16
+    const uint16_t* v;
+    const void* cu;        // [B+1]
+    int cu64;
+    int T;
+};
+
+struct CacheAttendArgs {
+    CacheArgs c;
+    const uint16_t* q;     // [B, Q, Hq, 128] bf16
+    int Q, Hq;
+    float scale;
+    uint16_t* out;         // [B, Q, Hq, 128] bf16
+    int* status;           // workspace
+    int4* piece;           // workspace: [kAttendCtas] {segment that CTA c begins and others end, pieces that follow, status}
+    float* ml;             // workspace: [kAttendCtas][2][16][2] running maximum (base 2) and sum of a piece
+    float* acc;            // workspace: [kAttendCtas][2][16][128]
+};
+constexpr int kAttendCtas = 296;  // 2 per SM
+
+int launch_cache_append(const CacheAppendArgs& p, cudaStream_t stream);
+int launch_cache_attend(const CacheAttendArgs& p, cudaStream_t stream);
 int launch_linear_decode(const LinearDecodeArgs& p, cudaStream_t stream);
 int launch_linear_prefill(const LinearPrefillArgs& p, cudaStream_t stream);
 

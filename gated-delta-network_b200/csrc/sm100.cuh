@@ -21,6 +21,7 @@ constexpr int kErrPrepTmaTimeout = 2;
 constexpr int kErrPrepMmaTimeout = 3;
 constexpr int kErrScanMmaTimeout = 4;
 constexpr int kErrBadSeqlens = 5;
+constexpr int kErrBadPage = 6;
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s
 
 __device__ __forceinline__ unsigned long long globaltimer_ns() {

@@ -115,3 +115,40 @@ def workspace_for(workspace, need: int, device: torch.device) -> torch.Tensor:
             or workspace.data_ptr() % 256):
         raise ValueError(f"workspace must be a contiguous, 256-byte aligned CUDA buffer of at least {need} bytes")
     return workspace
+
+
+CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}  # GDN_CODE_*
+PAGE_SIZES = (16, 32, 64, 128)
+
+
+def cache_tensors(k_cache, v_cache, k_scale, v_scale, device: torch.device):
+    """Checks of a paged 8-bit cache, which is used in place; returns (code, pages, Hkv, page size)."""
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != device.index or t.dtype not in CODES
+                or t.dim() != 4 or t.shape[3] != HEAD_DIM or not t.is_contiguous() or t.data_ptr() % 16):
+            raise ValueError(f"{name} must be a contiguous, 16-byte aligned int8 or float8_e4m3fn CUDA tensor "
+                             f"[pages, heads, page_size, {HEAD_DIM}]")
+    if k_cache.shape != v_cache.shape or k_cache.dtype is not v_cache.dtype:
+        raise ValueError("k_cache and v_cache must have the same shape and type")
+    pages, Hkv, P, _ = k_cache.shape
+    if P not in PAGE_SIZES:
+        raise ValueError(f"page size must be one of {PAGE_SIZES} (got {P})")
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if not out_ok(t, device, torch.float32, pages * Hkv) or tuple(t.shape) != (pages, Hkv):
+            raise ValueError(f"{name} must be a contiguous fp32 CUDA tensor [{pages}, {Hkv}]")
+    return CODES[k_cache.dtype], pages, Hkv, P
+
+
+def cache_rows(block_table, seq_lens, B: int, device: torch.device):
+    """(int32 block table, sequence lengths, 1 if those are int64 else 0, pages of a row), on `device`."""
+    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2 or block_table.shape[0] != B:
+        raise ValueError(f"block_table must be a tensor [{B}, max_pages]")
+    if block_table.dtype not in (torch.int32, torch.int64):
+        raise ValueError("block_table must be int32 or int64")
+    if not isinstance(seq_lens, torch.Tensor) or tuple(seq_lens.shape) != (B,):
+        raise ValueError(f"seq_lens must be a tensor [{B}]")
+    if seq_lens.dtype not in (torch.int32, torch.int64):
+        raise ValueError("seq_lens must be int32 or int64")
+    table = as_dev(block_table, torch.int32, device)
+    lens = as_dev(seq_lens, seq_lens.dtype, device)
+    return table, lens, 1 if lens.dtype is torch.int64 else 0, table.shape[1]

@@ -61,6 +61,14 @@ def load():
             lib.gdn_linear_prefill_fwd.argtypes = [_P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _F, _P, _P, _P, _SZ, _I, _I,
                                                    _I, _I, _P, _U]
             lib.gdn_linear_prefill_fwd.restype = _I
+            lib.gdn_cache_append.argtypes = [_P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I,
+                                             _P, _U]
+            lib.gdn_cache_append.restype = _I
+            lib.gdn_cache_attend_workspace_bytes.argtypes = []
+            lib.gdn_cache_attend_workspace_bytes.restype = _SZ
+            lib.gdn_cache_attend.argtypes = [_P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P,
+                                             _P, _SZ, _P, _U]
+            lib.gdn_cache_attend.restype = _I
             lib.gdn_status_string.argtypes = [_I]
             lib.gdn_status_string.restype = ctypes.c_char_p
             lib.gdn_version.restype = _I

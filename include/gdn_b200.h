@@ -79,6 +79,9 @@ enum gdn_status {
  * more 64-token chunks than the workspace holds and skipped the excess (the outputs of such a call
  * are invalid, but no access leaves the buffers). */
 #define GDN_DEVSTATUS_BAD_SEQLENS 5
+/* gdn_cache_attend: a page number outside the cache was met and its tokens were treated as hidden
+ * (5 there: a sequence is longer than its row of the block table, and was cut to it). */
+#define GDN_DEVSTATUS_BAD_PAGE 6
 
 /* Fixed shape family (the reference asserts exactly these:
  * reference/gdn_decode_ref.py:32-36, reference/gdn_prefill_ref.py:33-36). */
@@ -217,6 +220,45 @@ int gdn_linear_prefill_fwd(const void* q, const void* k, const void* v, const fl
                            int decay_per_token, const void* cu_seqlens, int cu_is_int64, int N, int T, float scale,
                            void* out, float* new_state, void* workspace, size_t workspace_bytes, int H, int HV, int K,
                            int V, void* stream, unsigned flags);
+
+/*
+ * Key/value cache in 8 bits with a scale for each page (block of tokens) and head, and attention over it:
+ * the softmax layers of a stack whose other layers are the operators above.  No counterpart in the
+ * reference.
+ *
+ *   k_cache, v_cache [num_pages, Hkv, page_size, D=128] codes, int8 (GDN_CODE_INT8) or e4m3 (GDN_CODE_E4M3);
+ *                    a value is code * scale.  16-byte aligned.  page_size is 16, 32, 64 or 128.
+ *   k_scale, v_scale [num_pages, Hkv]  f32, >= 0
+ *   block_table      [B, max_pages]    int32, device: page i of a sequence holds its tokens i * page_size ..
+ *   seq_lens         [B]               int32 / int64, device: tokens of each sequence, counting the call's
+ *                                      new ones; 0 for an unused row of a padded batch
+ *
+ * gdn_cache_append writes the new k, v rows [T, Hkv, 128] bf16, packed by cu_seqlens [B+1]: the n rows of
+ * sequence b become its last n tokens.  With m = 127 (int8) or 448 (e4m3), every page written to gets
+ *   scale = max(scale before, max |x| / m)     (from 0 if the page's first token is among the new ones)
+ * its older tokens are re-encoded if the scale grew, and codes are round(x / scale), ties to even, IEEE
+ * fp32 quotients.  Infinities become the largest code and a NaN a NaN (e4m3) or 0 (int8); neither enters
+ * the scale.  Rows before position 0 (seq_lens shorter than the rows given), beyond max_pages * page_size
+ * or in a page outside the cache are dropped.  Two sequences must not write to one page in one call.
+ *
+ * gdn_cache_attend: q [B, Q, Hq, 128] bf16 holds the last Q tokens of every sequence (Q = 1: the decode
+ * step), already appended; Hq is a multiple of Hkv and q head h reads kv head h / (Hq / Hkv).  Row i sees
+ * positions j < seq_len - Q + 1 + i; a row that sees none gets zeros.  out [B, Q, Hq, 128] bf16.  The
+ * workspace (256-byte aligned, at least gdn_cache_attend_workspace_bytes) carries nothing between calls;
+ * calls that can overlap need one each.  Its first int receives 0 or a GDN_DEVSTATUS_* code.
+ * flags must be 0.
+ */
+#define GDN_CODE_INT8 0
+#define GDN_CODE_E4M3 1
+int gdn_cache_append(const void* k, const void* v, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                     int code, const int* block_table, const void* seq_lens, int len_is_int64, const void* cu_seqlens,
+                     int cu_is_int64, int num_pages, int page_size, int max_pages, int B, int T, int Hkv, int D,
+                     void* stream, unsigned flags);
+size_t gdn_cache_attend_workspace_bytes(void);
+int gdn_cache_attend(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                     int code, const int* block_table, const void* seq_lens, int len_is_int64, int num_pages,
+                     int page_size, int max_pages, int B, int Q, int Hq, int Hkv, int D, float scale, void* out,
+                     void* workspace, size_t workspace_bytes, void* stream, unsigned flags);
 
 /* Human-readable name of a status code (static storage). */
 const char* gdn_status_string(int status);
