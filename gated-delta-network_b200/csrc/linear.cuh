@@ -34,19 +34,21 @@ struct LinearPrefillArgs {
     float scale;
     uint16_t* out;         // [T, HV, 128]
     float* new_state;      // [N, HV, 128, 128] (may alias state)
-    int m;                 // chunks per segment
-    int slots;             // work items per v-head: T / (64 m) + N
-    int states;            // state slots: 2 (T / (64 m))
-    int cut;               // a sequence can be longer than one segment: build and chain segment states
+    int ctas;              // stretches of the line of chunks, one per SM
+    int min_share;         // chunks of a stretch, at least
+    int keep;              // segments of at most this many chunks are not cut
+    int cut;               // a sequence can be longer than that: build and chain segment states
     int* status;           // workspace: first error code of a bounded wait
-    float* gamma;          // workspace: [states][HV] product of a segment's decays
-    float* seg;            // workspace: [states][HV][128 V][128 K] what a segment adds to the state, then
-                           //            (after the chain) the state at its end
+    int* kind;             // workspace: [ctas] what the stretch's last segment does: see the kernel
+    float* gamma;          // workspace: [ctas] product of its decays there
+    float* seg;            // workspace: [2 ctas][128 V][128 K] what it adds to the state, then (after the chain) the state
+                           //            at the stretch's end; behind them the initial states
 };
+constexpr int kLinearCtas = 148;
 
 struct LinearPrefillLayout {
-    int m, slots, states, cut;
-    size_t off_status, off_gamma, off_seg, total;
+    int min_share, keep, cut;
+    size_t off_status, off_kind, off_gamma, off_seg, total;
 };
 LinearPrefillLayout linear_prefill_layout(int N, int T, int HV);
 

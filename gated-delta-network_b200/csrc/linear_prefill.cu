@@ -4,17 +4,23 @@
 // C = 64 tokens with G_i = a_1 + .. + a_i and the state S_0 at its start:
 //   o_i = scale (e^{G_i} S_0 q_i + sum_{j <= i} e^{G_i - G_j} (q_i . k_j) v_j)
 //   S_C = e^{G_C} S_0 + sum_j (e^{G_C - G_j} v_j) k_j^T
-// All products run on tcgen05 with the V dimension as the M = 128 rows, so no accumulator row is wasted on
-// a 64-token chunk:
+// Four tcgen05 products a chunk, the V dimension as the 128 rows:
 //   QK  [Q; K] (128 x 128, K-major) x K (64 tokens)            -> rows 0-63: q_i . k_j
-//   OI  S_0 (128 V x 128 K, bf16)   x Q (64 tokens)            -> S_0 q_i, scaled by e^{G_i} in the epilogue
+//   U   Vd^T (128 V x 64 tokens, A from TMEM) x K (128 K)      -> what the chunk adds to the state
 //   OA  V^T (128 V x 64 tokens, MN-major from the v tile) x P  -> P = decayed, causal QK in bf16
-//   U   Vd^T (128 V x 64 tokens) x K (128 K)                   -> Vd = decayed v as bf16 hi + lo
-// The state stays in fp32 registers; hi + lo keeps what a chunk adds to it at 2^-17 relative.
+//   OI  S_0 (128 V x 128 K, A from TMEM) x Q (64 tokens)       -> S_0 q_i, scaled by e^{G_i} in the epilogue
+// The state stays in fp32 registers (one V row a thread); its bf16 copy for OI and P round to 2^-8, as the output
+// does.  The decayed v is cut into three bf16 parts that keep all 24 bits, so the state is as exact as an fp32 sum.
 //
-// The update does not read the state, so a long sequence is cut into segments of m chunks: a first launch
-// builds what every segment but the last adds to the state (U alone), a second one chains the segments, and
-// the output launch runs all segments side by side.
+// Bound by HBM (1 KB a token and head), then by shared-memory bandwidth: operands that a thread forms anyway (S_0,
+// Vd) go to TMEM, which takes 128 KB a chunk off it.  Every product and every group of warps works on a
+// chunk of its own: TMA and gates run ahead, the P and V warps prepare chunk c + 1 while the tensor core works on c
+// and the output warps write c - 1; only h <- e^{G_C} h + U and the product OI form a chain over chunks.
+//
+// Tokens are cut evenly over the CTAs whatever the lengths: all (sequence, v-head) segments lie on one line in
+// chunks, and a CTA takes an equal stretch of it.  The state at a stretch's start comes from two launches before:
+// what every unfinished segment adds to the state in its CTA (U alone; it does not read the state), and a chain over
+// those sums.  Stretches end at segment ends where segments are short, so such calls need one launch.
 #include <algorithm>
 
 #include "linear.cuh"
@@ -25,65 +31,145 @@ namespace gdn {
 
 namespace lin {
 constexpr int C = 64;
-constexpr int kThreads = 288;  // 8 math warps + 1 TMA warp
-constexpr int kMath = 256;
-constexpr int kStages = 2;
+constexpr int kThreads = 768;  // 6 warpgroups: {TMA, MMA, gates, -}, P, V, V, O, S
+constexpr int kStages = 3;
+constexpr int kGates = 8;
 // stage: [Q0 | K0 | Q1 | K1 | V0 | V1], each 64 tokens x 64 columns bf16, SWIZZLE_128B
 constexpr uint32_t kOffQ = 0, kOffK = 8192, kAtom = 16384, kOffV = 32768;
 constexpr uint32_t kStage = 49152;
-constexpr uint32_t kOffS = kStages * kStage;     // bf16 state [128 V][128 K]: two 64-column atoms of 16 KB
-constexpr uint32_t kOffVh = kOffS + 32768;       // decayed v, hi then lo: two atoms of 64 tokens x 128 B each
-constexpr uint32_t kOffVl = kOffVh + 16384;
-constexpr uint32_t kOffP = kOffVl + 16384;       // P [64 i][64 j] bf16
-constexpr uint32_t kOffO = kOffP + 8192;         // output staging [64 tokens][128 V] bf16, 16-byte chunks swizzled
-constexpr uint32_t kOffG = kOffO + 16384;        // f32 [64] G log2(e) | [64] e^G | [64] e^{G_C - G} | e^{G_C}
-constexpr uint32_t kOffBar = kOffG + 1024;
-constexpr uint32_t kSmem = kOffBar + 128 + 1024;
+constexpr uint32_t kOffP = kStages * kStage;     // P [2][64 i][64 j] bf16
+constexpr uint32_t kOffO = kOffP + 2 * 8192;     // output staging [2][2 atoms][64 tokens][64 V] bf16, SWIZZLE_128B
+constexpr uint32_t kOffG = kOffO + 2 * 16384;    // gates, kGates slots of f32: [64] G log2(e) | [64] scale e^G | [64] e^{G_C - G} | e^{G_C}
+constexpr uint32_t kGateFloats = 256;
+constexpr uint32_t kOffBar = kOffG + kGates * kGateFloats * 4;
+constexpr uint32_t kOffRange = kOffBar + 512;
+constexpr uint32_t kSmem = kOffRange + 256 + 1024;
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColP = 0, kColI = 64, kColA = 128, kColU = 192;
+// accumulators QK, OI, OA and the state S in fp32, then its bf16 copy and the three parts of the decayed v
+constexpr uint32_t kColQK = 0, kColI = 64, kColA = 128, kColS = 192, kColB = 320, kColV = 384;
 static_assert(kSmem <= 227 * 1024, "shared memory");
 
 constexpr float kLog2e = 1.4426950408889634f;
 // Log decays are clamped here: e^-110 is below every fp32 number, and -infinity would turn the differences
 // of prefix sums into NaN.
 constexpr float kMinDecay = -110.f;
+
+struct Bars {
+    uint64_t full[kStages], empty[kStages], g_full[kGates], g_empty[kGates];
+    uint64_t qk_full, qk_empty, p_full[2], p_empty[2], v_full, u_full, s_full, i_full, o_full, o_empty, done;
+    uint32_t tmem;
+};
+static_assert(sizeof(Bars) <= 512, "barriers");
 }  // namespace lin
 
 struct LinearMaps {
-    CUtensorMap q, k, v;  // (128, heads, T) bf16, box 64 x 1 x 64, SWIZZLE_128B
+    CUtensorMap q, k, v, o;  // (128, heads, T) bf16, box 64 x 1 x 64, SWIZZLE_128B
 };
 
-// Work items: sequence n owns the slots from cu[n] / len + n on (len = 64 m tokens), at least as many as it has
-// segments, and one if it is empty.  What its segments add to the state lies in the state slots from
-// 2 (cu[n] / len) on: a sequence of more than one segment has at most 2 floor(tokens / len) of them.  Neither needs
-// a prefix sum over the sequences, only a search for the owner.
-__device__ __forceinline__ int seq_start(const LinearPrefillArgs& p, int n) {
+// ---- the line of chunks ---------------------------------------------------------------------
+struct Mark {  // a place on the line: chunk `chunk` of (sequence n, v-head hv)
+    int n, hv, chunk, pos;
+};
+struct LinRange {
+    int sum[lin::kThreads / 32];
+    Mark at[2];  // the CTA's stretch
+};
+static_assert(sizeof(LinRange) <= 256, "range");
+
+__device__ __forceinline__ int lin_chunks(const LinearPrefillArgs& p, int n) {
     int s, e;
     seq_bounds(p.cu, p.cu64, n, p.T, s, e);
-    return s;
+    return max(1, (e - s + lin::C - 1) / lin::C);  // an empty sequence has a place too: its state is copied
 }
-struct SegItem {
-    int n, seg, nsegs, t0, t1, state0;  // tokens [t0, t1) of segment `seg` of sequence n (n < 0: none); its first state slot
-};
-__device__ __forceinline__ SegItem find_segment(const LinearPrefillArgs& p, int slot, int per_seq, int per_len) {
-    const int len = lin::C * p.m;
-    int lo = 0, hi = p.N - 1;  // the last sequence whose first slot, per_len (cu[n] / len) + per_seq n, is <= slot
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (per_len * (seq_start(p, mid) / len) + per_seq * mid <= slot) lo = mid;
-        else hi = mid - 1;
+
+// The stretch of CTA blockIdx.x.  All threads of the CTA take part; the result is in r->at.  (Positions are ints: the
+// entry point refuses calls of 2^31 chunks.)
+__device__ __forceinline__ void find_range(const LinearPrefillArgs& p, LinRange* r) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    int total = 0, want[2] = {0, 0};
+#pragma unroll 1
+    for (int round = 0; round < 2; ++round) {  // the sum of all lengths, then the two ends
+        int before = 0;  // chunks of the sequences in front of this pass
+#pragma unroll 1
+        for (int base = 0; base < p.N; base += blockDim.x) {
+            const int n = base + tid;
+            const int nc = n < p.N ? lin_chunks(p, n) : 0;
+            int x = nc;
+#pragma unroll 1
+            for (int off = 1; off < 32; off <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, off);
+                if (lane >= off) x += y;
+            }
+            __syncthreads();
+            if (lane == 31) r->sum[warp] = x;
+            __syncthreads();
+            int pass = 0;
+#pragma unroll 1
+            for (int w = 0; w < warps; ++w) {
+                if (w < warp) x += r->sum[w];
+                pass += r->sum[w];
+            }
+            const int lo = (before + x - nc) * p.HV;
+            if (round == 1) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int off = want[i] - lo;
+                    if (off >= 0 && off < nc * p.HV) {
+                        Mark m;
+                        m.n = n;
+                        m.hv = off / nc;
+                        m.chunk = off - m.hv * nc;
+                        m.pos = want[i];
+                        if (nc <= p.keep && m.chunk) {  // a short segment is not cut: to its nearer end
+                            const int up = 2 * m.chunk >= nc;
+                            m.pos += up ? nc - m.chunk : -m.chunk;
+                            m.chunk = 0;
+                            m.hv += up;
+                            if (m.hv == p.HV) {
+                                m.hv = 0;
+                                ++m.n;
+                            }
+                        }
+                        r->at[i] = m;
+                    }
+                }
+            }
+            before += pass;
+        }
+        if (round == 0) {
+            total = before * p.HV;
+            const int ctas = max(1, min(p.ctas, total / p.min_share)), per = total / ctas, more = total - per * ctas;
+            const int c = blockIdx.x;
+            want[0] = min(total, c * per + min(c, more));
+            want[1] = min(total, (c + 1) * per + min(c + 1, more));
+            if (tid < 2 && want[tid] == total) r->at[tid] = Mark{p.N, 0, 0, total};
+        }
     }
-    SegItem it;
-    int s, e;
-    seq_bounds(p.cu, p.cu64, lo, p.T, s, e);
-    it.nsegs = max(1, (e - s + len - 1) / len);
-    it.seg = slot - (per_len * (s / len) + per_seq * lo);
-    it.n = (it.seg >= 0 && it.seg < it.nsegs) ? lo : -1;  // also where cu_seqlens is not non-decreasing
-    it.t0 = s + it.seg * len;
-    it.t1 = min(e, it.t0 + len);
-    it.state0 = 2 * (s / len);
-    return it;
+    __syncthreads();
 }
+
+struct Piece {
+    int n, hv, s, e, ca, cb, nc;  // chunks [ca, cb) of the nc of segment (n, hv), tokens [s, e)
+};
+struct Walk {
+    int n, hv, chunk, left;
+    __device__ __forceinline__ bool next(const LinearPrefillArgs& p, Piece& x) {
+        if (left <= 0 || n >= p.N) return false;
+        x.n = n;
+        x.hv = hv;
+        seq_bounds(p.cu, p.cu64, n, p.T, x.s, x.e);
+        x.nc = max(1, (x.e - x.s + lin::C - 1) / lin::C);
+        x.ca = chunk;
+        x.cb = min(x.nc, chunk + left);
+        left -= x.cb - x.ca;
+        chunk = 0;
+        if (++hv == p.HV) {
+            hv = 0;
+            ++n;
+        }
+        return true;
+    }
+};
 
 __device__ __forceinline__ void zero_rows(const LinearPrefillArgs& p, int tid, int nthreads) {
     int lo, tmp, hi;
@@ -96,335 +182,698 @@ __device__ __forceinline__ void zero_rows(const LinearPrefillArgs& p, int tid, i
     for (size_t i = (size_t)hi * row_words + tid; i < (size_t)p.T * row_words; i += nthreads) o4[i] = make_uint4(0, 0, 0, 0);
 }
 
-// kOut: the output launch.  Otherwise the segment launch: what each segment but a sequence's last adds to the state.
+// ---- small pieces ---------------------------------------------------------------------------
+__device__ __forceinline__ float lin_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The MMA warp stays convergent and one elected lane issues by predicate: descriptors then live in uniform
+// registers, where a branch to one lane had each of them moved there per instruction (280 cycles a product step).
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r;
+}
+// Shared-memory descriptors as (low, high) words: the high one (stride 1024, SWIZZLE_128B) is the same for all.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t lbo_bytes) { return ((saddr >> 4) & 0x3fffu) | ((lbo_bytes >> 4) << 16); }
+template <bool kAccumulate>
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t dtmem, uint32_t adesc, uint32_t bdesc, uint32_t idesc) {
+    asm volatile(
+        "{\n.reg .pred p, e;\n.reg .b64 a, b;\nmov.b64 a, {%1, %6};\nmov.b64 b, {%2, %6};\nsetp.ne.b32 e, %5, 0;\n"
+        "setp.ne.b32 p, %4, 0;\n@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(dtmem),
+        "r"(adesc), "r"(bdesc), "r"(idesc), "n"(kAccumulate ? 1 : 0), "r"(one), "n"(kDescHigh)
+        : "memory");
+}
+// A from TMEM (K-major, two bf16 a column)
+template <bool kAccumulate>
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t dtmem, uint32_t atmem, uint32_t bdesc, uint32_t idesc) {
+    asm volatile(
+        "{\n.reg .pred p, e;\n.reg .b64 b;\nmov.b64 b, {%2, %6};\nsetp.ne.b32 e, %5, 0;\n"
+        "setp.ne.b32 p, %4, 0;\n@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(dtmem),
+        "r"(atmem), "r"(bdesc), "r"(idesc), "n"(kAccumulate ? 1 : 0), "r"(one), "n"(kDescHigh)
+        : "memory");
+}
+__device__ __forceinline__ void commit_one(uint32_t one, uint64_t* bar) {
+    asm volatile(
+        "{\n.reg .pred e;\nsetp.ne.b32 e, %1, 0;\n@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(
+            smem_u32(bar)),
+        "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// 16 lanes x 32 columns: register 2 i (2 i + 1) of thread t is lane t / 4 (+ 8), column 4 i + t % 4.
+__device__ __forceinline__ void tmem_st_16x128b_x8(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// 16 lanes x 32 columns: registers 4 i + {0, 1} ({2, 3}) of thread t are lane t / 4 (+ 8), columns 8 i + 2 (t % 4) + {0, 1}.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+// Four 8 x 8 blocks: register i of thread t holds (row t / 4, columns 2 (t % 4) + {0, 1}) of block i, lane 8 i + r gives
+// the address of its row r.
+__device__ __forceinline__ void stsm_x4(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
+}
+// Four 8 x 8 blocks, each stored transposed: register i of thread t holds (row t / 4, columns 2 (t % 4) + {0, 1}) of
+// block i, lane 8 i + c gives the address of its column c.
+__device__ __forceinline__ void stsm_x4_t(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
+                 : "memory");
+}
+__device__ __forceinline__ float2 bf2_to_f2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+
+// Bounded wait of a whole warp, which leaves it together (the vote makes the outcome uniform).  Kept short, it is
+// there 25 times: the clock is looked at every 1024 tries only, and the caller reports.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .u32 n;\n.reg .u64 t, e;\n"
+        "mov.u32 n, 0;\nmov.u64 e, 0;\n"
+        "LOOP:\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n@p bra DONE;\n"
+        "add.u32 n, n, 1;\nand.b32 %0, n, 1023;\nsetp.ne.u32 p, %0, 0;\n@p bra LOOP;\n"
+        "mov.u64 t, %%globaltimer;\nsetp.eq.u64 p, e, 0;\n@p add.u64 e, t, %3;\n"
+        "setp.lt.u64 p, t, e;\n@p bra LOOP;\n"  // falls through with p false: gave up
+        "DONE:\n"
+        "selp.u32 %0, 1, 0, p;\n}\n"
+        : "=&r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "n"(kWaitLimitNs)
+        : "memory");
+    return __all_sync(0xffffffffu, ok);
+}
+
+struct LinCtx {
+    unsigned char* sm;
+    uint32_t sbase;
+    static constexpr uint32_t tmem = 0;  // a CTA that holds all 512 columns holds them from column 0
+    lin::Bars* b;
+    Walk walk;
+    int prev;  // the CTA's slot of segment states is blockIdx.x; a stretch that begins inside a segment starts from `prev`
+};
+
+// ---- roles ----------------------------------------------------------------------------------
+// Every wait is bounded; on expiry the role returns false, and the others' waits expire in turn.
+#define LIN_WAIT(bar, parity) \
+    if (!warp_wait(&(bar), (uint32_t)(parity) & 1u)) return false
+
+// Warp 0: the TMA copies.
+template <bool kOut>
+__device__ __forceinline__ bool role_load(const LinearPrefillArgs& p, const LinearMaps& maps, const LinCtx& x, uint32_t one, int* issued) {
+    using namespace lin;
+    Walk w = x.walk;
+    Piece pc;
+    int s = 0, s_ph = 1;
+#pragma unroll 1
+    while (w.next(p, pc)) {
+        if (pc.e <= pc.s) continue;
+        const int hq = pc.hv / (p.HV / p.H);
+#pragma unroll 1
+        for (int c = pc.ca; c < pc.cb; ++c) {
+            const int t0 = pc.s + c * C;
+            LIN_WAIT(x.b->empty[s], s_ph);  // (the first round passes: the barriers are new)
+            if (one) {
+                unsigned char* st = x.sm + s * kStage;
+                mbar_arrive_expect_tx(&x.b->full[s], kOut ? 49152 : 32768);
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    if (kOut) tma_load_3d(st + kOffQ + a * kAtom, &maps.q, 64 * a, hq, t0, &x.b->full[s]);
+                    tma_load_3d(st + kOffK + a * kAtom, &maps.k, 64 * a, hq, t0, &x.b->full[s]);
+                    tma_load_3d(st + kOffV + a * 8192, &maps.v, 64 * a, pc.hv, t0, &x.b->full[s]);
+                }
+            }
+            __syncwarp();
+            ++*issued;
+            if (++s == kStages) {
+                s = 0;
+                s_ph ^= 1;
+            }
+        }
+    }
+    return true;
+}
+
+// Warp 2: prefix and suffix sums of every chunk's log decays, two tokens a lane.
+__device__ __forceinline__ bool role_gates(const LinearPrefillArgs& p, const LinCtx& x) {
+    using namespace lin;
+    const int lane = threadIdx.x & 31;
+    Walk w = x.walk;
+    Piece pc;
+    int g = 0;
+#pragma unroll 1
+    while (w.next(p, pc)) {
+        if (pc.e <= pc.s) continue;
+#pragma unroll 1
+        for (int c = pc.ca; c < pc.cb; ++c, ++g) {
+            const int t0 = pc.s + c * C, L = min(C, pc.e - t0);
+            float a0 = 0.f, a1 = 0.f;
+            if (2 * lane < L) a0 = p.decay[p.per_token ? (size_t)(t0 + 2 * lane) * p.HV + pc.hv : pc.hv];
+            if (2 * lane + 1 < L) a1 = p.decay[p.per_token ? (size_t)(t0 + 2 * lane + 1) * p.HV + pc.hv : pc.hv];
+            a0 = a0 < kMinDecay ? kMinDecay : a0;
+            a1 = a1 < kMinDecay ? kMinDecay : a1;
+            float pre = a0 + a1, suf = a0 + a1;
+#pragma unroll 1
+            for (int off = 1; off < 32; off <<= 1) {
+                const float y = __shfl_up_sync(0xffffffffu, pre, off), z = __shfl_down_sync(0xffffffffu, suf, off);
+                if (lane >= off) pre += y;
+                if (lane + off < 32) suf += z;
+            }
+            float before = __shfl_up_sync(0xffffffffu, pre, 1), after = __shfl_down_sync(0xffffffffu, suf, 1);
+            if (lane == 0) before = 0.f;
+            if (lane == 31) after = 0.f;
+            // the last group to finish chunk g - 7 has finished g - 8 for all the others: the slot is free
+            if (g >= kGates) LIN_WAIT(x.b->g_empty[(g + 1) % kGates], (g + 1) / kGates - 1);
+            float* gt = reinterpret_cast<float*>(x.sm + kOffG) + (g % kGates) * kGateFloats;
+            const float g0 = before + a0;
+            *reinterpret_cast<float2*>(gt + 2 * lane) = make_float2(g0 * kLog2e, pre * kLog2e);
+            *reinterpret_cast<float2*>(gt + 64 + 2 * lane) = make_float2(p.scale * lin_ex2(g0 * kLog2e), p.scale * lin_ex2(pre * kLog2e));
+            // e^{G_C - G_j} from the sum of the later decays: exact where it matters, near the chunk's end
+            *reinterpret_cast<float2*>(gt + 128 + 2 * lane) = make_float2(expf(after + a1), expf(after));
+            if (lane == 31) gt[192] = expf(pre);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&x.b->g_full[g % kGates]);
+        }
+    }
+    return true;
+}
+
+// Warp 1: all tensor-core products.
+template <bool kOut>
+__device__ __forceinline__ bool role_mma(const LinearPrefillArgs& p, const LinCtx& x, uint32_t one) {
+    using namespace lin;
+    Walk w = x.walk;
+    Piece pc;
+    int total = 0;
+#pragma unroll 1
+    while (w.next(p, pc))
+        if (pc.e > pc.s) total += pc.cb - pc.ca;
+    total = __shfl_sync(0xffffffffu, total, 0);
+    constexpr uint32_t idesc_qk = umma_idesc_bf16(64, 64, false, false), idesc_oi = umma_idesc_bf16(128, 64, false, false);
+    constexpr uint32_t idesc_oa = umma_idesc_bf16(128, 64, true, false), idesc_u = umma_idesc_bf16(128, 128, false, true);
+    // descriptors at stage 0; an offset adds its sixteenth
+    const uint32_t d_q = desc_low(x.sbase + kOffQ, 16), d_k = desc_low(x.sbase + kOffK, 16);
+    const uint32_t d_ku = desc_low(x.sbase + kOffK, kAtom), d_v = desc_low(x.sbase + kOffV, 8192), d_p = desc_low(x.sbase + kOffP, 16);
+    auto step = [](int kk) { return (uint32_t)(((kk >> 2) * kAtom + (kk & 3) * 32) >> 4); };  // 16 of 128 columns
+    auto qk = [&](uint32_t st) {
+        mma_ss<false>(one, x.tmem + kColQK, d_q + st, d_k + st, idesc_qk);
+#pragma unroll
+        for (int kk = 1; kk < 8; ++kk) mma_ss<true>(one, x.tmem + kColQK, d_q + st + step(kk), d_k + st + step(kk), idesc_qk);
+        commit_one(one, &x.b->qk_full);
+    };
+    int s = 0, s_ph = 0;  // stage of chunk g and its phase
+    const uint32_t kStep = kStage >> 4;
+    if (total > 0) LIN_WAIT(x.b->full[0], 0);
+    tc_fence_after();
+    if (kOut && total > 0) qk(0);
+#pragma unroll 1
+    for (int g = 0; g < total; ++g) {
+        const uint32_t st = (uint32_t)s * kStep, ph = g & 1;
+        const int sn = s + 1 == kStages ? 0 : s + 1, sn_ph = sn ? s_ph : s_ph ^ 1;
+        LIN_WAIT(x.b->v_full, ph);
+        LIN_WAIT(x.b->s_full, ph);
+        tc_fence_after();
+        // the chain over chunks goes through this product: it is issued first
+#pragma unroll
+        for (int kk = 0; kk < 12; ++kk) mma_ts<true>(one, x.tmem + kColS, x.tmem + kColV + 8 * kk, d_ku + st + 128 * (kk & 3), idesc_u);
+        commit_one(one, &x.b->u_full);
+        if (kOut) {
+            if (g > 0) LIN_WAIT(x.b->o_empty, ph ^ 1);
+            tc_fence_after();
+            mma_ts<false>(one, x.tmem + kColI, x.tmem + kColB, d_q + st, idesc_oi);
+#pragma unroll
+            for (int kk = 1; kk < 8; ++kk) mma_ts<true>(one, x.tmem + kColI, x.tmem + kColB + 8 * kk, d_q + st + step(kk), idesc_oi);
+            commit_one(one, &x.b->i_full);
+            LIN_WAIT(x.b->p_full[ph], g >> 1);
+            tc_fence_after();
+            const uint32_t pb = d_p + ph * 512u;
+            mma_ss<false>(one, x.tmem + kColA, d_v + st, pb, idesc_oa);
+#pragma unroll
+            for (int kk = 1; kk < 4; ++kk) mma_ss<true>(one, x.tmem + kColA, d_v + st + 128 * kk, pb + 2 * kk, idesc_oa);
+            commit_one(one, &x.b->p_empty[ph]);
+            commit_one(one, &x.b->o_full);
+        }
+        commit_one(one, &x.b->empty[s]);
+        if (g + 1 < total) {
+            LIN_WAIT(x.b->full[sn], sn_ph);
+            if (kOut) {
+                LIN_WAIT(x.b->qk_empty, ph);
+                tc_fence_after();
+                qk((uint32_t)sn * kStep);
+            }
+        }
+        s = sn;
+        s_ph = sn_ph;
+    }
+    return true;
+}
+
+// Warps 4-7: P, 16 rows a warp (a 64-row accumulator has its rows in the first 16 lanes of every quarter).  Blocks above
+// the diagonal stay the zeros that the kernel starts with.
+__device__ __forceinline__ bool role_p(const LinearPrefillArgs& p, const LinCtx& x) {
+    using namespace lin;
+    const int lane = threadIdx.x & 31, quarter = __shfl_sync(0xffffffffu, (threadIdx.x >> 5) & 3, 0);
+    const uint32_t tl = x.tmem + kColQK + ((uint32_t)(32 * quarter) << 16);
+    const int r = 16 * quarter + (lane >> 2);  // and r + 8
+    // stmatrix rows: P row (lane % 16), 16-byte chunk lane / 16 of a block of 16 columns
+    const uint32_t row = x.sbase + kOffP + (uint32_t)(16 * quarter + (lane & 15)) * 128, sw = lane & 7;
+    Walk w = x.walk;
+    Piece pc;
+    int g = 0;
+#pragma unroll 1
+    while (w.next(p, pc)) {
+        if (pc.e <= pc.s) continue;
+#pragma unroll 1
+        for (int c = pc.ca; c < pc.cb; ++c, ++g) {
+            const int L = min(C, pc.e - pc.s - c * C);
+            const float* g2 = reinterpret_cast<const float*>(x.sm + kOffG) + (g % kGates) * kGateFloats;
+            LIN_WAIT(x.b->g_full[g % kGates], g / kGates);
+            const float2 gi = make_float2(g2[r], g2[r + 8]);
+            LIN_WAIT(x.b->qk_full, g);
+            tc_fence_after();
+            uint32_t d[2][16];
+            tmem_ld_16x256b_x4(tl, d[0]);
+            tmem_ld_16x256b_x4(tl + 32, d[1]);
+            tmem_ld_wait();
+            tmem_regs_ready_n(d[0]);
+            tmem_regs_ready_n(d[1]);
+            tc_fence_before();
+            mbar_arrive(&x.b->qk_empty);
+            if (g >= 2) LIN_WAIT(x.b->p_empty[g & 1], (g >> 1) - 1);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {  // 16 columns
+                if (b > quarter) break;
+                uint32_t o[4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {  // 8 columns
+                    const float2 gj = *reinterpret_cast<const float2*>(g2 + 16 * b + 8 * i + 2 * (lane & 3));
+                    const int j = 16 * b + 8 * i + 2 * (lane & 3);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {  // rows r, r + 8
+                        const float gr = k ? gi.y : gi.x;
+                        const uint32_t* e = &d[b >> 1][8 * (b & 1) + 4 * i + 2 * k];
+                        const float y = __uint_as_float(e[0]) * lin_ex2(gr - gj.x), z = __uint_as_float(e[1]) * lin_ex2(gr - gj.y);
+                        const int lim = min(r + 8 * k, L - 1);
+                        o[2 * i + k] = pack_bf16x2(j <= lim ? y : 0.f, j + 1 <= lim ? z : 0.f);
+                    }
+                }
+                stsm_x4(row + (uint32_t)(g & 1) * 8192 + ((((uint32_t)(2 * b) + (lane >> 4)) ^ sw) << 4), o[0], o[1], o[2], o[3]);
+            }
+            fence_async_smem();
+            mbar_arrive(&x.b->p_full[g & 1]);
+        }
+    }
+    return true;
+}
+
+// Warps 8-15: the decayed v, transposed, as three bf16 parts in TMEM (lane = V index, two tokens a column); 16 V a warp.
+template <bool kOut>
+__device__ __forceinline__ bool role_v(const LinearPrefillArgs& p, const LinCtx& x) {
+    using namespace lin;
+    const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3, hf = (threadIdx.x >> 7) - 2, tid = threadIdx.x - 256;
+    const uint32_t tl = x.tmem + kColV + ((uint32_t)(32 * quarter + 16 * hf) << 16);
+    // ldmatrix rows: token (lane % 8) + 8 (lane / 16), 16-byte chunk of 8 V
+    const int tok = (lane & 7) + 8 * (lane >> 4), ch = 4 * quarter + 2 * hf + ((lane >> 3) & 1);
+    const uint32_t from = kOffV + (uint32_t)(ch >> 3) * 8192 + (uint32_t)tok * 128 + (uint32_t)(((ch & 7) ^ (tok & 7)) << 4);
+    Walk w = x.walk;
+    Piece pc;
+    int g = 0;
+#pragma unroll 1
+    while (w.next(p, pc)) {
+        if (pc.e <= pc.s) continue;
+#pragma unroll 1
+        for (int c = pc.ca; c < pc.cb; ++c, ++g) {
+            const int L = min(C, pc.e - pc.s - c * C);
+            const float* er = reinterpret_cast<const float*>(x.sm + kOffG) + (g % kGates) * kGateFloats + 128 + 2 * (lane & 3);
+            LIN_WAIT(x.b->g_full[g % kGates], g / kGates);
+            LIN_WAIT(x.b->full[g % kStages], g / kStages);
+            unsigned char* st = x.sm + (g % kStages) * kStage;
+            if (L < C) {
+                // Rows behind the segment's end hold another sequence's tokens, or zeros.  They become zero in v and
+                // k, so whatever they hold cannot reach a product.
+                for (int i = tid; i < (C - L) * 16; i += 256) {
+                    const uint32_t off = (uint32_t)(L + (i >> 4)) * 128 + (i & 7) * 16;
+                    *reinterpret_cast<uint4*>(st + kOffV + ((i >> 3) & 1) * 8192 + off) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(st + kOffK + ((i >> 3) & 1) * kAtom + off) = make_uint4(0, 0, 0, 0);
+                }
+                fence_async_smem();
+                named_bar_sync(1, 256);
+            }
+            uint32_t part[3][16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // 16 V x 16 tokens, transposed
+                uint32_t raw[4];
+                ldsm_x4_t(raw[0], raw[1], raw[2], raw[3], st + from + 2048 * i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {  // {0, 1}: tokens 16 i + .., {2, 3}: 8 later; odd ones are 8 V further
+                    float2 y = mul2(bf2_to_f2(raw[j]), *reinterpret_cast<const float2*>(er + 16 * i + 8 * (j >> 1)));
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) {
+                        part[k][4 * i + j] = pack_bf16x2(y.x, y.y);
+                        if (k < 2) y = sub2(y, bf2_to_f2(part[k][4 * i + j]));
+                    }
+                }
+            }
+            if (g > 0) LIN_WAIT(x.b->u_full, g - 1);  // the parts of the chunk before are consumed
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < 3; ++k) tmem_st_16x128b_x8(tl + 32 * k, part[k]);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&x.b->v_full);
+        }
+    }
+    return true;
+}
+
+// Warps 16-19: o = scale (e^{G_i} OI + OA), transposed into shared memory; whole chunks leave by TMA.
+__device__ __forceinline__ bool role_o(const LinearPrefillArgs& p, const LinearMaps& maps, const LinCtx& x) {
+    using namespace lin;
+    const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3, r = threadIdx.x & 127;
+    const uint32_t tl = x.tmem + ((uint32_t)(32 * quarter) << 16);
+    // stmatrix rows: token (lane % 8) + 8 (lane / 16), 16-byte chunk of 8 V
+    const uint32_t to = x.sbase + kOffO + (uint32_t)(quarter >> 1) * 8192 + (uint32_t)((lane & 7) + 8 * (lane >> 4)) * 128;
+    const uint32_t ch = 4 * (quarter & 1) + ((lane >> 3) & 1), sw = lane & 7;
+    Walk w = x.walk;
+    Piece pc;
+    int g = 0;
+#pragma unroll 1
+    while (w.next(p, pc)) {
+        if (pc.e <= pc.s) continue;
+#pragma unroll 1
+        for (int c = pc.ca; c < pc.cb; ++c, ++g) {
+            const int t0 = pc.s + c * C, L = min(C, pc.e - t0);
+            const float* eg = reinterpret_cast<const float*>(x.sm + kOffG) + (g % kGates) * kGateFloats + 64;
+            const uint32_t buf = (uint32_t)(g & 1) * 16384;
+            LIN_WAIT(x.b->g_full[g % kGates], g / kGates);
+            LIN_WAIT(x.b->o_full, g);
+            tc_fence_after();
+#pragma unroll 1
+            for (int th = 0; th < 2; ++th) {  // 32 tokens
+                float2 e2[4];  // tokens 8 i + 2 (lane % 4) and the next
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e2[i] = *reinterpret_cast<const float2*>(eg + 32 * th + 8 * i + 2 * (lane & 3));
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {  // 16 V
+                    uint32_t y[16], z[16];
+                    const uint32_t ta = tl + ((uint32_t)(16 * hf) << 16) + 32 * th;
+                    tmem_ld_16x256b_x4(ta + kColI, y);
+                    tmem_ld_16x256b_x4(ta + kColA, z);
+                    tmem_ld_wait();
+                    tmem_regs_ready_n(y);
+                    tmem_regs_ready_n(z);
+                    uint32_t o[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {  // even: V row lane / 4, odd: 8 further
+                        const float2 v2 = fma2(e2[i >> 1], make_float2(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])),
+                                               mul2(make_float2(p.scale, p.scale), make_float2(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1]))));
+                        o[i] = pack_bf16x2(v2.x, v2.y);
+                    }
+                    const uint32_t at = to + buf + (32 * th) * 128 + (((ch + 2 * hf) ^ sw) << 4);
+                    stsm_x4_t(at, o[0], o[1], o[2], o[3]);
+                    stsm_x4_t(at + 16 * 128, o[4], o[5], o[6], o[7]);
+                }
+            }
+            tc_fence_before();
+            mbar_arrive(&x.b->o_empty);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&x.b->g_empty[g % kGates]);
+            if (r == 0) tma_store_wait_read();  // the chunk before has left its buffer, which the next one writes
+            named_bar_sync(2, 128);
+            if (L == C) {
+                if (r == 0) {
+                    tma_store_3d(&maps.o, 0, pc.hv, t0, x.sm + kOffO + buf);
+                    tma_store_3d(&maps.o, 64, pc.hv, t0, x.sm + kOffO + buf + 8192);
+                    tma_store_commit();
+                }
+            } else {  // rows behind the segment's end are not its own
+#pragma unroll 1
+                for (int q = r; q < L * 16; q += 128) {
+                    const int i = q >> 4, k = q & 15;
+                    *reinterpret_cast<uint4*>(p.out + ((size_t)(t0 + i) * p.HV + pc.hv) * kD + 8 * k) =
+                        *reinterpret_cast<const uint4*>(x.sm + kOffO + buf + (k >> 3) * 8192 + i * 128 + (((k & 7) ^ (i & 7)) << 4));
+                }
+                named_bar_sync(2, 128);  // nobody writes the other buffer, then this one, before it is read
+            }
+        }
+    }
+    if (r == 0) tma_store_wait_all();
+    return true;
+}
+
+// Warps 20-23: the state, V row r a thread.  It lives in TMEM, where U adds to it: before U of chunk g the warps read
+// it, leave its bf16 copy for OI and write it back times e^{G_C}.
+template <bool kOut>
+__device__ __forceinline__ bool role_s(const LinearPrefillArgs& p, const LinCtx& x) {
+    using namespace lin;
+    const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3, r = threadIdx.x & 127;
+    const uint32_t tl = x.tmem + ((uint32_t)(32 * quarter) << 16);
+    Walk w = x.walk;
+    Piece pc;
+    int g = 0;
+#pragma unroll 1
+    while (w.next(p, pc)) {
+        const size_t at = ((size_t)pc.n * p.HV + pc.hv) * kD * kD;
+        const float* src = nullptr;
+        if (kOut) {
+            if (pc.ca > 0)
+                src = p.seg + (size_t)x.prev * kD * kD;
+            else if (p.state)
+                src = pc.cb < pc.nc ? p.seg + (size_t)(p.ctas + blockIdx.x) * kD * kD : p.state + at;
+        }
+        float* dst = kOut ? p.new_state + at : p.seg + (size_t)blockIdx.x * kD * kD;
+        const bool ends = !kOut || pc.cb == pc.nc;
+        if (pc.e <= pc.s) {  // an empty sequence keeps its state
+#pragma unroll 4
+            for (int j = r; j < kD * kD / 4; j += 128)
+                reinterpret_cast<float4*>(dst)[j] = src ? reinterpret_cast<const float4*>(src)[j] : make_float4(0.f, 0.f, 0.f, 0.f);
+            continue;
+        }
+        float gamma = 1.f;
+#pragma unroll 1
+        for (int c = pc.ca; c < pc.cb; ++c, ++g) {
+            const float* gt = reinterpret_cast<const float*>(x.sm + kOffG) + (g % kGates) * kGateFloats;
+            LIN_WAIT(x.b->g_full[g % kGates], g / kGates);
+            const float el = gt[192];
+            gamma *= el;
+            const bool begins = c == pc.ca;
+            if (g > 0) {
+                // the state is complete (or, at a segment's start, was read) and OI has read its copy
+                LIN_WAIT(x.b->u_full, g - 1);
+                if (kOut) LIN_WAIT(x.b->i_full, g - 1);
+            }
+            tc_fence_after();
+#pragma unroll 1
+            for (int b = 0; b < 4; ++b) {  // 32 K
+                uint32_t d[32], o[16];
+                if (begins) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float4 y = src ? *reinterpret_cast<const float4*>(src + (size_t)r * kD + 32 * b + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        d[4 * j] = __float_as_uint(y.x);
+                        d[4 * j + 1] = __float_as_uint(y.y);
+                        d[4 * j + 2] = __float_as_uint(y.z);
+                        d[4 * j + 3] = __float_as_uint(y.w);
+                    }
+                } else {
+                    tmem_ld32_async(tl + kColS + 32 * b, d);
+                    tmem_ld_wait();
+                    tmem_regs_ready(d);
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float2 y = make_float2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1]));
+                    if (kOut) o[j] = pack_bf16x2(y.x, y.y);
+                    const float2 z = mul2(y, make_float2(el, el));
+                    d[2 * j] = __float_as_uint(z.x);
+                    d[2 * j + 1] = __float_as_uint(z.y);
+                }
+                tmem_st32(tl + kColS + 32 * b, d);
+                if (kOut) tmem_st16(tl + kColB + 16 * b, o);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&x.b->s_full);
+            if (!kOut) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&x.b->g_empty[g % kGates]);
+            }
+        }
+        if (ends) {
+            LIN_WAIT(x.b->u_full, g - 1);
+            tc_fence_after();
+#pragma unroll 1
+            for (int b = 0; b < 4; ++b) {
+                uint32_t d[32];
+                tmem_ld32_async(tl + kColS + 32 * b, d);
+                tmem_ld_wait();
+                tmem_regs_ready(d);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    *reinterpret_cast<uint4*>(dst + (size_t)r * kD + 32 * b + 4 * j) = make_uint4(d[4 * j], d[4 * j + 1], d[4 * j + 2], d[4 * j + 3]);
+            }
+            if (!kOut && r == 0) p.gamma[blockIdx.x] = gamma;
+        }
+    }
+    return true;
+}
+#undef LIN_WAIT
+
+// kOut: the output launch.  Otherwise the segment launch: what the unfinished segment at the end of every stretch
+// adds to the state there.
 template <bool kOut>
 __global__ void __launch_bounds__(lin::kThreads, 1)
     gdn_linear_prefill_kernel(LinearPrefillArgs p, const __grid_constant__ LinearMaps maps) {
     using namespace lin;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    const uint32_t sbase = smem_u32(sm);
-    uint64_t* full = reinterpret_cast<uint64_t*>(sm + kOffBar);
-    uint64_t* empty = full + kStages;
-    uint64_t* bar_p = empty + kStages;
-    uint64_t* bar_u = bar_p + 1;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_u + 1);
-    uint32_t* tslot = reinterpret_cast<uint32_t*>(bar_u + 1) + 1;
-    float* sG2 = reinterpret_cast<float*>(sm + kOffG);
-    float* sEG = sG2 + 64;
-    float* sER = sEG + 64;
-    float* sEL = sER + 64;
-
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    Bars* b = reinterpret_cast<Bars*>(sm + kOffBar);
+    LinRange* range = reinterpret_cast<LinRange*>(sm + kOffRange);
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be uniform, and with it all role code
+    if (tid == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&b->full[s], 1);
+            mbar_init(&b->empty[s], 1);
+        }
+        for (int s = 0; s < kGates; ++s) {
+            mbar_init(&b->g_full[s], 1);
+            mbar_init(&b->g_empty[s], 4);
+        }
+        mbar_init(&b->qk_full, 1);
+        mbar_init(&b->qk_empty, 128);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&b->p_full[s], 128);
+            mbar_init(&b->p_empty[s], 1);
+        }
+        mbar_init(&b->v_full, 256);
+        mbar_init(&b->u_full, 1);
+        mbar_init(&b->s_full, 128);
+        mbar_init(&b->i_full, 1);
+        mbar_init(&b->o_full, 1);
+        mbar_init(&b->o_empty, 128);
+        mbar_init(&b->done, 1);
+        mbar_fence_init();
+    }
     pdl_wait();
     pdl_trigger();
     if (blockIdx.x == 0) {
         if (tid == 0 && (!kOut || !p.cut)) *p.status = 0;  // the call's first launch
         if (kOut && p.zero_unowned) zero_rows(p, tid, kThreads);
     }
-    const int hv = blockIdx.x % p.HV, slot = blockIdx.x / p.HV, hq = hv / (p.HV / p.H);
-    const SegItem it = kOut ? find_segment(p, slot, 1, 1) : find_segment(p, slot, 0, 2);
-    const bool last = it.seg == it.nsegs - 1;
-    if (it.n < 0 || (!kOut && last)) return;
-
-    if (tid == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            mbar_init(full + s, 1);
-            mbar_init(empty + s, kMath / 32);
-        }
-        mbar_init(bar_p, 1);
-        mbar_init(bar_u, 1);
-        *abort_flag = 0;
-        mbar_fence_init();
+    find_range(p, range);
+    const Mark m0 = range->at[0], m1 = range->at[1];
+    LinCtx x;
+    x.sm = sm;
+    x.sbase = smem_u32(sm);
+    x.b = b;
+    x.prev = (int)blockIdx.x - 1;
+    if (kOut) {
+        x.walk = Walk{m0.n, m0.hv, m0.chunk, m1.pos - m0.pos};
+    } else {
+        const bool same = m0.n == m1.n && m0.hv == m1.hv;
+        const int from = same ? m0.chunk : 0;
+        x.walk = Walk{m1.n, m1.hv, from, m1.pos > m0.pos ? m1.chunk - from : 0};
+        // 1: a segment begins here and goes on, 2: one goes through, 0: neither
+        if (tid == 0) p.kind[blockIdx.x] = x.walk.left <= 0 ? 0 : from > 0 ? 2 : 1;
     }
-    if (warp == 0) tmem_alloc(tslot, kTmemCols);
+    if (x.walk.left <= 0) return;  // the whole CTA
+
+    if (warp == 1) tmem_alloc(&b->tmem, kTmemCols);
+    if (kOut) {  // P above its diagonal
+        for (int i = tid; i < 1024; i += kThreads) reinterpret_cast<uint4*>(sm + kOffP)[i] = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tslot;
-    const int nchunks = max(0, (it.t1 - it.t0 + C - 1) / C);
 
-    if (warp == kMath / 32) {
-        if (lane == 0) {
-            for (int c = 0; c < nchunks; ++c) {
-                const int s = c % kStages;
-                if (c >= kStages && !mbar_wait(empty + s, (uint32_t)((c / kStages - 1) & 1), p.status, kErrScanTmaTimeout)) break;
-                unsigned char* st = sm + s * kStage;
-                const int t = it.t0 + c * C;
-                mbar_arrive_expect_tx(full + s, kOut ? 49152 : 32768);
-#pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    if (kOut) tma_load_3d(st + kOffQ + a * kAtom, &maps.q, 64 * a, hq, t, full + s);
-                    tma_load_3d(st + kOffK + a * kAtom, &maps.k, 64 * a, hq, t, full + s);
-                    tma_load_3d(st + kOffV + a * 8192, &maps.v, 64 * a, hv, t, full + s);
-                }
-            }
-        }
-    } else {
-        const int quarter = warp & 3, half = warp >> 2;
-        const int r = lane + 32 * quarter;  // TMEM lane: V row of the state, or token of the chunk
-        const uint32_t tl = tmem + ((uint32_t)(32 * quarter) << 16);
-        float h[64];  // state row r, columns 64 half ..
-        {
-            const float* src = nullptr;
-            if (kOut) {
-                if (it.nsegs == 1)
-                    src = p.state ? p.state + ((size_t)it.n * p.HV + hv) * kD * kD : nullptr;
-                else  // the chain left the states at the segments' ends, and the initial state behind them
-                    src = p.seg + ((size_t)(it.state0 + (it.seg == 0 ? it.nsegs - 1 : it.seg - 1)) * p.HV + hv) * kD * kD;
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float4 x = src ? *reinterpret_cast<const float4*>(src + (size_t)r * kD + 64 * half + 4 * j)
-                                     : make_float4(0.f, 0.f, 0.f, 0.f);
-                h[4 * j] = x.x;
-                h[4 * j + 1] = x.y;
-                h[4 * j + 2] = x.z;
-                h[4 * j + 3] = x.w;
-            }
-        }
-        // bf16 copy of the state: row r, atom `half`, eight 16-byte chunks XOR-swizzled by the row
-        auto write_s = [&]() {
-            unsigned char* row = sm + kOffS + half * 16384 + r * 128;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                *reinterpret_cast<uint4*>(row + ((j ^ (r & 7)) << 4)) =
-                    make_uint4(pack_bf16x2(h[8 * j], h[8 * j + 1]), pack_bf16x2(h[8 * j + 2], h[8 * j + 3]),
-                               pack_bf16x2(h[8 * j + 4], h[8 * j + 5]), pack_bf16x2(h[8 * j + 6], h[8 * j + 7]));
-        };
-        if (kOut && nchunks > 0) write_s();
-        constexpr uint32_t idesc_qk = umma_idesc_bf16(128, 64, false, false);
-        constexpr uint32_t idesc_oi = umma_idesc_bf16(128, 64, false, false);
-        constexpr uint32_t idesc_oa = umma_idesc_bf16(128, 64, true, false);
-        constexpr uint32_t idesc_u = umma_idesc_bf16(128, 128, true, true);
-        float gamma = 1.f;  // product of the segment's decays (thread 0 of the segment launch)
-        int c = 0;
-        for (; c < nchunks; ++c) {
-            const int s = c % kStages, t0 = it.t0 + c * C, L = min(C, it.t1 - t0);
-            unsigned char* st = sm + s * kStage;
-            const uint32_t sst = sbase + (uint32_t)s * kStage;
-            if (warp == 0) {
-                // prefix and suffix sums of the chunk's log decays, two tokens a lane
-                float a0 = 0.f, a1 = 0.f;
-                if (2 * lane < L) a0 = p.decay[p.per_token ? (size_t)(t0 + 2 * lane) * p.HV + hv : hv];
-                if (2 * lane + 1 < L) a1 = p.decay[p.per_token ? (size_t)(t0 + 2 * lane + 1) * p.HV + hv : hv];
-                a0 = a0 < kMinDecay ? kMinDecay : a0;
-                a1 = a1 < kMinDecay ? kMinDecay : a1;
-                float pre = a0 + a1, suf = a0 + a1;
-#pragma unroll
-                for (int off = 1; off < 32; off <<= 1) {
-                    const float x = __shfl_up_sync(0xffffffffu, pre, off), y = __shfl_down_sync(0xffffffffu, suf, off);
-                    if (lane >= off) pre += x;
-                    if (lane + off < 32) suf += y;
-                }
-                float before = __shfl_up_sync(0xffffffffu, pre, 1), after = __shfl_down_sync(0xffffffffu, suf, 1);
-                if (lane == 0) before = 0.f;
-                if (lane == 31) after = 0.f;
-                const float g0 = before + a0, g1 = pre;
-                sG2[2 * lane] = g0 * kLog2e;
-                sG2[2 * lane + 1] = g1 * kLog2e;
-                sEG[2 * lane] = expf(g0);
-                sEG[2 * lane + 1] = expf(g1);
-                // e^{G_C - G_j} from the sum of the later decays: exact where it matters, near the chunk's end
-                sER[2 * lane] = 2 * lane < L ? expf(after + a1) : 0.f;
-                sER[2 * lane + 1] = 2 * lane + 1 < L ? expf(after) : 0.f;
-                if (lane == 31) *sEL = expf(pre);
-            }
-            if (!mbar_wait(full + s, (uint32_t)((c / kStages) & 1), p.status, kErrScanTmaTimeout)) *abort_flag = 1;
-            fence_async_smem();  // the state copy (generic stores) -> the tensor core
-            tc_fence_before();
-            named_bar_sync(1, kMath);
-            if (*abort_flag) break;
-            tc_fence_after();
-            const float eL = *sEL;
-            if (kOut && tid == 0) {
-#pragma unroll
-                for (int kk = 0; kk < 8; ++kk)
-                    umma_bf16(tmem + kColP, umma_desc_sw128(sst + kOffQ + (uint32_t)(kk >> 2) * kAtom + (uint32_t)(kk & 3) * 32u, 16, 1024),
-                              umma_desc_sw128(sst + kOffK + (uint32_t)(kk >> 2) * kAtom + (uint32_t)(kk & 3) * 32u, 16, 1024), idesc_qk, kk > 0);
-                umma_commit(bar_p);
-#pragma unroll
-                for (int kk = 0; kk < 8; ++kk)
-                    umma_bf16(tmem + kColI, umma_desc_sw128(sbase + kOffS + (uint32_t)(kk >> 2) * 16384u + (uint32_t)(kk & 3) * 32u, 16, 1024),
-                              umma_desc_sw128(sst + kOffQ + (uint32_t)(kk >> 2) * kAtom + (uint32_t)(kk & 3) * 32u, 16, 1024), idesc_oi, kk > 0);
-            }
-            bool ok = true;
-            if (kOut && L < C) ok = mbar_wait(bar_p, (uint32_t)(c & 1), p.status, kErrScanMmaTimeout);
-            // Decayed v: thread (token i, 32 columns).  Rows behind the segment's end (another sequence's
-            // tokens, or zeros) become zero in v and k too, so whatever they hold cannot reach a product.
-            {
-                const int i = tid & 63, q4 = tid >> 6;  // columns 32 q4 ..
-                const float er = sER[i];
-                unsigned char* vt = st + kOffV + (q4 >> 1) * 8192 + i * 128;
-                unsigned char* vh = sm + kOffVh + (q4 >> 1) * 8192 + i * 128;
-                unsigned char* vl = sm + kOffVl + (q4 >> 1) * 8192 + i * 128;
-#pragma unroll
-                for (int jj = 0; jj < 4; ++jj) {
-                    const uint32_t off = (uint32_t)(((4 * (q4 & 1) + jj) ^ (i & 7)) << 4);
-                    uint4 x = *reinterpret_cast<const uint4*>(vt + off);
-                    if (i >= L) {
-                        x = make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4*>(vt + off) = x;
-                        *reinterpret_cast<uint4*>(st + kOffK + (q4 >> 1) * kAtom + i * 128 + off) = x;
-                    }
-                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 y = mul2(make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u)), make_float2(er, er));
-                        hi[e] = pack_bf16x2(y.x, y.y);
-                        const float2 z = sub2(y, make_float2(__uint_as_float(hi[e] << 16), __uint_as_float(hi[e] & 0xffff0000u)));
-                        lo[e] = pack_bf16x2(z.x, z.y);
-                    }
-                    *reinterpret_cast<uint4*>(vh + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(vl + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                }
-            }
-            if (kOut) {
-                if (L == C) ok = mbar_wait(bar_p, (uint32_t)(c & 1), p.status, kErrScanMmaTimeout);
-                tc_fence_after();
-                if (quarter < 2) {  // P row i = r, columns 32 half ..
-                    uint32_t d[32];
-                    tmem_ld32_async(tl + kColP + 32 * half, d);
-                    tmem_ld_wait();
-                    tmem_regs_ready(d);
-                    const float gi = sG2[r];
-                    unsigned char* row = sm + kOffP + r * 128;
-#pragma unroll
-                    for (int jj = 0; jj < 4; ++jj) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int j = 32 * half + 8 * jj + 2 * e;
-                            const float x = j <= r && j < L ? __uint_as_float(d[8 * jj + 2 * e]) * exp2f(gi - sG2[j]) : 0.f;
-                            const float y = j + 1 <= r && j + 1 < L ? __uint_as_float(d[8 * jj + 2 * e + 1]) * exp2f(gi - sG2[j + 1]) : 0.f;
-                            w[e] = pack_bf16x2(x, y);
-                        }
-                        *reinterpret_cast<uint4*>(row + (((4 * half + jj) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                }
-            }
-            fence_async_smem();
-            tc_fence_before();
-            if (!ok) *abort_flag = 1;
-            named_bar_sync(1, kMath);
-            tc_fence_after();
-            if (*abort_flag) break;
-            if (tid == 0) {
-                if (kOut) {
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        umma_bf16(tmem + kColA, umma_desc_sw128(sst + kOffV + 2048u * kk, 8192, 1024),
-                                  umma_desc_sw128(sbase + kOffP + 32u * kk, 16, 1024), idesc_oa, kk > 0);
-                }
-#pragma unroll
-                for (int kk = 0; kk < 8; ++kk)
-                    umma_bf16(tmem + kColU, umma_desc_sw128(sbase + (kk < 4 ? kOffVh : kOffVl) + 2048u * (kk & 3), 8192, 1024),
-                              umma_desc_sw128(sst + kOffK + 2048u * (kk & 3), kAtom, 1024), idesc_u, kk > 0);
-                umma_commit(bar_u);
-            }
-            ok = mbar_wait(bar_u, (uint32_t)(c & 1), p.status, kErrScanMmaTimeout);
-            tc_fence_after();
-            if (lane == 0) mbar_arrive(empty + s);  // the products of this stage are done
-            if (kOut) {
-                // output column r, tokens 32 half ..: o = scale (e^{G_i} OI + OA), staged so that rows leave whole
-                uint32_t x[32], y[32];
-                tmem_ld32_async(tl + kColI + 32 * half, x);
-                tmem_ld32_async(tl + kColA + 32 * half, y);
-                tmem_ld_wait();
-                tmem_regs_ready(x);
-                tmem_regs_ready(y);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const int i = 32 * half + j;
-                    const float o = p.scale * fmaf(sEG[i], __uint_as_float(x[j]), __uint_as_float(y[j]));
-                    *reinterpret_cast<uint16_t*>(sm + kOffO + i * 256 + (((r >> 3) ^ (i & 7)) << 4) + (r & 7) * 2) = f2bf(o);
-                }
-            }
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                uint32_t d[32];
-                tmem_ld32_async(tl + kColU + 64 * half + 32 * b, d);
-                tmem_ld_wait();
-                tmem_regs_ready(d);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) h[32 * b + j] = fmaf(eL, h[32 * b + j], __uint_as_float(d[j]));
-            }
-            gamma *= eL;
-            if (!ok) *abort_flag = 1;
-            if (kOut) {
-                write_s();
-                named_bar_sync(1, kMath);  // the staged output rows
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int i = 16 * q + (tid >> 4), ch = tid & 15;
-                    if (i < L)
-                        *reinterpret_cast<uint4*>(p.out + ((size_t)(t0 + i) * p.HV + hv) * kD + 8 * ch) =
-                            *reinterpret_cast<const uint4*>(sm + kOffO + i * 256 + ((ch ^ (i & 7)) << 4));
-                }
-            } else {
-                named_bar_sync(1, kMath);  // the chunk's decays are consumed
-            }
-        }
-        if (c < nchunks) {
+    bool ok = true;
+    if (warp == 0) {
+        int issued = 0;
+        if (!(ok = role_load<kOut>(p, maps, x, elect_one(), &issued)))
             // gave up: let copies already in flight land (bounded) before the CTA exits
-            if (tid == 0)
-                for (int cc = c; cc < min(nchunks, c + kStages); ++cc)
-                    mbar_wait(full + cc % kStages, (uint32_t)((cc / kStages) & 1), nullptr, 0);
-        } else if (!kOut || last) {
-            float* dst = kOut ? p.new_state + ((size_t)it.n * p.HV + hv) * kD * kD : p.seg + ((size_t)slot * p.HV + hv) * kD * kD;
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                *reinterpret_cast<float4*>(dst + (size_t)r * kD + 64 * half + 4 * j) =
-                    make_float4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
-            if (!kOut && tid == 0) p.gamma[(size_t)slot * p.HV + hv] = gamma;
-        }
+            for (int g = max(0, issued - kStages); g < issued; ++g) warp_wait(&b->full[g % kStages], (uint32_t)((g / kStages) & 1));
+    } else if (warp == 1) {
+        const uint32_t one = elect_one();
+        ok = role_mma<kOut>(p, x, one);
+        // products still in flight end before the TMEM is given back
+        commit_one(one, &b->done);
+        ok = warp_wait(&b->done, 0) && ok;
+    } else if (warp == 2) {
+        ok = role_gates(p, x);
+    } else if (warp < 4) {
+    } else if (warp < 8) {
+        if (kOut) ok = role_p(p, x);
+    } else if (warp < 16) {
+        ok = role_v<kOut>(p, x);
+    } else if (warp < 20) {
+        if (kOut) ok = role_o(p, maps, x);
+    } else {
+        ok = role_s<kOut>(p, x);
     }
+    if (!ok && lane == 0) atomicCAS(p.status, 0, kErrScanMmaTimeout);
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem, kTmemCols);
+    if (warp == 1) tmem_dealloc(b->tmem, kTmemCols);
 }
 
-// State at the end of every segment but a sequence's last, in place of what the segment adds, and the initial state
-// in the slot behind them: new_state may be state itself, and a last segment may end before a first one begins.
-// One CTA per (1024 state elements, v-head, start of a possible sequence of several segments).
+// The state at the end of every stretch that ends inside a segment, in place of what its last segment adds there, and
+// the segment's initial state in the slot p.ctas further: new_state may be state itself, and a segment may end in
+// one CTA before it begins in another.  One CTA per (stretch in which such a segment begins, 1024 state elements).
 __global__ void __launch_bounds__(256) gdn_linear_chain_kernel(LinearPrefillArgs p) {
+    __shared__ LinRange range;
     pdl_wait();
     pdl_trigger();
-    const int hv = blockIdx.x % p.HV;
-    const SegItem it = find_segment(p, 2 * (blockIdx.x / p.HV), 0, 2);
-    if (it.n < 0 || it.seg != 0 || it.nsegs == 1) return;
+    if (p.kind[blockIdx.x] != 1) return;
+    find_range(p, &range);
+    const int n = range.at[1].n, hv = range.at[1].hv;
     const size_t el = blockIdx.y * 1024 + threadIdx.x * 4;
     float4 h = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (p.state) h = *reinterpret_cast<const float4*>(p.state + ((size_t)it.n * p.HV + hv) * kD * kD + el);
-    *reinterpret_cast<float4*>(p.seg + ((size_t)(it.state0 + it.nsegs - 1) * p.HV + hv) * kD * kD + el) = h;
+    if (p.state) {
+        h = *reinterpret_cast<const float4*>(p.state + ((size_t)n * p.HV + hv) * kD * kD + el);
+        *reinterpret_cast<float4*>(p.seg + (size_t)(p.ctas + blockIdx.x) * kD * kD + el) = h;
+    }
+    int end = blockIdx.x + 1;
+    while (end < p.ctas && p.kind[end] == 2) ++end;
 #pragma unroll 4
-    for (int g = 0; g < it.nsegs - 1; ++g) {
-        const size_t at = (size_t)(it.state0 + g) * p.HV + hv;
-        const float gm = p.gamma[at];
-        float4* d = reinterpret_cast<float4*>(p.seg + at * kD * kD + el);
-        const float4 x = *d;
-        h = make_float4(fmaf(gm, h.x, x.x), fmaf(gm, h.y, x.y), fmaf(gm, h.z, x.z), fmaf(gm, h.w, x.w));
+    for (int c = blockIdx.x; c < end; ++c) {
+        const float gm = p.gamma[c];
+        float4* d = reinterpret_cast<float4*>(p.seg + (size_t)c * kD * kD + el);
+        const float4 y = *d;
+        h = make_float4(fmaf(gm, h.x, y.x), fmaf(gm, h.y, y.y), fmaf(gm, h.z, y.z), fmaf(gm, h.w, y.w));
         *d = h;
     }
 }
 
 LinearPrefillLayout linear_prefill_layout(int N, int T, int HV) {
     LinearPrefillLayout L{};
-    // Chunks per segment: as many as one of 148 SMs has to do, but at least 8 (below, the two more launches of a cut
-    // sequence cost more than its chunks).
-    const long long chunks = (long long)T / lin::C + N;
-    const long long m = std::min<long long>(std::max<long long>(8, (chunks * HV + 147) / 148), 1 << 20);
-    const long long len = lin::C * m;
-    L.m = (int)m;
-    L.cut = T > len ? 1 : 0;
-    L.slots = (int)(T / len) + N;
-    L.states = L.cut ? 2 * (int)(T / len) : 0;
+    const long long share = ((long long)T / lin::C + N) * HV / kLinearCtas;  // chunks of a CTA
+    L.min_share = 4;
+    L.keep = (int)std::max<long long>(8, std::min<long long>(share / 8, 1 << 20));
+    L.cut = T > (long long)lin::C * L.keep ? 1 : 0;
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+    const size_t slots = L.cut ? kLinearCtas : 0;
     L.off_status = 0;
-    L.off_gamma = 256;
-    L.off_seg = up(L.off_gamma + (size_t)L.states * HV * sizeof(float));
-    L.total = L.off_seg + (size_t)L.states * HV * kD * kD * sizeof(float);
+    L.off_kind = 256;
+    L.off_gamma = up(L.off_kind + slots * sizeof(int));
+    L.off_seg = up(L.off_gamma + slots * sizeof(float));
+    L.total = L.off_seg + 2 * slots * kD * kD * sizeof(float);
     return L;
 }
 
@@ -432,15 +881,15 @@ int launch_linear_prefill(const LinearPrefillArgs& p, cudaStream_t stream) {
     using namespace lin;
     LinearMaps maps{};
     if (p.T > 0 && !(map_bf16_rows(&maps.q, p.q, p.H, p.T) && map_bf16_rows(&maps.k, p.k, p.H, p.T) &&
-                     map_bf16_rows(&maps.v, p.v, p.HV, p.T)))
+                     map_bf16_rows(&maps.v, p.v, p.HV, p.T) && map_bf16_rows(&maps.o, p.out, p.HV, p.T)))
         return -3;
     if (cudaFuncSetAttribute(gdn_linear_prefill_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
         cudaFuncSetAttribute(gdn_linear_prefill_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
         return -1;
-    const dim3 grid((unsigned)p.slots * (unsigned)p.HV), seg_grid((unsigned)p.states * (unsigned)p.HV);
+    const dim3 grid((unsigned)p.ctas);
     if (p.cut) {
-        if (launch_pdl(gdn_linear_prefill_kernel<false>, seg_grid, dim3(kThreads), kSmem, stream, p, maps) != cudaSuccess) return -1;
-        if (launch_pdl(gdn_linear_chain_kernel, dim3(seg_grid.x / 2, 16), dim3(256), 0, stream, p) != cudaSuccess) return -1;
+        if (launch_pdl(gdn_linear_prefill_kernel<false>, grid, dim3(kThreads), kSmem, stream, p, maps) != cudaSuccess) return -1;
+        if (launch_pdl(gdn_linear_chain_kernel, dim3((unsigned)p.ctas, 16), dim3(256), 0, stream, p) != cudaSuccess) return -1;
     }
     return launch_pdl(gdn_linear_prefill_kernel<true>, grid, dim3(kThreads), kSmem, stream, p, maps) == cudaSuccess ? 0 : -1;
 }
