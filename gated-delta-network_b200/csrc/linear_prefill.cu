@@ -70,11 +70,6 @@ struct LinearMaps {
 struct Mark {  // a place on the line: chunk `chunk` of (sequence n, v-head hv)
     int n, hv, chunk, pos;
 };
-struct LinRange {
-    int sum[lin::kThreads / 32];
-    Mark at[2];  // the CTA's stretch
-};
-static_assert(sizeof(LinRange) <= 256, "range");
 
 __device__ __forceinline__ int lin_chunks(const LinearPrefillArgs& p, int n) {
     int s, e;
@@ -82,70 +77,51 @@ __device__ __forceinline__ int lin_chunks(const LinearPrefillArgs& p, int n) {
     return max(1, (e - s + lin::C - 1) / lin::C);  // an empty sequence has a place too: its state is copied
 }
 
-// The stretch of CTA blockIdx.x.  All threads of the CTA take part; the result is in r->at.  (Positions are ints: the
-// entry point refuses calls of 2^31 chunks.)
-__device__ __forceinline__ void find_range(const LinearPrefillArgs& p, LinRange* r) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-    int total = 0, want[2] = {0, 0};
+// The ends of the stretch of CTA blockIdx.x, by one warp: every lane sums up an equal part of the sequences.
+// (Positions are ints: the entry point refuses calls of 2^31 chunks.)
+__device__ __forceinline__ void find_range(const LinearPrefillArgs& p, Mark* at) {
+    const int lane = threadIdx.x & 31, part = (p.N + 31) / 32, n0 = min(p.N, lane * part), n1 = min(p.N, n0 + part);
+    int mine = 0;
+#pragma unroll 4
+    for (int n = n0; n < n1; ++n) mine += lin_chunks(p, n);
+    int x = mine;
 #pragma unroll 1
-    for (int round = 0; round < 2; ++round) {  // the sum of all lengths, then the two ends
-        int before = 0;  // chunks of the sequences in front of this pass
+    for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, off);
+        if (lane >= off) x += y;
+    }
+    const int total = __shfl_sync(0xffffffffu, x, 31) * p.HV;
+    const int ctas = max(1, min(p.ctas, total / p.min_share)), per = total / ctas, more = total - per * ctas;
 #pragma unroll 1
-        for (int base = 0; base < p.N; base += blockDim.x) {
-            const int n = base + tid;
-            const int nc = n < p.N ? lin_chunks(p, n) : 0;
-            int x = nc;
-#pragma unroll 1
-            for (int off = 1; off < 32; off <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, off);
-                if (lane >= off) x += y;
+    for (int i = 0; i < 2; ++i) {
+        const int c = blockIdx.x + i, want = min(total, c * per + min(c, more));
+        int lo = (x - mine) * p.HV;
+        if (want >= lo && want < lo + mine * p.HV) {
+            int n = n0, nc = lin_chunks(p, n);
+            while (want >= lo + nc * p.HV) {
+                lo += nc * p.HV;
+                nc = lin_chunks(p, ++n);
             }
-            __syncthreads();
-            if (lane == 31) r->sum[warp] = x;
-            __syncthreads();
-            int pass = 0;
-#pragma unroll 1
-            for (int w = 0; w < warps; ++w) {
-                if (w < warp) x += r->sum[w];
-                pass += r->sum[w];
-            }
-            const int lo = (before + x - nc) * p.HV;
-            if (round == 1) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int off = want[i] - lo;
-                    if (off >= 0 && off < nc * p.HV) {
-                        Mark m;
-                        m.n = n;
-                        m.hv = off / nc;
-                        m.chunk = off - m.hv * nc;
-                        m.pos = want[i];
-                        if (nc <= p.keep && m.chunk) {  // a short segment is not cut: to its nearer end
-                            const int up = 2 * m.chunk >= nc;
-                            m.pos += up ? nc - m.chunk : -m.chunk;
-                            m.chunk = 0;
-                            m.hv += up;
-                            if (m.hv == p.HV) {
-                                m.hv = 0;
-                                ++m.n;
-                            }
-                        }
-                        r->at[i] = m;
-                    }
+            Mark m;
+            m.n = n;
+            m.hv = (want - lo) / nc;
+            m.chunk = want - lo - m.hv * nc;
+            m.pos = want;
+            if (nc <= p.keep && m.chunk) {  // a short segment is not cut: to its nearer end
+                const int up = 2 * m.chunk >= nc;
+                m.pos += up ? nc - m.chunk : -m.chunk;
+                m.chunk = 0;
+                m.hv += up;
+                if (m.hv == p.HV) {
+                    m.hv = 0;
+                    ++m.n;
                 }
             }
-            before += pass;
-        }
-        if (round == 0) {
-            total = before * p.HV;
-            const int ctas = max(1, min(p.ctas, total / p.min_share)), per = total / ctas, more = total - per * ctas;
-            const int c = blockIdx.x;
-            want[0] = min(total, c * per + min(c, more));
-            want[1] = min(total, (c + 1) * per + min(c + 1, more));
-            if (tid < 2 && want[tid] == total) r->at[tid] = Mark{p.N, 0, 0, total};
+            at[i] = m;
+        } else if (lane == 0 && want == total) {
+            at[i] = Mark{p.N, 0, 0, total};
         }
     }
-    __syncthreads();
 }
 
 struct Piece {
@@ -418,6 +394,12 @@ __device__ __forceinline__ bool role_mma(const LinearPrefillArgs& p, const LinCt
 #pragma unroll
             for (int kk = 1; kk < 8; ++kk) mma_ts<true>(one, x.tmem + kColI, x.tmem + kColB + 8 * kk, d_q + st + step(kk), idesc_oi);
             commit_one(one, &x.b->i_full);
+            if (g + 1 < total) {  // ahead of OA, so that the P warps have chunk g + 1 while the tensor core ends g
+                LIN_WAIT(x.b->full[sn], sn_ph);
+                LIN_WAIT(x.b->qk_empty, ph);
+                tc_fence_after();
+                qk((uint32_t)sn * kStep);
+            }
             LIN_WAIT(x.b->p_full[ph], g >> 1);
             tc_fence_after();
             const uint32_t pb = d_p + ph * 512u;
@@ -426,16 +408,10 @@ __device__ __forceinline__ bool role_mma(const LinearPrefillArgs& p, const LinCt
             for (int kk = 1; kk < 4; ++kk) mma_ss<true>(one, x.tmem + kColA, d_v + st + 128 * kk, pb + 2 * kk, idesc_oa);
             commit_one(one, &x.b->p_empty[ph]);
             commit_one(one, &x.b->o_full);
+        } else if (g + 1 < total) {
+            LIN_WAIT(x.b->full[sn], sn_ph);
         }
         commit_one(one, &x.b->empty[s]);
-        if (g + 1 < total) {
-            LIN_WAIT(x.b->full[sn], sn_ph);
-            if (kOut) {
-                LIN_WAIT(x.b->qk_empty, ph);
-                tc_fence_after();
-                qk((uint32_t)sn * kStep);
-            }
-        }
         s = sn;
         s_ph = sn_ph;
     }
@@ -743,7 +719,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     Bars* b = reinterpret_cast<Bars*>(sm + kOffBar);
-    LinRange* range = reinterpret_cast<LinRange*>(sm + kOffRange);
+    Mark* range = reinterpret_cast<Mark*>(sm + kOffRange);
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be uniform, and with it all role code
     if (tid == 0) {
@@ -776,8 +752,16 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         if (tid == 0 && (!kOut || !p.cut)) *p.status = 0;  // the call's first launch
         if (kOut && p.zero_unowned) zero_rows(p, tid, kThreads);
     }
-    find_range(p, range);
-    const Mark m0 = range->at[0], m1 = range->at[1];
+    if (warp == 0) find_range(p, range);
+    if (warp == 1) tmem_alloc(&b->tmem, kTmemCols);
+    if (kOut) {  // P above its diagonal
+        for (int i = tid; i < 1024; i += kThreads) reinterpret_cast<uint4*>(sm + kOffP)[i] = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const Mark m0 = range[0], m1 = range[1];
     LinCtx x;
     x.sm = sm;
     x.sbase = smem_u32(sm);
@@ -792,17 +776,6 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         // 1: a segment begins here and goes on, 2: one goes through, 0: neither
         if (tid == 0) p.kind[blockIdx.x] = x.walk.left <= 0 ? 0 : from > 0 ? 2 : 1;
     }
-    if (x.walk.left <= 0) return;  // the whole CTA
-
-    if (warp == 1) tmem_alloc(&b->tmem, kTmemCols);
-    if (kOut) {  // P above its diagonal
-        for (int i = tid; i < 1024; i += kThreads) reinterpret_cast<uint4*>(sm + kOffP)[i] = make_uint4(0, 0, 0, 0);
-        fence_async_smem();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-
     bool ok = true;
     if (warp == 0) {
         int issued = 0;
@@ -837,12 +810,13 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
 // the segment's initial state in the slot p.ctas further: new_state may be state itself, and a segment may end in
 // one CTA before it begins in another.  One CTA per (stretch in which such a segment begins, 1024 state elements).
 __global__ void __launch_bounds__(256) gdn_linear_chain_kernel(LinearPrefillArgs p) {
-    __shared__ LinRange range;
+    __shared__ Mark range[2];
     pdl_wait();
     pdl_trigger();
     if (p.kind[blockIdx.x] != 1) return;
-    find_range(p, &range);
-    const int n = range.at[1].n, hv = range.at[1].hv;
+    if (threadIdx.x < 32) find_range(p, range);
+    __syncthreads();
+    const int n = range[1].n, hv = range[1].hv;
     const size_t el = blockIdx.y * 1024 + threadIdx.x * 4;
     float4 h = make_float4(0.f, 0.f, 0.f, 0.f);
     if (p.state) {
@@ -864,9 +838,9 @@ __global__ void __launch_bounds__(256) gdn_linear_chain_kernel(LinearPrefillArgs
 LinearPrefillLayout linear_prefill_layout(int N, int T, int HV) {
     LinearPrefillLayout L{};
     const long long share = ((long long)T / lin::C + N) * HV / kLinearCtas;  // chunks of a CTA
-    L.min_share = 4;
-    L.keep = (int)std::max<long long>(8, std::min<long long>(share / 8, 1 << 20));
+    L.keep = (int)std::max<long long>(8, std::min<long long>(3 * share / 10, 1 << 20));
     L.cut = T > (long long)lin::C * L.keep ? 1 : 0;
+    L.min_share = L.cut ? 4 : 1;
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     const size_t slots = L.cut ? kLinearCtas : 0;
     L.off_status = 0;
