@@ -31,7 +31,7 @@ namespace gdn {
 
 namespace lin {
 constexpr int C = 64;
-constexpr int kThreads = 768;  // 6 warpgroups: {TMA, MMA, gates, -}, P, V, V, O, S
+constexpr int kThreads = 768;  // 6 warpgroups: {TMA, U, gates, QK + OI + OA}, P, V, V, O, S
 constexpr int kStages = 3;
 constexpr int kGates = 8;
 // stage: [Q0 | K0 | Q1 | K1 | V0 | V1], each 64 tokens x 64 columns bf16, SWIZZLE_128B
@@ -39,8 +39,9 @@ constexpr uint32_t kOffQ = 0, kOffK = 8192, kAtom = 16384, kOffV = 32768;
 constexpr uint32_t kStage = 49152;
 constexpr uint32_t kOffP = kStages * kStage;     // P [2][64 i][64 j] bf16
 constexpr uint32_t kOffO = kOffP + 2 * 8192;     // output staging [2][2 atoms][64 tokens][64 V] bf16, SWIZZLE_128B
-constexpr uint32_t kOffG = kOffO + 2 * 16384;    // gates, kGates slots of f32: [64] G log2(e) | [64] scale e^G | [64] e^{G_C - G} | e^{G_C}
-constexpr uint32_t kGateFloats = 256;
+constexpr uint32_t kOffG = kOffO + 2 * 16384;    // gates, kGates slots of f32: [64] G | [64] factors of OI | [64] of v | [64] e^{G_b - G}, b the
+                                                 // last of the token's block of 16 | state: factor, unit at the end, decay, whether to multiply
+constexpr uint32_t kGateFloats = 264;
 constexpr uint32_t kOffBar = kOffG + kGates * kGateFloats * 4;
 constexpr uint32_t kOffRange = kOffBar + 512;
 constexpr uint32_t kSmem = kOffRange + 256 + 1024;
@@ -54,9 +55,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 // of prefix sums into NaN.
 constexpr float kMinDecay = -110.f;
 
+// A wait tells a phase from the one before it only, so whoever waits on a barrier must be needed for its next phase
+// but one: hence the pairs p_full and p_empty, whose sides run up to two chunks apart.
 struct Bars {
     uint64_t full[kStages], empty[kStages], g_full[kGates], g_empty[kGates];
-    uint64_t qk_full, qk_empty, p_full[2], p_empty[2], v_full, u_full, s_full, i_full, o_full, o_empty, done;
+    uint64_t qk_full, qk_empty, u_ready, u_full, b_ready, i_full, p_full[2], p_empty[2], o_empty, o_full, done[2];
     uint32_t tmem;
 };
 static_assert(sizeof(Bars) <= 512, "barriers");
@@ -71,55 +74,67 @@ struct Mark {  // a place on the line: chunk `chunk` of (sequence n, v-head hv)
     int n, hv, chunk, pos;
 };
 
-__device__ __forceinline__ int lin_chunks(const LinearPrefillArgs& p, int n) {
-    int s, e;
-    seq_bounds(p.cu, p.cu64, n, p.T, s, e);
-    return max(1, (e - s + lin::C - 1) / lin::C);  // an empty sequence has a place too: its state is copied
+// cu_seqlens[n], clamped to [0, T]; a sequence that ends before it begins is empty.
+__device__ __forceinline__ int cu_at(const LinearPrefillArgs& p, int n) {
+    const long long x = p.cu64 ? reinterpret_cast<const long long*>(p.cu)[n] : reinterpret_cast<const int*>(p.cu)[n];
+    return (int)max(0ll, min((long long)p.T, x));
 }
+// Chunks of a sequence of tokens [s, e): an empty one has a place on the line too, its state is copied.
+__device__ __forceinline__ int lin_chunks(int s, int e) { return max(1, (e - s + lin::C - 1) / lin::C); }
 
 // The ends of the stretch of CTA blockIdx.x, by one warp: every lane sums up an equal part of the sequences.
 // (Positions are ints: the entry point refuses calls of 2^31 chunks.)
 __device__ __forceinline__ void find_range(const LinearPrefillArgs& p, Mark* at) {
     const int lane = threadIdx.x & 31, part = (p.N + 31) / 32, n0 = min(p.N, lane * part), n1 = min(p.N, n0 + part);
-    int mine = 0;
-#pragma unroll 4
-    for (int n = n0; n < n1; ++n) mine += lin_chunks(p, n);
-    int x = mine;
+    int x = 0, lo = 0, total = 0, ctas = 1, per = 0, more = 0;
 #pragma unroll 1
-    for (int off = 1; off < 32; off <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, off);
-        if (lane >= off) x += y;
-    }
-    const int total = __shfl_sync(0xffffffffu, x, 31) * p.HV;
-    const int ctas = max(1, min(p.ctas, total / p.min_share)), per = total / ctas, more = total - per * ctas;
-#pragma unroll 1
-    for (int i = 0; i < 2; ++i) {
-        const int c = blockIdx.x + i, want = min(total, c * per + min(c, more));
-        int lo = (x - mine) * p.HV;
-        if (want >= lo && want < lo + mine * p.HV) {
-            int n = n0, nc = lin_chunks(p, n);
-            while (want >= lo + nc * p.HV) {
-                lo += nc * p.HV;
-                nc = lin_chunks(p, ++n);
+    for (int round = 0; round < 2; ++round) {  // the sum of the lane's lengths, then the marks among them
+        int s = n0 < n1 ? cu_at(p, n0) : 0;
+#pragma unroll 2
+        for (int n = n0; n < n1; ++n) {
+            const int e = cu_at(p, n + 1), nc = lin_chunks(s, e);
+            s = e;
+            if (round == 0) {
+                x += nc;
+                continue;
             }
-            Mark m;
-            m.n = n;
-            m.hv = (want - lo) / nc;
-            m.chunk = want - lo - m.hv * nc;
-            m.pos = want;
-            if (nc <= p.keep && m.chunk) {  // a short segment is not cut: to its nearer end
-                const int up = 2 * m.chunk >= nc;
-                m.pos += up ? nc - m.chunk : -m.chunk;
-                m.chunk = 0;
-                m.hv += up;
-                if (m.hv == p.HV) {
-                    m.hv = 0;
-                    ++m.n;
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) {
+                const int c = blockIdx.x + i, want = min(total, c * per + min(c, more)), off = want - lo;
+                if (off < 0 || off >= nc * p.HV) continue;
+                Mark m;
+                m.n = n;
+                m.hv = off / nc;
+                m.chunk = off - m.hv * nc;
+                m.pos = want;
+                if (nc <= p.keep && m.chunk) {  // a short segment is not cut: to its nearer end
+                    const int up = 2 * m.chunk >= nc;
+                    m.pos += up ? nc - m.chunk : -m.chunk;
+                    m.chunk = 0;
+                    m.hv += up;
+                    if (m.hv == p.HV) {
+                        m.hv = 0;
+                        ++m.n;
+                    }
                 }
+                at[i] = m;
             }
-            at[i] = m;
-        } else if (lane == 0 && want == total) {
-            at[i] = Mark{p.N, 0, 0, total};
+            lo += nc * p.HV;
+        }
+        if (round == 0) {
+            const int mine = x;
+#pragma unroll 1
+            for (int off = 1; off < 32; off <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, off);
+                if (lane >= off) x += y;
+            }
+            lo = (x - mine) * p.HV;
+            total = __shfl_sync(0xffffffffu, x, 31) * p.HV;
+            ctas = max(1, min(p.ctas, total / p.min_share));
+            per = total / ctas;
+            more = total - per * ctas;
+            const int c = blockIdx.x + lane;
+            if (lane < 2 && min(total, c * per + min(c, more)) == total) at[lane] = Mark{p.N, 0, 0, total};
         }
     }
 }
@@ -133,8 +148,9 @@ struct Walk {
         if (left <= 0 || n >= p.N) return false;
         x.n = n;
         x.hv = hv;
-        seq_bounds(p.cu, p.cu64, n, p.T, x.s, x.e);
-        x.nc = max(1, (x.e - x.s + lin::C - 1) / lin::C);
+        x.s = cu_at(p, n);
+        x.e = max(x.s, cu_at(p, n + 1));
+        x.nc = lin_chunks(x.s, x.e);
         x.ca = chunk;
         x.cb = min(x.nc, chunk + left);
         left -= x.cb - x.ca;
@@ -205,13 +221,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-// 16 lanes x 32 columns: register 2 i (2 i + 1) of thread t is lane t / 4 (+ 8), column 4 i + t % 4.
-__device__ __forceinline__ void tmem_st_16x128b_x8(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
+// 16 lanes x 8 columns: register 2 i (2 i + 1) of thread t is lane t / 4 (+ 8), column 4 i + t % 4.
+__device__ __forceinline__ void tmem_st_16x128b_x2(uint32_t taddr, const uint32_t (&r)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                 : "memory");
 }
 // 16 lanes x 32 columns: registers 4 i + {0, 1} ({2, 3}) of thread t are lane t / 4 (+ 8), columns 8 i + 2 (t % 4) + {0, 1}.
 __device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
@@ -220,6 +233,11 @@ __device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_16x256b_x2(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
 }
 // Four 8 x 8 blocks: register i of thread t holds (row t / 4, columns 2 (t % 4) + {0, 1}) of block i, lane 8 i + r gives
 // the address of its row r.
@@ -234,22 +252,20 @@ __device__ __forceinline__ void stsm_x4_t(uint32_t addr, uint32_t r0, uint32_t r
 }
 __device__ __forceinline__ float2 bf2_to_f2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 
-// Bounded wait of a whole warp, which leaves it together (the vote makes the outcome uniform).  Kept short, it is
-// there 25 times: the clock is looked at every 1024 tries only, and the caller reports.
+// Bounded wait of a whole warp (about a second), which leaves it together: the vote makes the outcome uniform.  Kept
+// short, for it is there 30 times and the roles' loops share the instruction cache; the caller reports.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
-        "{\n.reg .pred p;\n.reg .u32 n;\n.reg .u64 t, e;\n"
-        "mov.u32 n, 0;\nmov.u64 e, 0;\n"
+        "{\n.reg .pred p;\n.reg .u32 t, t0;\n"
+        "mov.u32 t0, %%clock;\n"
         "LOOP:\n"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n@p bra DONE;\n"
-        "add.u32 n, n, 1;\nand.b32 %0, n, 1023;\nsetp.ne.u32 p, %0, 0;\n@p bra LOOP;\n"
-        "mov.u64 t, %%globaltimer;\nsetp.eq.u64 p, e, 0;\n@p add.u64 e, t, %3;\n"
-        "setp.lt.u64 p, t, e;\n@p bra LOOP;\n"  // falls through with p false: gave up
+        "mov.u32 t, %%clock;\nsub.u32 t, t, t0;\nsetp.lt.u32 p, t, 0x78000000;\n@p bra LOOP;\n"  // falls through with p false
         "DONE:\n"
         "selp.u32 %0, 1, 0, p;\n}\n"
         : "=&r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "n"(kWaitLimitNs)
+        : "r"(smem_u32(bar)), "r"(parity)
         : "memory");
     return __all_sync(0xffffffffu, ok);
 }
@@ -286,7 +302,7 @@ __device__ __forceinline__ bool role_load(const LinearPrefillArgs& p, const Line
             if (one) {
                 unsigned char* st = x.sm + s * kStage;
                 mbar_arrive_expect_tx(&x.b->full[s], kOut ? 49152 : 32768);
-#pragma unroll
+#pragma unroll 1
                 for (int a = 0; a < 2; ++a) {
                     if (kOut) tma_load_3d(st + kOffQ + a * kAtom, &maps.q, 64 * a, hq, t0, &x.b->full[s]);
                     tma_load_3d(st + kOffK + a * kAtom, &maps.k, 64 * a, hq, t0, &x.b->full[s]);
@@ -304,7 +320,10 @@ __device__ __forceinline__ bool role_load(const LinearPrefillArgs& p, const Line
     return true;
 }
 
-// Warp 2: prefix and suffix sums of every chunk's log decays, two tokens a lane.
+// Warp 2: prefix and suffix sums of every chunk's log decays (base 2 from here on), two tokens a lane.  The state in TMEM
+// is S 2^-X: as long as -8 <= X <= 8 a chunk's decay only moves X (its own tokens enter times 2^-(G_j + X)), so the state
+// is not touched; beyond that it is multiplied by 2^(X + G_C) and X is 0 again.  The exponents stay small, so fp32 holds
+// them to 2^-21.
 __device__ __forceinline__ bool role_gates(const LinearPrefillArgs& p, const LinCtx& x) {
     using namespace lin;
     const int lane = threadIdx.x & 31;
@@ -314,14 +333,15 @@ __device__ __forceinline__ bool role_gates(const LinearPrefillArgs& p, const Lin
 #pragma unroll 1
     while (w.next(p, pc)) {
         if (pc.e <= pc.s) continue;
+        float X = 0.f;
 #pragma unroll 1
         for (int c = pc.ca; c < pc.cb; ++c, ++g) {
             const int t0 = pc.s + c * C, L = min(C, pc.e - t0);
             float a0 = 0.f, a1 = 0.f;
             if (2 * lane < L) a0 = p.decay[p.per_token ? (size_t)(t0 + 2 * lane) * p.HV + pc.hv : pc.hv];
             if (2 * lane + 1 < L) a1 = p.decay[p.per_token ? (size_t)(t0 + 2 * lane + 1) * p.HV + pc.hv : pc.hv];
-            a0 = a0 < kMinDecay ? kMinDecay : a0;
-            a1 = a1 < kMinDecay ? kMinDecay : a1;
+            a0 = (a0 < kMinDecay ? kMinDecay : a0) * kLog2e;
+            a1 = (a1 < kMinDecay ? kMinDecay : a1) * kLog2e;
             float pre = a0 + a1, suf = a0 + a1;
 #pragma unroll 1
             for (int off = 1; off < 32; off <<= 1) {
@@ -332,15 +352,24 @@ __device__ __forceinline__ bool role_gates(const LinearPrefillArgs& p, const Lin
             float before = __shfl_up_sync(0xffffffffu, pre, 1), after = __shfl_down_sync(0xffffffffu, suf, 1);
             if (lane == 0) before = 0.f;
             if (lane == 31) after = 0.f;
+            const float total = __shfl_sync(0xffffffffu, pre, 31), g0 = before + a0, gb = __shfl_sync(0xffffffffu, pre, lane | 7);
+            const bool scale = fabsf(X + total) > 8.f;
             // the last group to finish chunk g - 7 has finished g - 8 for all the others: the slot is free
             if (g >= kGates) LIN_WAIT(x.b->g_empty[(g + 1) % kGates], (g + 1) / kGates - 1);
             float* gt = reinterpret_cast<float*>(x.sm + kOffG) + (g % kGates) * kGateFloats;
-            const float g0 = before + a0;
-            *reinterpret_cast<float2*>(gt + 2 * lane) = make_float2(g0 * kLog2e, pre * kLog2e);
-            *reinterpret_cast<float2*>(gt + 64 + 2 * lane) = make_float2(p.scale * lin_ex2(g0 * kLog2e), p.scale * lin_ex2(pre * kLog2e));
-            // e^{G_C - G_j} from the sum of the later decays: exact where it matters, near the chunk's end
-            *reinterpret_cast<float2*>(gt + 128 + 2 * lane) = make_float2(expf(after + a1), expf(after));
-            if (lane == 31) gt[192] = expf(pre);
+            *reinterpret_cast<float2*>(gt + 2 * lane) = make_float2(g0, pre);
+            *reinterpret_cast<float2*>(gt + 64 + 2 * lane) = make_float2(p.scale * lin_ex2(g0 + X), p.scale * lin_ex2(pre + X));
+            // 2^(G_C - G_j) from the sum of the later decays: exact where it matters, near the chunk's end
+            *reinterpret_cast<float2*>(gt + 128 + 2 * lane) =
+                scale ? make_float2(lin_ex2(after + a1), lin_ex2(after)) : make_float2(lin_ex2(-(g0 + X)), lin_ex2(-(pre + X)));
+            *reinterpret_cast<float2*>(gt + 192 + 2 * lane) = make_float2(lin_ex2(gb - g0), lin_ex2(gb - pre));
+            if (lane == 0) gt[256] = scale ? lin_ex2(X + total) : 1.f;  // what the state is multiplied by
+            X = scale ? 0.f : X + total;
+            if (lane == 0) {
+                gt[257] = lin_ex2(X);      // of the state at the chunk's end
+                gt[258] = lin_ex2(total);  // the chunk's decay
+                gt[259] = scale ? 1.f : 0.f;
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(&x.b->g_full[g % kGates]);
         }
@@ -348,72 +377,84 @@ __device__ __forceinline__ bool role_gates(const LinearPrefillArgs& p, const Lin
     return true;
 }
 
-// Warp 1: all tensor-core products.
-template <bool kOut>
-__device__ __forceinline__ bool role_mma(const LinearPrefillArgs& p, const LinCtx& x, uint32_t one) {
-    using namespace lin;
-    Walk w = x.walk;
+__device__ __forceinline__ int count_chunks(const LinearPrefillArgs& p, Walk w) {
     Piece pc;
     int total = 0;
 #pragma unroll 1
     while (w.next(p, pc))
         if (pc.e > pc.s) total += pc.cb - pc.ca;
-    total = __shfl_sync(0xffffffffu, total, 0);
-    constexpr uint32_t idesc_qk = umma_idesc_bf16(64, 64, false, false), idesc_oi = umma_idesc_bf16(128, 64, false, false);
-    constexpr uint32_t idesc_oa = umma_idesc_bf16(128, 64, true, false), idesc_u = umma_idesc_bf16(128, 128, false, true);
-    // descriptors at stage 0; an offset adds its sixteenth
-    const uint32_t d_q = desc_low(x.sbase + kOffQ, 16), d_k = desc_low(x.sbase + kOffK, 16);
-    const uint32_t d_ku = desc_low(x.sbase + kOffK, kAtom), d_v = desc_low(x.sbase + kOffV, 8192), d_p = desc_low(x.sbase + kOffP, 16);
-    auto step = [](int kk) { return (uint32_t)(((kk >> 2) * kAtom + (kk & 3) * 32) >> 4); };  // 16 of 128 columns
-    auto qk = [&](uint32_t st) {
-        mma_ss<false>(one, x.tmem + kColQK, d_q + st, d_k + st, idesc_qk);
-#pragma unroll
-        for (int kk = 1; kk < 8; ++kk) mma_ss<true>(one, x.tmem + kColQK, d_q + st + step(kk), d_k + st + step(kk), idesc_qk);
-        commit_one(one, &x.b->qk_full);
-    };
-    int s = 0, s_ph = 0;  // stage of chunk g and its phase
-    const uint32_t kStep = kStage >> 4;
-    if (total > 0) LIN_WAIT(x.b->full[0], 0);
-    tc_fence_after();
-    if (kOut && total > 0) qk(0);
+    return __shfl_sync(0xffffffffu, total, 0);
+}
+
+// Warp 1: the products U, which the chain over chunks goes through.
+__device__ __forceinline__ bool role_u(const LinearPrefillArgs& p, const LinCtx& x, uint32_t one) {
+    using namespace lin;
+    const int total = count_chunks(p, x.walk);
+    constexpr uint32_t idesc = umma_idesc_bf16(128, 128, false, true);
+    const uint32_t d_k = desc_low(x.sbase + kOffK, kAtom);  // at stage 0; an offset adds its sixteenth
+    int s = 0;
 #pragma unroll 1
     for (int g = 0; g < total; ++g) {
-        const uint32_t st = (uint32_t)s * kStep, ph = g & 1;
-        const int sn = s + 1 == kStages ? 0 : s + 1, sn_ph = sn ? s_ph : s_ph ^ 1;
-        LIN_WAIT(x.b->v_full, ph);
-        LIN_WAIT(x.b->s_full, ph);
+        const uint32_t st = (uint32_t)s * (kStage >> 4);
+        LIN_WAIT(x.b->u_ready, g);
         tc_fence_after();
-        // the chain over chunks goes through this product: it is issued first
 #pragma unroll
-        for (int kk = 0; kk < 12; ++kk) mma_ts<true>(one, x.tmem + kColS, x.tmem + kColV + 8 * kk, d_ku + st + 128 * (kk & 3), idesc_u);
+        for (int kk = 0; kk < 12; ++kk) mma_ts<true>(one, x.tmem + kColS, x.tmem + kColV + 8 * kk, d_k + st + 128 * (kk & 3), idesc);
         commit_one(one, &x.b->u_full);
-        if (kOut) {
-            if (g > 0) LIN_WAIT(x.b->o_empty, ph ^ 1);
+        commit_one(one, &x.b->empty[s]);
+        if (++s == kStages) s = 0;
+    }
+    return true;
+}
+
+// Warp 3: the products of the output.
+__device__ __forceinline__ bool role_mma(const LinearPrefillArgs& p, const LinCtx& x, uint32_t one) {
+    using namespace lin;
+    const int total = count_chunks(p, x.walk);
+    constexpr uint32_t idesc_qk = umma_idesc_bf16(64, 64, false, false), idesc_oi = umma_idesc_bf16(128, 64, false, false);
+    constexpr uint32_t idesc_oa = umma_idesc_bf16(128, 64, true, false);
+    // descriptors at stage 0; an offset adds its sixteenth
+    const uint32_t d_q = desc_low(x.sbase + kOffQ, 16), d_k = desc_low(x.sbase + kOffK, 16);
+    const uint32_t d_v = desc_low(x.sbase + kOffV, 8192), d_p = desc_low(x.sbase + kOffP, 16);
+    auto step = [](int kk) { return (uint32_t)(((kk >> 2) * kAtom + (kk & 3) * 32) >> 4); };  // 16 of 128 columns
+    int s = 0, sn = 0, sn_ph = 0;  // stages of chunk g and of the next QK, and the latter's phase
+#pragma unroll 1
+    for (int g = -1; g < total; ++g) {
+        const uint32_t st = (uint32_t)s * (kStage >> 4), pb = d_p + (uint32_t)(g & 1) * 512u;
+        if (g >= 0) {
+            LIN_WAIT(x.b->b_ready, g);  // the state's bf16 copy
+            if (g > 0) LIN_WAIT(x.b->o_empty, g - 1);
             tc_fence_after();
             mma_ts<false>(one, x.tmem + kColI, x.tmem + kColB, d_q + st, idesc_oi);
 #pragma unroll
             for (int kk = 1; kk < 8; ++kk) mma_ts<true>(one, x.tmem + kColI, x.tmem + kColB + 8 * kk, d_q + st + step(kk), idesc_oi);
             commit_one(one, &x.b->i_full);
-            if (g + 1 < total) {  // ahead of OA, so that the P warps have chunk g + 1 while the tensor core ends g
-                LIN_WAIT(x.b->full[sn], sn_ph);
-                LIN_WAIT(x.b->qk_empty, ph);
-                tc_fence_after();
-                qk((uint32_t)sn * kStep);
-            }
-            LIN_WAIT(x.b->p_full[ph], g >> 1);
+        }
+        if (g + 1 < total) {  // QK of the next chunk, so that the P warps are ahead
+            LIN_WAIT(x.b->full[sn], sn_ph);
+            if (g >= 0) LIN_WAIT(x.b->qk_empty, g);
             tc_fence_after();
-            const uint32_t pb = d_p + ph * 512u;
+            const uint32_t st1 = (uint32_t)sn * (kStage >> 4);
+            mma_ss<false>(one, x.tmem + kColQK, d_q + st1, d_k + st1, idesc_qk);
+#pragma unroll
+            for (int kk = 1; kk < 8; ++kk) mma_ss<true>(one, x.tmem + kColQK, d_q + st1 + step(kk), d_k + st1 + step(kk), idesc_qk);
+            commit_one(one, &x.b->qk_full);
+            if (++sn == kStages) {
+                sn = 0;
+                sn_ph ^= 1;
+            }
+        }
+        if (g >= 0) {
+            LIN_WAIT(x.b->p_full[g & 1], g >> 1);
+            tc_fence_after();
             mma_ss<false>(one, x.tmem + kColA, d_v + st, pb, idesc_oa);
 #pragma unroll
             for (int kk = 1; kk < 4; ++kk) mma_ss<true>(one, x.tmem + kColA, d_v + st + 128 * kk, pb + 2 * kk, idesc_oa);
-            commit_one(one, &x.b->p_empty[ph]);
             commit_one(one, &x.b->o_full);
-        } else if (g + 1 < total) {
-            LIN_WAIT(x.b->full[sn], sn_ph);
+            commit_one(one, &x.b->p_empty[g & 1]);
+            commit_one(one, &x.b->empty[s]);
+            if (++s == kStages) s = 0;
         }
-        commit_one(one, &x.b->empty[s]);
-        s = sn;
-        s_ph = sn_ph;
     }
     return true;
 }
@@ -441,34 +482,41 @@ __device__ __forceinline__ bool role_p(const LinearPrefillArgs& p, const LinCtx&
             const float2 gi = make_float2(g2[r], g2[r + 8]);
             LIN_WAIT(x.b->qk_full, g);
             tc_fence_after();
-            uint32_t d[2][16];
-            tmem_ld_16x256b_x4(tl, d[0]);
-            tmem_ld_16x256b_x4(tl + 32, d[1]);
-            tmem_ld_wait();
-            tmem_regs_ready_n(d[0]);
-            tmem_regs_ready_n(d[1]);
-            tc_fence_before();
-            mbar_arrive(&x.b->qk_empty);
             if (g >= 2) LIN_WAIT(x.b->p_empty[g & 1], (g >> 1) - 1);
+#pragma unroll 1
+            for (int b = 0; b <= quarter; ++b) {  // 16 columns
+                uint32_t d[8], o[4];
+                tmem_ld_16x256b_x2(tl + 16 * b, d);
+                // e^{G_i - G_j} = e^{G_i - G_b} e^{G_b - G_j} below the diagonal (both factors <= 1), directly on it
+                const bool diag = b == quarter;
+                const float gb = g2[16 * b + 15];
+                const float2 rf = diag ? gi : make_float2(lin_ex2(gi.x - gb), lin_ex2(gi.y - gb));
+                const int j0 = 16 * b + 2 * (lane & 3);
+                const float2 c0 = *reinterpret_cast<const float2*>(g2 + (diag ? 0 : 192) + j0);
+                const float2 c1 = *reinterpret_cast<const float2*>(g2 + (diag ? 0 : 192) + j0 + 8);
+                float2 f[4] = {mul2(make_float2(rf.x, rf.x), c0), mul2(make_float2(rf.y, rf.y), c0),
+                               mul2(make_float2(rf.x, rf.x), c1), mul2(make_float2(rf.y, rf.y), c1)};
+                if (diag) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {  // 16 columns
-                if (b > quarter) break;
-                uint32_t o[4];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {  // 8 columns
-                    const float2 gj = *reinterpret_cast<const float2*>(g2 + 16 * b + 8 * i + 2 * (lane & 3));
-                    const int j = 16 * b + 8 * i + 2 * (lane & 3);
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {  // rows r, r + 8
-                        const float gr = k ? gi.y : gi.x;
-                        const uint32_t* e = &d[b >> 1][8 * (b & 1) + 4 * i + 2 * k];
-                        const float y = __uint_as_float(e[0]) * lin_ex2(gr - gj.x), z = __uint_as_float(e[1]) * lin_ex2(gr - gj.y);
-                        const int lim = min(r + 8 * k, L - 1);
-                        o[2 * i + k] = pack_bf16x2(j <= lim ? y : 0.f, j + 1 <= lim ? z : 0.f);
+                    for (int i = 0; i < 4; ++i) {  // columns j0 (+ 8), rows r (+ 8)
+                        const float2 c = i < 2 ? c0 : c1;
+                        const float fr = i & 1 ? rf.y : rf.x;
+                        f[i] = make_float2(lin_ex2(fr - c.x), lin_ex2(fr - c.y));
                     }
+                }
+                tmem_ld_wait();
+                tmem_regs_ready_n(d);
+                // kept: columns on or below the diagonal, and not behind the segment's end (k rows of another sequence)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = j0 + 8 * (i >> 1), lim = min(r + 8 * (i & 1), L - 1);
+                    const float2 y = mul2(f[i], make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])));
+                    o[i] = pack_bf16x2(j <= lim ? y.x : 0.f, j + 1 <= lim ? y.y : 0.f);
                 }
                 stsm_x4(row + (uint32_t)(g & 1) * 8192 + ((((uint32_t)(2 * b) + (lane >> 4)) ^ sw) << 4), o[0], o[1], o[2], o[3]);
             }
+            tc_fence_before();
+            mbar_arrive(&x.b->qk_empty);
             fence_async_smem();
             mbar_arrive(&x.b->p_full[g & 1]);
         }
@@ -509,28 +557,27 @@ __device__ __forceinline__ bool role_v(const LinearPrefillArgs& p, const LinCtx&
                 fence_async_smem();
                 named_bar_sync(1, 256);
             }
-            uint32_t part[3][16];
-#pragma unroll
+            if (g > 0) LIN_WAIT(x.b->u_full, g - 1);  // the parts of the chunk before are consumed
+            tc_fence_after();
+#pragma unroll 1
             for (int i = 0; i < 4; ++i) {  // 16 V x 16 tokens, transposed
-                uint32_t raw[4];
+                uint32_t raw[4], part[3][4];
                 ldsm_x4_t(raw[0], raw[1], raw[2], raw[3], st + from + 2048 * i);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {  // {0, 1}: tokens 16 i + .., {2, 3}: 8 later; odd ones are 8 V further
                     float2 y = mul2(bf2_to_f2(raw[j]), *reinterpret_cast<const float2*>(er + 16 * i + 8 * (j >> 1)));
 #pragma unroll
                     for (int k = 0; k < 3; ++k) {
-                        part[k][4 * i + j] = pack_bf16x2(y.x, y.y);
-                        if (k < 2) y = sub2(y, bf2_to_f2(part[k][4 * i + j]));
+                        part[k][j] = pack_bf16x2(y.x, y.y);
+                        if (k < 2) y = sub2(y, bf2_to_f2(part[k][j]));
                     }
                 }
-            }
-            if (g > 0) LIN_WAIT(x.b->u_full, g - 1);  // the parts of the chunk before are consumed
-            tc_fence_after();
 #pragma unroll
-            for (int k = 0; k < 3; ++k) tmem_st_16x128b_x8(tl + 32 * k, part[k]);
+                for (int k = 0; k < 3; ++k) tmem_st_16x128b_x2(tl + 32 * k + 8 * i, part[k]);
+            }
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(&x.b->v_full);
+            mbar_arrive(&x.b->u_ready);
         }
     }
     return true;
@@ -563,7 +610,7 @@ __device__ __forceinline__ bool role_o(const LinearPrefillArgs& p, const LinearM
                 float2 e2[4];  // tokens 8 i + 2 (lane % 4) and the next
 #pragma unroll
                 for (int i = 0; i < 4; ++i) e2[i] = *reinterpret_cast<const float2*>(eg + 32 * th + 8 * i + 2 * (lane & 3));
-#pragma unroll
+#pragma unroll 1
                 for (int hf = 0; hf < 2; ++hf) {  // 16 V
                     uint32_t y[16], z[16];
                     const uint32_t ta = tl + ((uint32_t)(16 * hf) << 16) + 32 * th;
@@ -613,7 +660,7 @@ __device__ __forceinline__ bool role_o(const LinearPrefillArgs& p, const LinearM
 }
 
 // Warps 20-23: the state, V row r a thread.  It lives in TMEM, where U adds to it: before U of chunk g the warps read
-// it, leave its bf16 copy for OI and write it back times e^{G_C}.
+// it and leave its bf16 copy for OI; now and then (see the gates) they write it back in another unit.
 template <bool kOut>
 __device__ __forceinline__ bool role_s(const LinearPrefillArgs& p, const LinCtx& x) {
     using namespace lin;
@@ -640,52 +687,64 @@ __device__ __forceinline__ bool role_s(const LinearPrefillArgs& p, const LinCtx&
                 reinterpret_cast<float4*>(dst)[j] = src ? reinterpret_cast<const float4*>(src)[j] : make_float4(0.f, 0.f, 0.f, 0.f);
             continue;
         }
-        float gamma = 1.f;
+        float gamma = 1.f, unit = 1.f;
 #pragma unroll 1
         for (int c = pc.ca; c < pc.cb; ++c, ++g) {
             const float* gt = reinterpret_cast<const float*>(x.sm + kOffG) + (g % kGates) * kGateFloats;
             LIN_WAIT(x.b->g_full[g % kGates], g / kGates);
-            const float el = gt[192];
-            gamma *= el;
-            const bool begins = c == pc.ca;
+            const float factor = gt[256];
+            unit = gt[257];
+            gamma *= gt[258];
+            const bool begins = c == pc.ca, write = begins || gt[259] != 0.f;
             if (g > 0) {
                 // the state is complete (or, at a segment's start, was read) and OI has read its copy
                 LIN_WAIT(x.b->u_full, g - 1);
                 if (kOut) LIN_WAIT(x.b->i_full, g - 1);
             }
             tc_fence_after();
+            if (kOut || write) {
 #pragma unroll 1
-            for (int b = 0; b < 4; ++b) {  // 32 K
-                uint32_t d[32], o[16];
-                if (begins) {
+                for (int b = 0; b < 4; ++b) {  // 32 K
+                    uint32_t d[32];
+                    if (begins) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float4 y = src ? *reinterpret_cast<const float4*>(src + (size_t)r * kD + 32 * b + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        d[4 * j] = __float_as_uint(y.x);
-                        d[4 * j + 1] = __float_as_uint(y.y);
-                        d[4 * j + 2] = __float_as_uint(y.z);
-                        d[4 * j + 3] = __float_as_uint(y.w);
+                        for (int j = 0; j < 8; ++j) {
+                            const float4 y = src ? *reinterpret_cast<const float4*>(src + (size_t)r * kD + 32 * b + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            d[4 * j] = __float_as_uint(y.x);
+                            d[4 * j + 1] = __float_as_uint(y.y);
+                            d[4 * j + 2] = __float_as_uint(y.z);
+                            d[4 * j + 3] = __float_as_uint(y.w);
+                        }
+                    } else {
+                        tmem_ld32_async(tl + kColS + 32 * b, d);
+                        tmem_ld_wait();
+                        tmem_regs_ready(d);
                     }
-                } else {
-                    tmem_ld32_async(tl + kColS + 32 * b, d);
-                    tmem_ld_wait();
-                    tmem_regs_ready(d);
-                }
+                    if (kOut) {
+                        uint32_t o[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float2 y = make_float2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1]));
-                    if (kOut) o[j] = pack_bf16x2(y.x, y.y);
-                    const float2 z = mul2(y, make_float2(el, el));
-                    d[2 * j] = __float_as_uint(z.x);
-                    d[2 * j + 1] = __float_as_uint(z.y);
+                        for (int j = 0; j < 16; ++j) o[j] = pack_bf16x2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1]));
+                        tmem_st16(tl + kColB + 16 * b, o);
+                    }
+                    if (write) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            const float2 z = mul2(make_float2(__uint_as_float(d[j]), __uint_as_float(d[j + 1])), make_float2(factor, factor));
+                            d[j] = __float_as_uint(z.x);
+                            d[j + 1] = __float_as_uint(z.y);
+                        }
+                        tmem_st32(tl + kColS + 32 * b, d);
+                    }
                 }
-                tmem_st32(tl + kColS + 32 * b, d);
-                if (kOut) tmem_st16(tl + kColB + 16 * b, o);
+                if (write) tmem_st_wait();
             }
-            tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(&x.b->s_full);
-            if (!kOut) {
+            mbar_arrive(&x.b->u_ready);  // U may add to the state
+            if (kOut) {
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&x.b->b_ready);
+            } else {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&x.b->g_empty[g % kGates]);
             }
@@ -700,8 +759,10 @@ __device__ __forceinline__ bool role_s(const LinearPrefillArgs& p, const LinCtx&
                 tmem_ld_wait();
                 tmem_regs_ready(d);
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    *reinterpret_cast<uint4*>(dst + (size_t)r * kD + 32 * b + 4 * j) = make_uint4(d[4 * j], d[4 * j + 1], d[4 * j + 2], d[4 * j + 3]);
+                for (int j = 0; j < 32; j += 4)
+                    *reinterpret_cast<float4*>(dst + (size_t)r * kD + 32 * b + j) =
+                        make_float4(unit * __uint_as_float(d[j]), unit * __uint_as_float(d[j + 1]), unit * __uint_as_float(d[j + 2]),
+                                    unit * __uint_as_float(d[j + 3]));
             }
             if (!kOut && r == 0) p.gamma[blockIdx.x] = gamma;
         }
@@ -725,7 +786,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&b->full[s], 1);
-            mbar_init(&b->empty[s], 1);
+            mbar_init(&b->empty[s], kOut ? 2 : 1);
         }
         for (int s = 0; s < kGates; ++s) {
             mbar_init(&b->g_full[s], 1);
@@ -733,17 +794,18 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         }
         mbar_init(&b->qk_full, 1);
         mbar_init(&b->qk_empty, 128);
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(&b->p_full[s], 128);
-            mbar_init(&b->p_empty[s], 1);
-        }
-        mbar_init(&b->v_full, 256);
+        mbar_init(&b->u_ready, 256 + 128);  // V and S warps
         mbar_init(&b->u_full, 1);
-        mbar_init(&b->s_full, 128);
+        mbar_init(&b->p_full[0], 128);
+        mbar_init(&b->p_full[1], 128);
+        mbar_init(&b->p_empty[0], 1);
+        mbar_init(&b->p_empty[1], 1);
+        mbar_init(&b->b_ready, 128);
         mbar_init(&b->i_full, 1);
-        mbar_init(&b->o_full, 1);
         mbar_init(&b->o_empty, 128);
-        mbar_init(&b->done, 1);
+        mbar_init(&b->o_full, 1);
+        mbar_init(&b->done[0], 1);
+        mbar_init(&b->done[1], 1);
         mbar_fence_init();
     }
     pdl_wait();
@@ -782,12 +844,12 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         if (!(ok = role_load<kOut>(p, maps, x, elect_one(), &issued)))
             // gave up: let copies already in flight land (bounded) before the CTA exits
             for (int g = max(0, issued - kStages); g < issued; ++g) warp_wait(&b->full[g % kStages], (uint32_t)((g / kStages) & 1));
-    } else if (warp == 1) {
+    } else if (warp == 1 || (kOut && warp == 3)) {
         const uint32_t one = elect_one();
-        ok = role_mma<kOut>(p, x, one);
+        ok = warp == 1 ? role_u(p, x, one) : role_mma(p, x, one);
         // products still in flight end before the TMEM is given back
-        commit_one(one, &b->done);
-        ok = warp_wait(&b->done, 0) && ok;
+        commit_one(one, &b->done[warp >> 1]);
+        ok = warp_wait(&b->done[warp >> 1], 0) && ok;
     } else if (warp == 2) {
         ok = role_gates(p, x);
     } else if (warp < 4) {
