@@ -44,7 +44,7 @@ constexpr uint32_t kOffG = kOffO + 2 * 16384;    // gates, kGates slots of f32: 
 constexpr uint32_t kGateFloats = 264;
 constexpr uint32_t kOffBar = kOffG + kGates * kGateFloats * 4;
 constexpr uint32_t kOffRange = kOffBar + 512;
-constexpr uint32_t kSmem = kOffRange + 256 + 1024;
+constexpr uint32_t kSmem = kOffRange + 256;
 constexpr uint32_t kTmemCols = 512;
 // accumulators QK, OI, OA and the state S in fp32, then its bf16 copy and the three parts of the decayed v
 constexpr uint32_t kColQK = 0, kColI = 64, kColA = 128, kColS = 192, kColB = 320, kColV = 384;
@@ -252,9 +252,9 @@ __device__ __forceinline__ void stsm_x4_t(uint32_t addr, uint32_t r0, uint32_t r
 }
 __device__ __forceinline__ float2 bf2_to_f2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 
-// Bounded wait of a whole warp (about a second), which leaves it together: the vote makes the outcome uniform.  Kept
-// short, for it is there 30 times and the roles' loops share the instruction cache; the caller reports.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+// Bounded wait (about a second); false when it gave up.  Kept short and free of branches of its own, for it is there 30
+// times and the roles' loops share the instruction cache: a role looks at the results once a chunk.
+__device__ __forceinline__ uint32_t lin_wait(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n.reg .pred p;\n.reg .u32 t, t0;\n"
@@ -264,25 +264,32 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
         "mov.u32 t, %%clock;\nsub.u32 t, t, t0;\nsetp.lt.u32 p, t, 0x78000000;\n@p bra LOOP;\n"  // falls through with p false
         "DONE:\n"
         "selp.u32 %0, 1, 0, p;\n}\n"
-        : "=&r"(ok)
+        : "=r"(ok)
         : "r"(smem_u32(bar)), "r"(parity)
         : "memory");
-    return __all_sync(0xffffffffu, ok);
+    return ok;
+}
+
+// The kernel's shared memory.  Named directly everywhere, so that every access is a shared-memory one with a
+// constant offset; the kernel checks the alignment that the swizzled tiles need.
+extern __shared__ __align__(1024) unsigned char lin_sm[];
+__device__ __forceinline__ lin::Bars* lin_bars() { return reinterpret_cast<lin::Bars*>(lin_sm + lin::kOffBar); }
+__device__ __forceinline__ float* lin_gates(uint32_t g) {
+    return reinterpret_cast<float*>(lin_sm + lin::kOffG + (g % lin::kGates) * (lin::kGateFloats * 4));
 }
 
 struct LinCtx {
-    unsigned char* sm;
     uint32_t sbase;
     static constexpr uint32_t tmem = 0;  // a CTA that holds all 512 columns holds them from column 0
-    lin::Bars* b;
     Walk walk;
     int prev;  // the CTA's slot of segment states is blockIdx.x; a stretch that begins inside a segment starts from `prev`
 };
 
 // ---- roles ----------------------------------------------------------------------------------
-// Every wait is bounded; on expiry the role returns false, and the others' waits expire in turn.
-#define LIN_WAIT(bar, parity) \
-    if (!warp_wait(&(bar), (uint32_t)(parity) & 1u)) return false
+// Every wait is bounded; on expiry the role ends at the end of its chunk, and the others' waits expire in turn.
+#define LIN_WAIT(bar, parity) ok &= lin_wait(&(bar), (uint32_t)(parity) & 1u)
+#define LIN_CHECK() \
+    if (!__all_sync(0xffffffffu, ok)) return false
 
 // Warp 0: the TMA copies.
 template <bool kOut>
@@ -290,7 +297,7 @@ __device__ __forceinline__ bool role_load(const LinearPrefillArgs& p, const Line
     using namespace lin;
     Walk w = x.walk;
     Piece pc;
-    int s = 0, s_ph = 1;
+    uint32_t s = 0, s_ph = 1, ok = 1;
 #pragma unroll 1
     while (w.next(p, pc)) {
         if (pc.e <= pc.s) continue;
@@ -298,15 +305,16 @@ __device__ __forceinline__ bool role_load(const LinearPrefillArgs& p, const Line
 #pragma unroll 1
         for (int c = pc.ca; c < pc.cb; ++c) {
             const int t0 = pc.s + c * C;
-            LIN_WAIT(x.b->empty[s], s_ph);  // (the first round passes: the barriers are new)
+            LIN_WAIT(lin_bars()->empty[s], s_ph);  // (the first round passes: the barriers are new)
+            LIN_CHECK();
             if (one) {
-                unsigned char* st = x.sm + s * kStage;
-                mbar_arrive_expect_tx(&x.b->full[s], kOut ? 49152 : 32768);
+                unsigned char* st = lin_sm + s * kStage;
+                mbar_arrive_expect_tx(&lin_bars()->full[s], kOut ? 49152 : 32768);
 #pragma unroll 1
                 for (int a = 0; a < 2; ++a) {
-                    if (kOut) tma_load_3d(st + kOffQ + a * kAtom, &maps.q, 64 * a, hq, t0, &x.b->full[s]);
-                    tma_load_3d(st + kOffK + a * kAtom, &maps.k, 64 * a, hq, t0, &x.b->full[s]);
-                    tma_load_3d(st + kOffV + a * 8192, &maps.v, 64 * a, pc.hv, t0, &x.b->full[s]);
+                    if (kOut) tma_load_3d(st + kOffQ + a * kAtom, &maps.q, 64 * a, hq, t0, &lin_bars()->full[s]);
+                    tma_load_3d(st + kOffK + a * kAtom, &maps.k, 64 * a, hq, t0, &lin_bars()->full[s]);
+                    tma_load_3d(st + kOffV + a * 8192, &maps.v, 64 * a, pc.hv, t0, &lin_bars()->full[s]);
                 }
             }
             __syncwarp();
@@ -329,7 +337,7 @@ __device__ __forceinline__ bool role_gates(const LinearPrefillArgs& p, const Lin
     const int lane = threadIdx.x & 31;
     Walk w = x.walk;
     Piece pc;
-    int g = 0;
+    uint32_t g = 0, ok = 1;
 #pragma unroll 1
     while (w.next(p, pc)) {
         if (pc.e <= pc.s) continue;
@@ -355,8 +363,8 @@ __device__ __forceinline__ bool role_gates(const LinearPrefillArgs& p, const Lin
             const float total = __shfl_sync(0xffffffffu, pre, 31), g0 = before + a0, gb = __shfl_sync(0xffffffffu, pre, lane | 7);
             const bool scale = fabsf(X + total) > 8.f;
             // the last group to finish chunk g - 7 has finished g - 8 for all the others: the slot is free
-            if (g >= kGates) LIN_WAIT(x.b->g_empty[(g + 1) % kGates], (g + 1) / kGates - 1);
-            float* gt = reinterpret_cast<float*>(x.sm + kOffG) + (g % kGates) * kGateFloats;
+            if (g >= kGates) LIN_WAIT(lin_bars()->g_empty[(g + 1) % kGates], (g + 1) / kGates - 1);
+            float* gt = lin_gates(g);
             *reinterpret_cast<float2*>(gt + 2 * lane) = make_float2(g0, pre);
             *reinterpret_cast<float2*>(gt + 64 + 2 * lane) = make_float2(p.scale * lin_ex2(g0 + X), p.scale * lin_ex2(pre + X));
             // 2^(G_C - G_j) from the sum of the later decays: exact where it matters, near the chunk's end
@@ -371,7 +379,8 @@ __device__ __forceinline__ bool role_gates(const LinearPrefillArgs& p, const Lin
                 gt[259] = scale ? 1.f : 0.f;
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&x.b->g_full[g % kGates]);
+            if (lane == 0) mbar_arrive(&lin_bars()->g_full[g % kGates]);
+            LIN_CHECK();
         }
     }
     return true;
@@ -392,17 +401,18 @@ __device__ __forceinline__ bool role_u(const LinearPrefillArgs& p, const LinCtx&
     const int total = count_chunks(p, x.walk);
     constexpr uint32_t idesc = umma_idesc_bf16(128, 128, false, true);
     const uint32_t d_k = desc_low(x.sbase + kOffK, kAtom);  // at stage 0; an offset adds its sixteenth
-    int s = 0;
+    uint32_t s = 0, ok = 1;
 #pragma unroll 1
     for (int g = 0; g < total; ++g) {
         const uint32_t st = (uint32_t)s * (kStage >> 4);
-        LIN_WAIT(x.b->u_ready, g);
+        LIN_WAIT(lin_bars()->u_ready, g);
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < 12; ++kk) mma_ts<true>(one, x.tmem + kColS, x.tmem + kColV + 8 * kk, d_k + st + 128 * (kk & 3), idesc);
-        commit_one(one, &x.b->u_full);
-        commit_one(one, &x.b->empty[s]);
+        commit_one(one, &lin_bars()->u_full);
+        commit_one(one, &lin_bars()->empty[s]);
         if (++s == kStages) s = 0;
+        LIN_CHECK();
     }
     return true;
 }
@@ -417,44 +427,45 @@ __device__ __forceinline__ bool role_mma(const LinearPrefillArgs& p, const LinCt
     const uint32_t d_q = desc_low(x.sbase + kOffQ, 16), d_k = desc_low(x.sbase + kOffK, 16);
     const uint32_t d_v = desc_low(x.sbase + kOffV, 8192), d_p = desc_low(x.sbase + kOffP, 16);
     auto step = [](int kk) { return (uint32_t)(((kk >> 2) * kAtom + (kk & 3) * 32) >> 4); };  // 16 of 128 columns
-    int s = 0, sn = 0, sn_ph = 0;  // stages of chunk g and of the next QK, and the latter's phase
+    uint32_t s = 0, sn = 0, sn_ph = 0, ok = 1;  // stages of chunk g and of the next QK, and the latter's phase
 #pragma unroll 1
     for (int g = -1; g < total; ++g) {
         const uint32_t st = (uint32_t)s * (kStage >> 4), pb = d_p + (uint32_t)(g & 1) * 512u;
         if (g >= 0) {
-            LIN_WAIT(x.b->b_ready, g);  // the state's bf16 copy
-            if (g > 0) LIN_WAIT(x.b->o_empty, g - 1);
+            LIN_WAIT(lin_bars()->b_ready, g);  // the state's bf16 copy
+            if (g > 0) LIN_WAIT(lin_bars()->o_empty, g - 1);
             tc_fence_after();
             mma_ts<false>(one, x.tmem + kColI, x.tmem + kColB, d_q + st, idesc_oi);
 #pragma unroll
             for (int kk = 1; kk < 8; ++kk) mma_ts<true>(one, x.tmem + kColI, x.tmem + kColB + 8 * kk, d_q + st + step(kk), idesc_oi);
-            commit_one(one, &x.b->i_full);
+            commit_one(one, &lin_bars()->i_full);
         }
         if (g + 1 < total) {  // QK of the next chunk, so that the P warps are ahead
-            LIN_WAIT(x.b->full[sn], sn_ph);
-            if (g >= 0) LIN_WAIT(x.b->qk_empty, g);
+            LIN_WAIT(lin_bars()->full[sn], sn_ph);
+            if (g >= 0) LIN_WAIT(lin_bars()->qk_empty, g);
             tc_fence_after();
             const uint32_t st1 = (uint32_t)sn * (kStage >> 4);
             mma_ss<false>(one, x.tmem + kColQK, d_q + st1, d_k + st1, idesc_qk);
 #pragma unroll
             for (int kk = 1; kk < 8; ++kk) mma_ss<true>(one, x.tmem + kColQK, d_q + st1 + step(kk), d_k + st1 + step(kk), idesc_qk);
-            commit_one(one, &x.b->qk_full);
+            commit_one(one, &lin_bars()->qk_full);
             if (++sn == kStages) {
                 sn = 0;
                 sn_ph ^= 1;
             }
         }
         if (g >= 0) {
-            LIN_WAIT(x.b->p_full[g & 1], g >> 1);
+            LIN_WAIT(lin_bars()->p_full[g & 1], g >> 1);
             tc_fence_after();
             mma_ss<false>(one, x.tmem + kColA, d_v + st, pb, idesc_oa);
 #pragma unroll
             for (int kk = 1; kk < 4; ++kk) mma_ss<true>(one, x.tmem + kColA, d_v + st + 128 * kk, pb + 2 * kk, idesc_oa);
-            commit_one(one, &x.b->o_full);
-            commit_one(one, &x.b->p_empty[g & 1]);
-            commit_one(one, &x.b->empty[s]);
+            commit_one(one, &lin_bars()->o_full);
+            commit_one(one, &lin_bars()->p_empty[g & 1]);
+            commit_one(one, &lin_bars()->empty[s]);
             if (++s == kStages) s = 0;
         }
+        LIN_CHECK();
     }
     return true;
 }
@@ -470,19 +481,19 @@ __device__ __forceinline__ bool role_p(const LinearPrefillArgs& p, const LinCtx&
     const uint32_t row = x.sbase + kOffP + (uint32_t)(16 * quarter + (lane & 15)) * 128, sw = lane & 7;
     Walk w = x.walk;
     Piece pc;
-    int g = 0;
+    uint32_t g = 0, ok = 1;
 #pragma unroll 1
     while (w.next(p, pc)) {
         if (pc.e <= pc.s) continue;
 #pragma unroll 1
         for (int c = pc.ca; c < pc.cb; ++c, ++g) {
             const int L = min(C, pc.e - pc.s - c * C);
-            const float* g2 = reinterpret_cast<const float*>(x.sm + kOffG) + (g % kGates) * kGateFloats;
-            LIN_WAIT(x.b->g_full[g % kGates], g / kGates);
+            const float* g2 = lin_gates(g);
+            LIN_WAIT(lin_bars()->g_full[g % kGates], g / kGates);
             const float2 gi = make_float2(g2[r], g2[r + 8]);
-            LIN_WAIT(x.b->qk_full, g);
+            LIN_WAIT(lin_bars()->qk_full, g);
             tc_fence_after();
-            if (g >= 2) LIN_WAIT(x.b->p_empty[g & 1], (g >> 1) - 1);
+            if (g >= 2) LIN_WAIT(lin_bars()->p_empty[g & 1], (g >> 1) - 1);
 #pragma unroll 1
             for (int b = 0; b <= quarter; ++b) {  // 16 columns
                 uint32_t d[8], o[4];
@@ -516,9 +527,10 @@ __device__ __forceinline__ bool role_p(const LinearPrefillArgs& p, const LinCtx&
                 stsm_x4(row + (uint32_t)(g & 1) * 8192 + ((((uint32_t)(2 * b) + (lane >> 4)) ^ sw) << 4), o[0], o[1], o[2], o[3]);
             }
             tc_fence_before();
-            mbar_arrive(&x.b->qk_empty);
+            mbar_arrive(&lin_bars()->qk_empty);
             fence_async_smem();
-            mbar_arrive(&x.b->p_full[g & 1]);
+            mbar_arrive(&lin_bars()->p_full[g & 1]);
+            LIN_CHECK();
         }
     }
     return true;
@@ -535,17 +547,17 @@ __device__ __forceinline__ bool role_v(const LinearPrefillArgs& p, const LinCtx&
     const uint32_t from = kOffV + (uint32_t)(ch >> 3) * 8192 + (uint32_t)tok * 128 + (uint32_t)(((ch & 7) ^ (tok & 7)) << 4);
     Walk w = x.walk;
     Piece pc;
-    int g = 0;
+    uint32_t g = 0, s = 0, s_ph = 0, ok = 1;
 #pragma unroll 1
     while (w.next(p, pc)) {
         if (pc.e <= pc.s) continue;
 #pragma unroll 1
         for (int c = pc.ca; c < pc.cb; ++c, ++g) {
             const int L = min(C, pc.e - pc.s - c * C);
-            const float* er = reinterpret_cast<const float*>(x.sm + kOffG) + (g % kGates) * kGateFloats + 128 + 2 * (lane & 3);
-            LIN_WAIT(x.b->g_full[g % kGates], g / kGates);
-            LIN_WAIT(x.b->full[g % kStages], g / kStages);
-            unsigned char* st = x.sm + (g % kStages) * kStage;
+            const float* er = lin_gates(g) + 128 + 2 * (lane & 3);
+            LIN_WAIT(lin_bars()->g_full[g % kGates], g / kGates);
+            LIN_WAIT(lin_bars()->full[s], s_ph);
+            unsigned char* st = lin_sm + s * kStage;
             if (L < C) {
                 // Rows behind the segment's end hold another sequence's tokens, or zeros.  They become zero in v and
                 // k, so whatever they hold cannot reach a product.
@@ -557,7 +569,7 @@ __device__ __forceinline__ bool role_v(const LinearPrefillArgs& p, const LinCtx&
                 fence_async_smem();
                 named_bar_sync(1, 256);
             }
-            if (g > 0) LIN_WAIT(x.b->u_full, g - 1);  // the parts of the chunk before are consumed
+            if (g > 0) LIN_WAIT(lin_bars()->u_full, g - 1);  // the parts of the chunk before are consumed
             tc_fence_after();
 #pragma unroll 1
             for (int i = 0; i < 4; ++i) {  // 16 V x 16 tokens, transposed
@@ -577,7 +589,12 @@ __device__ __forceinline__ bool role_v(const LinearPrefillArgs& p, const LinCtx&
             }
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(&x.b->u_ready);
+            mbar_arrive(&lin_bars()->u_ready);
+            if (++s == kStages) {
+                s = 0;
+                s_ph ^= 1;
+            }
+            LIN_CHECK();
         }
     }
     return true;
@@ -593,17 +610,17 @@ __device__ __forceinline__ bool role_o(const LinearPrefillArgs& p, const LinearM
     const uint32_t ch = 4 * (quarter & 1) + ((lane >> 3) & 1), sw = lane & 7;
     Walk w = x.walk;
     Piece pc;
-    int g = 0;
+    uint32_t g = 0, ok = 1;
 #pragma unroll 1
     while (w.next(p, pc)) {
         if (pc.e <= pc.s) continue;
 #pragma unroll 1
         for (int c = pc.ca; c < pc.cb; ++c, ++g) {
             const int t0 = pc.s + c * C, L = min(C, pc.e - t0);
-            const float* eg = reinterpret_cast<const float*>(x.sm + kOffG) + (g % kGates) * kGateFloats + 64;
+            const float* eg = lin_gates(g) + 64;
             const uint32_t buf = (uint32_t)(g & 1) * 16384;
-            LIN_WAIT(x.b->g_full[g % kGates], g / kGates);
-            LIN_WAIT(x.b->o_full, g);
+            LIN_WAIT(lin_bars()->g_full[g % kGates], g / kGates);
+            LIN_WAIT(lin_bars()->o_full, g);
             tc_fence_after();
 #pragma unroll 1
             for (int th = 0; th < 2; ++th) {  // 32 tokens
@@ -632,16 +649,16 @@ __device__ __forceinline__ bool role_o(const LinearPrefillArgs& p, const LinearM
                 }
             }
             tc_fence_before();
-            mbar_arrive(&x.b->o_empty);
+            mbar_arrive(&lin_bars()->o_empty);
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&x.b->g_empty[g % kGates]);
+            if (lane == 0) mbar_arrive(&lin_bars()->g_empty[g % kGates]);
             if (r == 0) tma_store_wait_read();  // the chunk before has left its buffer, which the next one writes
             named_bar_sync(2, 128);
             if (L == C) {
                 if (r == 0) {
-                    tma_store_3d(&maps.o, 0, pc.hv, t0, x.sm + kOffO + buf);
-                    tma_store_3d(&maps.o, 64, pc.hv, t0, x.sm + kOffO + buf + 8192);
+                    tma_store_3d(&maps.o, 0, pc.hv, t0, lin_sm + kOffO + buf);
+                    tma_store_3d(&maps.o, 64, pc.hv, t0, lin_sm + kOffO + buf + 8192);
                     tma_store_commit();
                 }
             } else {  // rows behind the segment's end are not its own
@@ -649,10 +666,11 @@ __device__ __forceinline__ bool role_o(const LinearPrefillArgs& p, const LinearM
                 for (int q = r; q < L * 16; q += 128) {
                     const int i = q >> 4, k = q & 15;
                     *reinterpret_cast<uint4*>(p.out + ((size_t)(t0 + i) * p.HV + pc.hv) * kD + 8 * k) =
-                        *reinterpret_cast<const uint4*>(x.sm + kOffO + buf + (k >> 3) * 8192 + i * 128 + (((k & 7) ^ (i & 7)) << 4));
+                        *reinterpret_cast<const uint4*>(lin_sm + kOffO + buf + (k >> 3) * 8192 + i * 128 + (((k & 7) ^ (i & 7)) << 4));
                 }
                 named_bar_sync(2, 128);  // nobody writes the other buffer, then this one, before it is read
             }
+            LIN_CHECK();
         }
     }
     if (r == 0) tma_store_wait_all();
@@ -668,7 +686,7 @@ __device__ __forceinline__ bool role_s(const LinearPrefillArgs& p, const LinCtx&
     const uint32_t tl = x.tmem + ((uint32_t)(32 * quarter) << 16);
     Walk w = x.walk;
     Piece pc;
-    int g = 0;
+    uint32_t g = 0, ok = 1;
 #pragma unroll 1
     while (w.next(p, pc)) {
         const size_t at = ((size_t)pc.n * p.HV + pc.hv) * kD * kD;
@@ -690,16 +708,16 @@ __device__ __forceinline__ bool role_s(const LinearPrefillArgs& p, const LinCtx&
         float gamma = 1.f, unit = 1.f;
 #pragma unroll 1
         for (int c = pc.ca; c < pc.cb; ++c, ++g) {
-            const float* gt = reinterpret_cast<const float*>(x.sm + kOffG) + (g % kGates) * kGateFloats;
-            LIN_WAIT(x.b->g_full[g % kGates], g / kGates);
+            const float* gt = lin_gates(g);
+            LIN_WAIT(lin_bars()->g_full[g % kGates], g / kGates);
             const float factor = gt[256];
             unit = gt[257];
             gamma *= gt[258];
             const bool begins = c == pc.ca, write = begins || gt[259] != 0.f;
             if (g > 0) {
                 // the state is complete (or, at a segment's start, was read) and OI has read its copy
-                LIN_WAIT(x.b->u_full, g - 1);
-                if (kOut) LIN_WAIT(x.b->i_full, g - 1);
+                LIN_WAIT(lin_bars()->u_full, g - 1);
+                if (kOut) LIN_WAIT(lin_bars()->i_full, g - 1);
             }
             tc_fence_after();
             if (kOut || write) {
@@ -739,18 +757,20 @@ __device__ __forceinline__ bool role_s(const LinearPrefillArgs& p, const LinCtx&
                 if (write) tmem_st_wait();
             }
             tc_fence_before();
-            mbar_arrive(&x.b->u_ready);  // U may add to the state
+            mbar_arrive(&lin_bars()->u_ready);  // U may add to the state
             if (kOut) {
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(&x.b->b_ready);
+                mbar_arrive(&lin_bars()->b_ready);
             } else {
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&x.b->g_empty[g % kGates]);
+                if (lane == 0) mbar_arrive(&lin_bars()->g_empty[g % kGates]);
             }
+            LIN_CHECK();
         }
         if (ends) {
-            LIN_WAIT(x.b->u_full, g - 1);
+            LIN_WAIT(lin_bars()->u_full, g - 1);
+            LIN_CHECK();
             tc_fence_after();
 #pragma unroll 1
             for (int b = 0; b < 4; ++b) {
@@ -777,12 +797,14 @@ template <bool kOut>
 __global__ void __launch_bounds__(lin::kThreads, 1)
     gdn_linear_prefill_kernel(LinearPrefillArgs p, const __grid_constant__ LinearMaps maps) {
     using namespace lin;
-    extern __shared__ unsigned char smem_raw[];
-    unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    Bars* b = reinterpret_cast<Bars*>(sm + kOffBar);
-    Mark* range = reinterpret_cast<Mark*>(sm + kOffRange);
+    Bars* b = lin_bars();
+    Mark* range = reinterpret_cast<Mark*>(lin_sm + kOffRange);
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be uniform, and with it all role code
+    if (smem_u32(lin_sm) & 1023u) {
+        if (tid == 0) atomicCAS(p.status, 0, kErrPrepTmaTimeout);
+        return;
+    }
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&b->full[s], 1);
@@ -817,7 +839,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     if (warp == 0) find_range(p, range);
     if (warp == 1) tmem_alloc(&b->tmem, kTmemCols);
     if (kOut) {  // P above its diagonal
-        for (int i = tid; i < 1024; i += kThreads) reinterpret_cast<uint4*>(sm + kOffP)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = tid; i < 1024; i += kThreads) reinterpret_cast<uint4*>(lin_sm + kOffP)[i] = make_uint4(0, 0, 0, 0);
         fence_async_smem();
     }
     tc_fence_before();
@@ -825,9 +847,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     tc_fence_after();
     const Mark m0 = range[0], m1 = range[1];
     LinCtx x;
-    x.sm = sm;
-    x.sbase = smem_u32(sm);
-    x.b = b;
+    x.sbase = smem_u32(lin_sm);
     x.prev = (int)blockIdx.x - 1;
     if (kOut) {
         x.walk = Walk{m0.n, m0.hv, m0.chunk, m1.pos - m0.pos};
@@ -843,13 +863,13 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         int issued = 0;
         if (!(ok = role_load<kOut>(p, maps, x, elect_one(), &issued)))
             // gave up: let copies already in flight land (bounded) before the CTA exits
-            for (int g = max(0, issued - kStages); g < issued; ++g) warp_wait(&b->full[g % kStages], (uint32_t)((g / kStages) & 1));
+            for (int g = max(0, issued - kStages); g < issued; ++g) lin_wait(&b->full[g % kStages], (uint32_t)((g / kStages) & 1));
     } else if (warp == 1 || (kOut && warp == 3)) {
         const uint32_t one = elect_one();
         ok = warp == 1 ? role_u(p, x, one) : role_mma(p, x, one);
         // products still in flight end before the TMEM is given back
         commit_one(one, &b->done[warp >> 1]);
-        ok = warp_wait(&b->done[warp >> 1], 0) && ok;
+        ok = lin_wait(&b->done[warp >> 1], 0) && ok;
     } else if (warp == 2) {
         ok = role_gates(p, x);
     } else if (warp < 4) {
