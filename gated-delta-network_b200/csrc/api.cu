@@ -240,7 +240,7 @@ int gdn_linear_prefill_fwd(const void* q, const void* k, const void* v, const fl
         (reinterpret_cast<uintptr_t>(cu_seqlens) & (cu_is_int64 ? 7u : 3u)))
         return GDN_ERR_ALIGN;
     const gdn::LinearPrefillLayout lay = gdn::linear_prefill_layout(N, T, HV);
-    if (((long long)T / 64 + N) * HV > 0x7fffffffll) return GDN_ERR_SIZE;
+    if (((long long)T / 64 + 3ll * N) * HV > 0x7fffffffll) return GDN_ERR_SIZE;
     if (!workspace || workspace_bytes < lay.total || (reinterpret_cast<uintptr_t>(workspace) & 255u))
         return GDN_ERR_WORKSPACE;
     const int rc = check_device();
@@ -267,7 +267,7 @@ int gdn_linear_prefill_fwd(const void* q, const void* k, const void* v, const fl
     p.min_share = lay.min_share;
     p.keep = lay.keep;
     p.cut = lay.cut;
-    p.kind = reinterpret_cast<int*>(ws + lay.off_kind);
+    p.kind = reinterpret_cast<int4*>(ws + lay.off_kind);
     p.status = reinterpret_cast<int*>(ws + lay.off_status);
     p.gamma = reinterpret_cast<float*>(ws + lay.off_gamma);
     p.seg = reinterpret_cast<float*>(ws + lay.off_seg);

@@ -39,7 +39,7 @@ struct LinearPrefillArgs {
     int keep;              // segments of at most this many chunks are not cut
     int cut;               // a sequence can be longer than that: build and chain segment states
     int* status;           // workspace: first error code of a bounded wait
-    int* kind;             // workspace: [ctas] what the stretch's last segment does: see the kernel
+    int4* kind;            // workspace: [ctas] what the stretch's last segment does, its sequence and v-head
     float* gamma;          // workspace: [ctas] product of its decays there
     float* seg;            // workspace: [2 ctas][128 V][128 K] what it adds to the state, then (after the chain) the state
                            //            at the stretch's end; behind them the initial states

@@ -71,7 +71,7 @@ struct LinearMaps {
 
 // ---- the line of chunks ---------------------------------------------------------------------
 struct Mark {  // a place on the line: chunk `chunk` of (sequence n, v-head hv)
-    int n, hv, chunk, pos;
+    int n, hv, chunk;
 };
 
 // cu_seqlens[n], clamped to [0, T]; a sequence that ends before it begins is empty.
@@ -79,47 +79,37 @@ __device__ __forceinline__ int cu_at(const LinearPrefillArgs& p, int n) {
     const long long x = p.cu64 ? reinterpret_cast<const long long*>(p.cu)[n] : reinterpret_cast<const int*>(p.cu)[n];
     return (int)max(0ll, min((long long)p.T, x));
 }
-// Chunks of a sequence of tokens [s, e): an empty one has a place on the line too, its state is copied.
-__device__ __forceinline__ int lin_chunks(int s, int e) { return max(1, (e - s + lin::C - 1) / lin::C); }
+__device__ __forceinline__ int lin_chunks(int s, int e) { return max(0, (e - s + lin::C - 1) / lin::C); }
 
-// The ends of the stretch of CTA blockIdx.x, by one warp: every lane sums up an equal part of the sequences.
-// (Positions are ints: the entry point refuses calls of 2^31 chunks.)
+// The ends of the stretch of CTA blockIdx.x, by one warp: every lane sums up an equal part of the sequences.  A segment
+// takes its chunks and 2 more places for its state, which is 128 KB to the 48 of a chunk.  (Places are ints: the entry
+// point refuses calls of 2^31 chunks.)
 __device__ __forceinline__ void find_range(const LinearPrefillArgs& p, Mark* at) {
     const int lane = threadIdx.x & 31, part = (p.N + 31) / 32, n0 = min(p.N, lane * part), n1 = min(p.N, n0 + part);
-    int x = 0, lo = 0, total = 0, ctas = 1, per = 0, more = 0;
+    int x = 0, lo = 0, total = 0, per = 0, more = 0;
 #pragma unroll 1
     for (int round = 0; round < 2; ++round) {  // the sum of the lane's lengths, then the marks among them
         int s = n0 < n1 ? cu_at(p, n0) : 0;
-#pragma unroll 2
+#pragma unroll 1
         for (int n = n0; n < n1; ++n) {
-            const int e = cu_at(p, n + 1), nc = lin_chunks(s, e);
+            const int e = cu_at(p, n + 1), nc = lin_chunks(s, e), w = nc + 2;
             s = e;
-            if (round == 0) {
-                x += nc;
-                continue;
-            }
+            x += w;
+            if (round == 0) continue;
 #pragma unroll 1
             for (int i = 0; i < 2; ++i) {
-                const int c = blockIdx.x + i, want = min(total, c * per + min(c, more)), off = want - lo;
-                if (off < 0 || off >= nc * p.HV) continue;
-                Mark m;
-                m.n = n;
-                m.hv = off / nc;
-                m.chunk = off - m.hv * nc;
-                m.pos = want;
-                if (nc <= p.keep && m.chunk) {  // a short segment is not cut: to its nearer end
-                    const int up = 2 * m.chunk >= nc;
-                    m.pos += up ? nc - m.chunk : -m.chunk;
-                    m.chunk = 0;
-                    m.hv += up;
-                    if (m.hv == p.HV) {
-                        m.hv = 0;
-                        ++m.n;
-                    }
+                const int c = blockIdx.x + i, off = min(total, c * per + min(c, more)) - lo;
+                if (off < 0 || off >= w * p.HV) continue;
+                Mark m{n, off / w, 0};
+                const int place = off - m.hv * w - 2;
+                if (nc > p.keep) {
+                    m.chunk = max(0, place);
+                } else if (2 * place >= nc) {  // a short segment is not cut: to its nearer end
+                    if (++m.hv == p.HV) m = Mark{n + 1, 0, 0};
                 }
                 at[i] = m;
             }
-            lo += nc * p.HV;
+            lo += w * p.HV;
         }
         if (round == 0) {
             const int mine = x;
@@ -130,11 +120,10 @@ __device__ __forceinline__ void find_range(const LinearPrefillArgs& p, Mark* at)
             }
             lo = (x - mine) * p.HV;
             total = __shfl_sync(0xffffffffu, x, 31) * p.HV;
-            ctas = max(1, min(p.ctas, total / p.min_share));
+            const int ctas = max(1, min(p.ctas, total / p.min_share)), c = blockIdx.x + lane;
             per = total / ctas;
             more = total - per * ctas;
-            const int c = blockIdx.x + lane;
-            if (lane < 2 && min(total, c * per + min(c, more)) == total) at[lane] = Mark{p.N, 0, 0, total};
+            if (lane < 2 && min(total, c * per + min(c, more)) == total) at[lane] = Mark{p.N, 0, 0};
         }
     }
 }
@@ -142,24 +131,26 @@ __device__ __forceinline__ void find_range(const LinearPrefillArgs& p, Mark* at)
 struct Piece {
     int n, hv, s, e, ca, cb, nc;  // chunks [ca, cb) of the nc of segment (n, hv), tokens [s, e)
 };
-struct Walk {
-    int n, hv, chunk, left;
+struct Walk {  // from a mark to another one
+    Mark at, end;
     __device__ __forceinline__ bool next(const LinearPrefillArgs& p, Piece& x) {
-        if (left <= 0 || n >= p.N) return false;
-        x.n = n;
-        x.hv = hv;
-        x.s = cu_at(p, n);
-        x.e = max(x.s, cu_at(p, n + 1));
+        if (at.n > end.n || (at.n == end.n && (at.hv > end.hv || (at.hv == end.hv && at.chunk >= end.chunk)))) return false;
+        x.n = at.n;
+        x.hv = at.hv;
+        x.s = cu_at(p, x.n);
+        x.e = max(x.s, cu_at(p, x.n + 1));
         x.nc = lin_chunks(x.s, x.e);
-        x.ca = chunk;
-        x.cb = min(x.nc, chunk + left);
-        left -= x.cb - x.ca;
-        chunk = 0;
-        if (++hv == p.HV) {
-            hv = 0;
-            ++n;
+        x.ca = at.chunk;
+        x.cb = x.n == end.n && x.hv == end.hv ? end.chunk : x.nc;
+        at.chunk = 0;
+        if (++at.hv == p.HV) {
+            at.hv = 0;
+            ++at.n;
         }
         return true;
+    }
+    __device__ __forceinline__ bool empty() const {
+        return at.n > end.n || (at.n == end.n && (at.hv > end.hv || (at.hv == end.hv && at.chunk >= end.chunk)));
     }
 };
 
@@ -233,6 +224,32 @@ __device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_16x256b_x8(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_16x256b_x8(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x256b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_16x128b_x8(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
 }
 __device__ __forceinline__ void tmem_ld_16x256b_x2(uint32_t taddr, uint32_t (&r)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -699,6 +716,8 @@ __device__ __forceinline__ bool role_s(const LinearPrefillArgs& p, const LinCtx&
         }
         float* dst = kOut ? p.new_state + at : p.seg + (size_t)blockIdx.x * kD * kD;
         const bool ends = !kOut || pc.cb == pc.nc;
+        if (src && pc.e > pc.s)  // on its way to L2 while the gates and the first tiles are
+            for (int j = r; j < kD * kD / 32; j += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + 32 * j));
         if (pc.e <= pc.s) {  // an empty sequence keeps its state
 #pragma unroll 4
             for (int j = r; j < kD * kD / 4; j += 128)
@@ -713,31 +732,44 @@ __device__ __forceinline__ bool role_s(const LinearPrefillArgs& p, const LinCtx&
             const float factor = gt[256];
             unit = gt[257];
             gamma *= gt[258];
-            const bool begins = c == pc.ca, write = begins || gt[259] != 0.f;
+            const bool begins = c == pc.ca, write = gt[259] != 0.f;
             if (g > 0) {
                 // the state is complete (or, at a segment's start, was read) and OI has read its copy
                 LIN_WAIT(lin_bars()->u_full, g - 1);
                 if (kOut) LIN_WAIT(lin_bars()->i_full, g - 1);
             }
             tc_fence_after();
-            if (kOut || write) {
+            if (begins) {
+                // 16 V x 64 K a round, as fragments: a load of the warp covers eight whole 32-byte sectors
+#pragma unroll 1
+                for (int b = 0; b < 4; ++b) {
+                    uint32_t d[32];
+                    const float* row = src + (size_t)(32 * quarter + 16 * (b & 1) + (lane >> 2)) * kD + 64 * (b >> 1) + 2 * (lane & 3);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float2 y = src ? *reinterpret_cast<const float2*>(row + 8 * (j >> 1) + 8 * kD * (j & 1)) : make_float2(0.f, 0.f);
+                        d[2 * j] = __float_as_uint(y.x);
+                        d[2 * j + 1] = __float_as_uint(y.y);
+                    }
+                    const uint32_t ta = tl + ((uint32_t)(16 * (b & 1)) << 16);
+                    if (kOut) {
+                        uint32_t o[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = pack_bf16x2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1]));
+                        tmem_st_16x128b_x8(ta + kColB + 32 * (b >> 1), o);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) d[j] = __float_as_uint(factor * __uint_as_float(d[j]));
+                    tmem_st_16x256b_x8(ta + kColS + 64 * (b >> 1), d);
+                }
+                tmem_st_wait();
+            } else if (kOut || write) {
 #pragma unroll 1
                 for (int b = 0; b < 4; ++b) {  // 32 K
                     uint32_t d[32];
-                    if (begins) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float4 y = src ? *reinterpret_cast<const float4*>(src + (size_t)r * kD + 32 * b + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
-                            d[4 * j] = __float_as_uint(y.x);
-                            d[4 * j + 1] = __float_as_uint(y.y);
-                            d[4 * j + 2] = __float_as_uint(y.z);
-                            d[4 * j + 3] = __float_as_uint(y.w);
-                        }
-                    } else {
-                        tmem_ld32_async(tl + kColS + 32 * b, d);
-                        tmem_ld_wait();
-                        tmem_regs_ready(d);
-                    }
+                    tmem_ld32_async(tl + kColS + 32 * b, d);
+                    tmem_ld_wait();
+                    tmem_regs_ready(d);
                     if (kOut) {
                         uint32_t o[16];
 #pragma unroll
@@ -775,14 +807,14 @@ __device__ __forceinline__ bool role_s(const LinearPrefillArgs& p, const LinCtx&
 #pragma unroll 1
             for (int b = 0; b < 4; ++b) {
                 uint32_t d[32];
-                tmem_ld32_async(tl + kColS + 32 * b, d);
+                tmem_ld_16x256b_x8(tl + ((uint32_t)(16 * (b & 1)) << 16) + kColS + 64 * (b >> 1), d);
                 tmem_ld_wait();
                 tmem_regs_ready(d);
+                float* row = dst + (size_t)(32 * quarter + 16 * (b & 1) + (lane >> 2)) * kD + 64 * (b >> 1) + 2 * (lane & 3);
 #pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                    *reinterpret_cast<float4*>(dst + (size_t)r * kD + 32 * b + j) =
-                        make_float4(unit * __uint_as_float(d[j]), unit * __uint_as_float(d[j + 1]), unit * __uint_as_float(d[j + 2]),
-                                    unit * __uint_as_float(d[j + 3]));
+                for (int j = 0; j < 16; ++j)
+                    *reinterpret_cast<float2*>(row + 8 * (j >> 1) + 8 * kD * (j & 1)) =
+                        make_float2(unit * __uint_as_float(d[2 * j]), unit * __uint_as_float(d[2 * j + 1]));
             }
             if (!kOut && r == 0) p.gamma[blockIdx.x] = gamma;
         }
@@ -850,13 +882,12 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     x.sbase = smem_u32(lin_sm);
     x.prev = (int)blockIdx.x - 1;
     if (kOut) {
-        x.walk = Walk{m0.n, m0.hv, m0.chunk, m1.pos - m0.pos};
+        x.walk = Walk{m0, m1};
     } else {
-        const bool same = m0.n == m1.n && m0.hv == m1.hv;
-        const int from = same ? m0.chunk : 0;
-        x.walk = Walk{m1.n, m1.hv, from, m1.pos > m0.pos ? m1.chunk - from : 0};
+        const int from = m0.n == m1.n && m0.hv == m1.hv ? m0.chunk : 0;
+        x.walk = Walk{Mark{m1.n, m1.hv, from}, m1};
         // 1: a segment begins here and goes on, 2: one goes through, 0: neither
-        if (tid == 0) p.kind[blockIdx.x] = x.walk.left <= 0 ? 0 : from > 0 ? 2 : 1;
+        if (tid == 0) p.kind[blockIdx.x] = make_int4(x.walk.empty() ? 0 : from > 0 ? 2 : 1, m1.n, m1.hv, 0);
     }
     bool ok = true;
     if (warp == 0) {
@@ -892,22 +923,25 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
 // the segment's initial state in the slot p.ctas further: new_state may be state itself, and a segment may end in
 // one CTA before it begins in another.  One CTA per (stretch in which such a segment begins, 1024 state elements).
 __global__ void __launch_bounds__(256) gdn_linear_chain_kernel(LinearPrefillArgs p) {
-    __shared__ Mark range[2];
     pdl_wait();
     pdl_trigger();
-    if (p.kind[blockIdx.x] != 1) return;
-    if (threadIdx.x < 32) find_range(p, range);
-    __syncthreads();
-    const int n = range[1].n, hv = range[1].hv;
+    const int4 kind = p.kind[blockIdx.x];
+    if (kind.x != 1) return;
+    // the stretches that the segment goes through from here: a run of 2s
+    const int lane = threadIdx.x & 31;
+    int end = blockIdx.x + 1;
+    while (true) {
+        const unsigned through = __ballot_sync(0xffffffffu, end + lane < p.ctas && p.kind[min(end + lane, p.ctas - 1)].x == 2);
+        end += __ffs(~through) ? __ffs(~through) - 1 : 32;
+        if (through != 0xffffffffu) break;
+    }
     const size_t el = blockIdx.y * 1024 + threadIdx.x * 4;
     float4 h = make_float4(0.f, 0.f, 0.f, 0.f);
     if (p.state) {
-        h = *reinterpret_cast<const float4*>(p.state + ((size_t)n * p.HV + hv) * kD * kD + el);
+        h = *reinterpret_cast<const float4*>(p.state + ((size_t)kind.y * p.HV + kind.z) * kD * kD + el);
         *reinterpret_cast<float4*>(p.seg + (size_t)(p.ctas + blockIdx.x) * kD * kD + el) = h;
     }
-    int end = blockIdx.x + 1;
-    while (end < p.ctas && p.kind[end] == 2) ++end;
-#pragma unroll 4
+#pragma unroll 8
     for (int c = blockIdx.x; c < end; ++c) {
         const float gm = p.gamma[c];
         float4* d = reinterpret_cast<float4*>(p.seg + (size_t)c * kD * kD + el);
@@ -919,7 +953,7 @@ __global__ void __launch_bounds__(256) gdn_linear_chain_kernel(LinearPrefillArgs
 
 LinearPrefillLayout linear_prefill_layout(int N, int T, int HV) {
     LinearPrefillLayout L{};
-    const long long share = ((long long)T / lin::C + N) * HV / kLinearCtas;  // chunks of a CTA
+    const long long share = ((long long)T / lin::C + 3ll * N) * HV / kLinearCtas;  // places of a CTA
     L.keep = (int)std::max<long long>(8, std::min<long long>(3 * share / 10, 1 << 20));
     L.cut = T > (long long)lin::C * L.keep ? 1 : 0;
     L.min_share = L.cut ? 4 : 1;
@@ -927,7 +961,7 @@ LinearPrefillLayout linear_prefill_layout(int N, int T, int HV) {
     const size_t slots = L.cut ? kLinearCtas : 0;
     L.off_status = 0;
     L.off_kind = 256;
-    L.off_gamma = up(L.off_kind + slots * sizeof(int));
+    L.off_gamma = up(L.off_kind + slots * sizeof(int4));
     L.off_seg = up(L.off_gamma + slots * sizeof(float));
     L.total = L.off_seg + 2 * slots * kD * kD * sizeof(float);
     return L;
