@@ -4,6 +4,8 @@
 // (reference/gdn_decode_ref.py:32-36, reference/gdn_prefill_ref.py:33-36) and
 // adds the checks the kernels rely on (alignment, workspace size, device).
 // Nothing here synchronises, copies to the host or allocates device memory.
+#include <algorithm>
+
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -361,7 +363,13 @@ int gdn_cache_attend(const void* q, const void* k_cache, const void* v_cache, co
                         max_pages, B, Hkv, D, &p.c);
     if (rc != GDN_OK) return rc;
     if (Hq < Hkv || Hq % Hkv != 0) return GDN_ERR_SHAPE;
-    if (Q < 0 || flags != 0 || (long long)B * Hkv * (((long long)Q * (Hq / Hkv) + 15) / 16) > 0x7fffffffll) return GDN_ERR_SIZE;
+    if (Q < 0 || flags != 0) return GDN_ERR_SIZE;
+    {  // segments and their 32-token blocks are counted in ints
+        const long long rows = (long long)Q * (Hq / Hkv);
+        if (rows > (1 << 20)) return GDN_ERR_SIZE;
+        const long long tile = 8 * gdn::attend_tiles((int)rows), segs = Hkv * ((rows + tile - 1) / tile);
+        if (B * segs * std::max<long long>(1, ((long long)max_pages * page_size + 31) / 32) > 0x7fffffffll) return GDN_ERR_SIZE;
+    }
     if (B == 0 || Q == 0) return GDN_OK;
     if (!q || !out) return GDN_ERR_NULL;
     if (!aligned16(q) || !aligned16(out)) return GDN_ERR_ALIGN;

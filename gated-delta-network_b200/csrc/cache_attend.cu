@@ -4,18 +4,22 @@
 //   s_j = scale q . k_j,   out = sum_j e^{s_j - m} v_j / sum_j e^{s_j - m},   x = code * scale[page][h]
 // A row that sees no position is zero.
 //
-// Bound by HBM for up to about 16 rows a kv head: 256 bytes a token and head, each read once.
+// Bound by HBM for up to some 16 rows a kv head: 256 bytes a token and head, each read once.
 //  * Codes go to the tensor cores as fp16, which holds every int8 and e4m3 value exactly (mma.sync m16n8k16,
-//    fp32 accumulation: 16 rows are all there is, a 128-row tcgen05 tile would be 7/8 empty). q is brought to
-//    fp16 by a power of two per row (its largest element lands in [1, 2), the others keep an absolute 2^-25 of
-//    it), and the page's key scale multiplies the fp32 scores.
-//  * The value scale enters the weights: p v_scale / r <= 1 in fp16 with r the largest value scale so far, kept
-//    like the running maximum, so the accumulator never sees the scales' range; the sum of p stays fp32 and unrounded.
+//    fp32 accumulation).  The tokens are the 16 rows of S^T = K Q^T, the dims those of O^T = V^T P^T, and the q rows
+//    the 8 columns, so a decode step of 4 or 8 rows wastes little; a 128-row tcgen05 tile would.  More rows take
+//    several column tiles against the same converted fragments (the conversion costs as much as the products).
+//  * q is brought to fp16 by a power of two per row (its largest element lands in [1, 2), the others keep an absolute
+//    2^-25 of it), and the page's key scale multiplies the fp32 scores.
+//  * The maximum is a reference that moves only when a score exceeds it by 4 (base 2), so most steps need no
+//    reduction and no rescaling; weights stay below 2^4 in fp16, their sum is fp32 and of the unrounded ones.
+//  * The value scale enters the weights: p v_scale / r with r the largest value scale so far, kept like the maximum,
+//    so the accumulator never sees the scales' range.
 //  * Both contractions may permute their index, so a thread takes 16 consecutive bytes of a row and no fragment
 //    needs a shuffle or a transposing load: key step s of lane l holds dims 16 (l % 4) + 4 s .. and the same of q;
-//    value lane l holds dims 16 (l / 4) .. of the four tokens whose weights it owns. Every thread reads back only the
-//    shared memory it filled itself (cp.async), so the ring needs no barrier.
-//  * Tokens are cut evenly over the CTAs whatever the lengths: all (sequence, head, 16-row tile) segments in 32-token
+//    value lane l holds dims 16 (l / 4) .. of the four tokens whose weights it owns (after one 8 x 8 transpose). Every
+//    thread reads back only the shared memory it filled itself (cp.async), so the ring needs no barrier.
+//  * Tokens are cut evenly over the CTAs whatever the lengths: all (sequence, head, row tile) segments in 32-token
 //    blocks on one line, an equal stretch of it per CTA. A stretch's first and last segment may continue in a
 //    neighbour; those pieces go to the workspace, and a second launch joins them.
 #include <cuda_fp16.h>
@@ -30,24 +34,32 @@ constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kBlock = 32;                       // tokens of the unit that is divided over the CTAs
 constexpr int kStages = 3;
 constexpr int kStageBytes = 4096;                // a warp's 16 tokens of k and v: 8 x 16 bytes a lane
-constexpr int kRing = kWarps * kStages * kStageBytes;
-constexpr int kOffQ = kRing;                     // q as A fragments: [8 steps][32 lanes][16 bytes]
-constexpr int kOffF = kOffQ + 4096;              // f32 [16] row factors
-constexpr int kOffM = kOffF + 64;                // f32 [kWarps][16] maxima, then sums
-constexpr int kSmem = kOffM + 2 * kWarps * 16 * 4;
 constexpr float kLog2e = 1.4426950408889634f;
-static_assert(kWarps * 16 * 128 * 4 <= kRing, "the warps' results take the ring's place");
+constexpr float kSlack = 4.f;                    // scores may exceed the reference by this (base 2)
+// Shared memory for tiles of 8 NT rows: the ring, whose place the warps' results take; q as B fragments
+// [NT][8 steps][32 lanes][8 bytes]; f32 [8 NT] row factors; f32 [kWarps][8 NT] references, then sums.
+template <int NT>
+struct Smem {
+    static constexpr int kRing = kWarps * kStages * kStageBytes, kJoin = kWarps * 8 * NT * 128 * 4;
+    static constexpr int kOffQ = kRing > kJoin ? kRing : kJoin, kOffF = kOffQ + NT * 2048, kOffM = kOffF + NT * 32;
+    static constexpr int kSize = kOffM + 2 * kWarps * 8 * NT * 4;
+};
 }  // namespace att
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 // The two codes in the low (kHigh: high) half of w as fp16, exactly.  int8: w holds code + 128.
@@ -62,11 +74,13 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(kHigh ? w >> 16 : w)));
     return h;
 }
-
-struct Line {  // segment (b, h, row tile) and the 32-token blocks of it
-    int b, seg_in_b, blocks;
-    long long begin;  // first block on the line
-};
+template <bool kInt8>
+__device__ __forceinline__ uint4 load_codes(const unsigned char* p) {
+    uint4 x = *reinterpret_cast<const uint4*>(p);
+    if (kInt8) x = make_uint4(x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u);
+    return x;
+}
+__device__ __forceinline__ uint32_t word(const uint4& x, int e) { return e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w; }
 
 __device__ __forceinline__ int visible_length(const CacheArgs& c, int b) {
     return (int)min((long long)cache_length(c, b), (long long)c.max_pages << c.page_shift);
@@ -75,103 +89,128 @@ __device__ __forceinline__ int seq_blocks(const CacheArgs& c, int b) {
     return max(1, (visible_length(c, b) + att::kBlock - 1) / att::kBlock);
 }
 
-// Total blocks of the line, and the sequence that holds block `at` with the line position of its first block.
-// All threads of the CTA take part; two passes over the lengths.
-__device__ __forceinline__ long long line_total(const CacheArgs& c, int segs, long long* s_sum) {
-    long long sum = 0;
-    for (int b = threadIdx.x; b < c.B; b += att::kThreads) sum += seq_blocks(c, b);
-#pragma unroll
-    for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = sum;
-    __syncthreads();
-    sum = 0;
-#pragma unroll
-    for (int w = 0; w < att::kWarps; ++w) sum += s_sum[w];
-    __syncthreads();
-    return sum * segs;
-}
-__device__ __forceinline__ void line_find(const CacheArgs& c, int segs, long long at, long long* s_sum, int* s_b, long long* s_begin) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long before = 0;  // blocks of the sequences in front of this pass
-    for (int base = 0; base < c.B; base += att::kThreads) {
-        const int b = base + threadIdx.x;
-        const long long mine = b < c.B ? (long long)seq_blocks(c, b) * segs : 0;
-        long long x = mine;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x, off);
-            if (lane >= off) x += y;
+// Total blocks of the line, the number of CTAs that share it, and where this CTA's stretch begins: its place, the
+// sequence there and the place of that sequence's first block.  By one warp, every lane with an equal part of the
+// sequences.  (Places are ints: the entry point refuses more.)
+struct Stretch {
+    int total, ctas, first, end, b, begin;
+};
+__device__ __forceinline__ void find_stretch(const CacheArgs& c, int segs, Stretch* out) {
+    const int lane = threadIdx.x & 31, part = (c.B + 31) / 32, b0 = min(c.B, lane * part), b1 = min(c.B, b0 + part);
+    int x = 0, mine = 0;
+#pragma unroll 4
+    for (int b = b0; b < b1; ++b) mine += seq_blocks(c, b);
+    x = mine;
+#pragma unroll 1
+    for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, off);
+        if (lane >= off) x += y;
+    }
+    const int total = __shfl_sync(0xffffffffu, x, 31) * segs;
+    // at least a block for each warp, so that short caches are not cut into more pieces than they are worth
+    const int ctas = min((int)gridDim.x, (total + att::kWarps - 1) / att::kWarps), per = total / ctas, more = total - per * ctas;
+    const int k = blockIdx.x, first = min(total, k * per + min(k, more));
+    int lo = (x - mine) * segs;
+    if (first >= lo && first < lo + mine * segs) {
+        int b = b0, n = seq_blocks(c, b) * segs;
+        while (first >= lo + n) {
+            lo += n;
+            n = seq_blocks(c, ++b) * segs;
         }
-        if (lane == 31) s_sum[warp] = x;
-        __syncthreads();
-        long long total = 0;
-#pragma unroll
-        for (int w = 0; w < att::kWarps; ++w) {
-            if (w < warp) x += s_sum[w];
-            total += s_sum[w];
-        }
-        const long long lo = before + x - mine;
-        if (at >= lo && at < lo + mine) {
-            *s_b = b;
-            *s_begin = lo;
-        }
-        before += total;
-        __syncthreads();
-        if (at < before) break;
+        out->b = b;
+        out->begin = lo;
+    }
+    if (lane == 0) {
+        out->total = total;
+        out->ctas = ctas;
+        out->first = first;
+        out->end = min(total, (k + 1) * per + min(k + 1, more));
     }
 }
+// The CTA whose stretch holds place x.
+__device__ __forceinline__ int cta_of(int x, int total, int ctas) {
+    const int per = total / ctas, more = total - per * ctas, big = more * (per + 1);
+    return x < big ? x / (per + 1) : more + (x - big) / per;
+}
 
-template <bool kInt8>
-__global__ void __launch_bounds__(att::kThreads, 2) gdn_cache_attend_kernel(CacheAttendArgs p) {
+template <bool kInt8, int NT>
+__global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_attend_kernel(CacheAttendArgs p) {
     using namespace att;
-    extern __shared__ __align__(128) unsigned char sm[];
-    __shared__ long long s_sum[kWarps], s_begin;
-    __shared__ int s_b, s_status;
+    using S = Smem<NT>;
+    constexpr int kRows = 8 * NT;
+    extern __shared__ __align__(128) unsigned char att_sm[];
+    __shared__ Stretch s_line;
+    __shared__ int s_status;
     const CacheArgs& c = p.c;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    float* s_f = reinterpret_cast<float*>(sm + kOffF);
-    float* s_m = reinterpret_cast<float*>(sm + kOffM);
-    float* s_l = s_m + kWarps * 16;
+    float* s_f = reinterpret_cast<float*>(att_sm + S::kOffF);
+    float* s_m = reinterpret_cast<float*>(att_sm + S::kOffM);
+    float* s_l = s_m + kWarps * kRows;
+    if (tid == 0) s_status = 0;
     pdl_wait();
     pdl_trigger();
-    if (tid == 0) s_status = 0;
 
-    const int G = p.Hq / c.Hkv, R = p.Q * G, tiles = (R + 15) / 16, segs = c.Hkv * tiles;
-    const long long total = line_total(c, segs, s_sum);
-    // at least a block for each warp, so that short caches are not cut into more pieces than they are worth
-    const long long ctas = min((long long)gridDim.x, (total + kWarps - 1) / kWarps);
-    const long long first = blockIdx.x * total / ctas, end = min(total, (blockIdx.x + 1) * total / ctas);
-    int2 piece = make_int2(-1, 0);  // the segment that begins here and ends elsewhere (thread 0)
-    if (blockIdx.x >= ctas) {
-        if (tid == 0) p.piece[blockIdx.x] = make_int4(-1, 0, 0, 0);
-        return;
-    }
-    line_find(c, segs, first, s_sum, &s_b, &s_begin);
+    const int G = p.Hq / c.Hkv, R = p.Q * G, tiles = (R + kRows - 1) / kRows, segs = c.Hkv * tiles;
+    if (warp == 0) find_stretch(c, segs, &s_line);
     __syncthreads();
-    int b = s_b;
-    long long begin = s_begin;
+    const Stretch line = s_line;
+    int2 piece = make_int2(-1, 0);  // the segment that begins here and ends elsewhere (thread 0)
+    int b = line.b, begin = line.begin;
 
-    for (long long at = first; at < end;) {
+#pragma unroll 1
+    for (int at = line.first; at < line.end;) {
         const int nb = seq_blocks(c, b);
-        if (at >= begin + (long long)nb * segs) {
-            begin += (long long)nb * segs;
+        if (at >= begin + nb * segs) {
+            begin += nb * segs;
             ++b;
             continue;
         }
-        const int seg = (int)((at - begin) / nb), h = seg / tiles, row0 = (seg % tiles) * 16;
-        const long long seg_begin = begin + (long long)seg * nb, seg_end = seg_begin + nb;
-        const long long stop = min(seg_end, end);
+        const int seg = (at - begin) / nb, h = seg / tiles, row0 = (seg - h * tiles) * kRows;
+        const int seg_begin = begin + seg * nb, seg_end = seg_begin + nb, stop = min(seg_end, line.end);
         const int len = visible_length(c, b);
         if (tid == 0 && cache_length(c, b) > len) s_status = kErrBadSeqlens;
-        const int tok0 = (int)(at - seg_begin) * kBlock, tok1 = min(len, (int)(stop - seg_begin) * kBlock);
+        const int tok0 = (at - seg_begin) * kBlock, tok1 = min(len, (stop - seg_begin) * kBlock);
         const int steps = tok1 > tok0 ? (tok1 - tok0 + 15) / 16 : 0;
 
+        unsigned char* ring = att_sm + warp * kStages * kStageBytes + lane * 16;
+        const int mine = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;  // steps warp, warp + 8, ..
+        const int* trow = c.table + (size_t)b * c.max_pages;
+        const int t_first = tok0 + 16 * warp;
+        auto page_of = [&](int n) { return n < mine ? trow[(t_first + 16 * kWarps * n) >> c.page_shift] : 0; };
+        auto issue = [&](int n, int stage, int page) {
+            if (n < mine) {
+                const int t = t_first + 16 * kWarps * n;
+                const bool ok = (unsigned)page < (unsigned)c.pages;
+                const size_t off = ((((size_t)(ok ? page : 0) * c.Hkv + h) << c.page_shift) + (t & ((1 << c.page_shift) - 1))) * kD;
+                const unsigned char* kp = static_cast<const unsigned char*>(c.k_cache) + off + (lane >> 2) * kD + (lane & 3) * 16;
+                const unsigned char* vp = static_cast<const unsigned char*>(c.v_cache) + off + (lane & 3) * 2 * kD + (lane >> 2) * 16;
+                unsigned char* st = ring + stage * kStageBytes;
+                const int left = ok ? tok1 - t : 0;  // rows behind the end arrive as zeros
+#pragma unroll
+                for (int i = 0; i < 4; ++i)  // token lane / 4 (+ 8), 16-byte chunk lane % 4 (+ 4)
+                    cp_async16(st + i * 512, kp + 8 * (i >> 1) * kD + 64 * (i & 1), (lane >> 2) + 8 * (i >> 1) < left);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)  // tokens 2 (lane % 4) + {0, 1} (+ 8), chunk lane / 4
+                    cp_async16(st + 2048 + i * 512, vp + ((i & 1) + 8 * (i >> 1)) * kD, 2 * (lane & 3) + (i & 1) + 8 * (i >> 1) < left);
+            }
+            cp_async_commit();
+        };
+        int pg0 = page_of(0), pg1 = page_of(1), pg2 = page_of(2);  // pages of the steps in the ring and of the next
+        issue(0, 0, pg0);
+        issue(1, 1, pg1);
+        auto scale_at = [&](int page) { return (size_t)((unsigned)page < (unsigned)c.pages ? page : 0) * c.Hkv + h; };
+        float ks = 0.f, vs = 0.f;
+        if (mine > 0) {
+            ks = c.k_scale[scale_at(pg0)];
+            vs = c.v_scale[scale_at(pg0)];
+        }
+
         // q rows as fp16 fragments; 16 threads a row
-        {
-            const int r = tid >> 4, x = tid & 15, row = row0 + r;
+#pragma unroll 1
+        for (int r = tid >> 4; r < kRows; r += kThreads / 16) {
+            const int x = tid & 15, row = row0 + r, i = row / G;
             uint4 w = make_uint4(0, 0, 0, 0);
-            if (row < R)
-                w = *reinterpret_cast<const uint4*>(p.q + (((size_t)b * p.Q + row / G) * p.Hq + h * G + row % G) * kD + 8 * x);
+            if (row < R) w = *reinterpret_cast<const uint4*>(p.q + (((size_t)b * p.Q + i) * p.Hq + h * G + row - i * G) * kD + 8 * x);
             const uint32_t u[4] = {w.x, w.y, w.z, w.w};
             float f[8], top = 0.f;
 #pragma unroll
@@ -190,244 +229,201 @@ __global__ void __launch_bounds__(att::kThreads, 2) gdn_cache_attend_kernel(Cach
             const int xl = (x >> 1) & 3, s0 = 2 * (x & 1) + 4 * (x >> 3);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const __half2 a = __floats2half2_rn(f[4 * e] * inv, f[4 * e + 1] * inv);
-                const __half2 d = __floats2half2_rn(f[4 * e + 2] * inv, f[4 * e + 3] * inv);
-                uint32_t* dst = reinterpret_cast<uint32_t*>(sm + kOffQ + (s0 + e) * 512 + ((r & 7) * 4 + xl) * 16);
-                dst[r >> 3] = *reinterpret_cast<const uint32_t*>(&a);
-                dst[2 + (r >> 3)] = *reinterpret_cast<const uint32_t*>(&d);
+                const __half2 lo = __floats2half2_rn(f[4 * e] * inv, f[4 * e + 1] * inv);
+                const __half2 hi = __floats2half2_rn(f[4 * e + 2] * inv, f[4 * e + 3] * inv);
+                *reinterpret_cast<uint2*>(att_sm + S::kOffQ + (r >> 3) * 2048 + (s0 + e) * 256 + ((r & 7) * 4 + xl) * 8) =
+                    make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
             }
         }
         __syncthreads();
 
-        float acc[16][4];
+        // this thread's q rows of column tile j: row0 + 8 j + 2 (lane % 4) and the next
+        float acc[NT][8][4], m[NT][2], l[NT][2], rf[NT][2], vref = 0.f;
+        int lim[NT][2];  // positions that the rows see
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
+        for (int j = 0; j < NT; ++j) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, vref = 0.f;
-        const int ra = row0 + (lane >> 2), rb = ra + 8;
-        const int lim[2] = {len - p.Q + 1 + ra / G, len - p.Q + 1 + rb / G};  // positions that the rows see
-        const float rf[2] = {s_f[lane >> 2], s_f[(lane >> 2) + 8]};
-
-        unsigned char* ring = sm + warp * kStages * kStageBytes + lane * 16;
-        const int mine = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;  // steps warp, warp + 8, ..
-        const int* trow = c.table + (size_t)b * c.max_pages;
-        const size_t head_stride = (size_t)kD << c.page_shift;
-        auto page_of = [&](int n) { return n < mine ? trow[(tok0 + 16 * (warp + kWarps * n)) >> c.page_shift] : 0; };
-        auto issue = [&](int n, int page) {
-            if (n < mine) {
-                const int t = tok0 + 16 * (warp + kWarps * n);
-                const bool ok = (unsigned)page < (unsigned)c.pages;
-                const size_t off = ((size_t)(ok ? page : 0) * c.Hkv + h) * head_stride + (size_t)(t & ((1 << c.page_shift) - 1)) * kD;
-                const unsigned char* kp = static_cast<const unsigned char*>(c.k_cache) + off;
-                const unsigned char* vp = static_cast<const unsigned char*>(c.v_cache) + off;
-                unsigned char* st = ring + (n % kStages) * kStageBytes;
-                const int left = ok ? tok1 - t : 0;  // rows behind the end arrive as zeros
+            for (int d = 0; d < 8; ++d)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = (lane >> 2) + 8 * (i >> 1), ch = (lane & 3) + 4 * (i & 1);
-                    cp_async16(st + i * 512, kp + row * kD + ch * 16, row < left);
-                }
+                for (int e = 0; e < 4; ++e) acc[j][d][e] = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = 2 * (lane & 3) + (i & 1) + 8 * (i >> 1);
-                    cp_async16(st + 2048 + i * 512, vp + row * kD + (lane >> 2) * 16, row < left);
-                }
+            for (int r = 0; r < 2; ++r) {
+                const int row = 8 * j + 2 * (lane & 3) + r;
+                m[j][r] = -INFINITY;
+                l[j][r] = 0.f;
+                rf[j][r] = s_f[row];
+                lim[j][r] = len - p.Q + 1 + (row0 + row) / G;
             }
-            cp_async_commit();
-        };
-        int pg[kStages];  // pages of the steps in the ring, and of the next one to issue
+        }
+        const int all_see = len - p.Q + 1 + row0 / G;  // positions that every row of the tile sees
+        uint2 qf[NT == 1 ? 8 : 1];
+        if (NT == 1) {
 #pragma unroll
-        for (int n = 0; n < kStages; ++n) pg[n] = page_of(n);
-#pragma unroll
-        for (int n = 0; n < kStages - 1; ++n) issue(n, pg[n]);
+            for (int e = 0; e < 8; ++e) qf[NT == 1 ? e : 0] = *reinterpret_cast<const uint2*>(att_sm + S::kOffQ + e * 256 + lane * 8);
+        }
 
+        int stage = 0, next = 2;
+#pragma unroll 1
         for (int n = 0; n < mine; ++n) {
-            const int page = pg[0];
-            issue(n + kStages - 1, pg[kStages - 1]);
-#pragma unroll
-            for (int i = 0; i + 1 < kStages; ++i) pg[i] = pg[i + 1];
-            pg[kStages - 1] = page_of(n + kStages);
-            const bool ok = (unsigned)page < (unsigned)c.pages;
+            issue(n + 2, next, pg2);
+            const bool ok = (unsigned)pg0 < (unsigned)c.pages;
             if (!ok) s_status = kErrBadPage;
-            const size_t si = (size_t)(ok ? page : 0) * c.Hkv + h;
-            const float ks = c.k_scale[si], vs = ok ? c.v_scale[si] : 0.f;
-            cp_async_wait<kStages - 1>();
-            const unsigned char* st = ring + (n % kStages) * kStageBytes;
-            const int t = tok0 + 16 * (warp + kWarps * n);
+            const float ks0 = ks, vs0 = ok ? vs : 0.f;
+            pg0 = pg1;
+            pg1 = pg2;
+            pg2 = page_of(n + 3);
+            if (n + 1 < mine) {
+                ks = c.k_scale[scale_at(pg0)];
+                vs = c.v_scale[scale_at(pg0)];
+            }
+            cp_async_wait<2>();
+            const unsigned char* st = ring + stage * kStageBytes;
+            const int t = t_first + 16 * kWarps * n;
 
-            float s[2][4] = {};
+            float s[NT][4] = {};  // tokens lane / 4 and + 8, rows 2 (lane % 4) and the next: [token + 8][row]
 #pragma unroll
             for (int half = 0; half < 2; ++half) {  // dims 0-63, 64-127
-                uint4 kk[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    kk[i] = *reinterpret_cast<const uint4*>(st + (2 * i + half) * 512);
-                    if (kInt8) kk[i] = make_uint4(kk[i].x ^ 0x80808080u, kk[i].y ^ 0x80808080u, kk[i].z ^ 0x80808080u, kk[i].w ^ 0x80808080u);
-                }
+                const uint4 k0 = load_codes<kInt8>(st + half * 512), k1 = load_codes<kInt8>(st + (2 + half) * 512);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint4 a = *reinterpret_cast<const uint4*>(sm + kOffQ + (4 * half + e) * 512 + lane * 16);
+                    const uint32_t w0 = word(k0, e), w1 = word(k1, e);
+                    const uint32_t a[4] = {codes_f16<kInt8, false>(w0), codes_f16<kInt8, false>(w1), codes_f16<kInt8, true>(w0), codes_f16<kInt8, true>(w1)};
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t w = e == 0 ? kk[i].x : e == 1 ? kk[i].y : e == 2 ? kk[i].z : kk[i].w;
-                        mma_f16(s[i], a.x, a.y, a.z, a.w, codes_f16<kInt8, false>(w), codes_f16<kInt8, true>(w));
+                    for (int j = 0; j < NT; ++j) {
+                        const uint2 q = NT == 1 ? qf[NT == 1 ? 4 * half + e : 0]
+                                                : *reinterpret_cast<const uint2*>(att_sm + S::kOffQ + j * 2048 + (4 * half + e) * 256 + lane * 8);
+                        mma_f16(s[j], a, q.x, q.y);
                     }
                 }
             }
             // scores in base 2; hidden ones are -infinity
-            float top[2] = {m[0], m[1]};
+            bool over = false;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int pos = t + 8 * i + 2 * (lane & 3) + (e & 1);
-                    s[i][e] = ok && pos < lim[e >> 1] ? s[i][e] * (ks * rf[e >> 1]) : -INFINITY;
-                    top[e >> 1] = fmaxf(top[e >> 1], s[i][e]);
-                }
+                for (int e = 0; e < 4; ++e) s[j][e] *= ks0 * rf[j][e & 1];
+            if (t + 16 > all_see || !ok) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!ok || t + (lane >> 2) + 8 * (e >> 1) >= lim[j][e & 1]) s[j][e] = -INFINITY;
             }
-            const float vnew = fmaxf(vref, vs);
-            if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1]) || vnew > vref) {
-                const float vr = vnew > 0.f ? vref / vnew : 1.f;
-                float f[2];
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    f[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - top[r]);
-                    l[r] *= f[r];
-                    f[r] *= vr;
-                    m[r] = top[r];
-                }
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) over |= s[j][e] > m[j][e & 1] + kSlack;
+            const float vnew = fmaxf(vref, vs0);
+            if (__any_sync(0xffffffffu, over) || vnew > vref) {
+                const float vr = vnew > 0.f ? vref / vnew : 1.f;
                 vref = vnew;
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
+                for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[j][e] *= f[e >> 1];
+                    for (int r = 0; r < 2; ++r) {
+                        float top = fmaxf(s[j][r], s[j][2 + r]);
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        top = fmaxf(top, m[j][r]);
+                        const float f = m[j][r] == -INFINITY ? 0.f : ex2(m[j][r] - top);
+                        m[j][r] = top;
+                        l[j][r] *= f;
+#pragma unroll
+                        for (int d = 0; d < 8; ++d) {
+                            acc[j][d][r] *= f * vr;
+                            acc[j][d][2 + r] *= f * vr;
+                        }
+                    }
             }
-            const float mv = vref > 0.f ? vs / vref : 0.f;
-            uint32_t a[4];
+            const float mv = vref > 0.f ? vs0 / vref : 0.f;
+            uint32_t w0[NT], w1[NT];  // weights as B fragments: tokens 2 (lane % 4) + {0, 1} (+ 8), row lane / 4
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int j = 0; j < NT; ++j) {
+                float e[4];
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float base = m[r] == -INFINITY ? 0.f : m[r];
-                    const float x = ex2(s[i][2 * r] - base), y = ex2(s[i][2 * r + 1] - base);
-                    l[r] += x + y;
-                    const __half2 w = __floats2half2_rn(x * mv, y * mv);
-                    a[2 * i + r] = *reinterpret_cast<const uint32_t*>(&w);
+                for (int i = 0; i < 4; ++i) {
+                    e[i] = ex2(s[j][i] - (m[j][i & 1] == -INFINITY ? 0.f : m[j][i & 1]));
+                    l[j][i & 1] += e[i];
                 }
+                const __half2 x = __floats2half2_rn(e[0] * mv, e[1] * mv), y = __floats2half2_rn(e[2] * mv, e[3] * mv);
+                w0[j] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&x));
+                w1[j] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&y));
+            }
             uint4 v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] = *reinterpret_cast<const uint4*>(st + 2048 + i * 512);
-                if (kInt8) v[i] = make_uint4(v[i].x ^ 0x80808080u, v[i].y ^ 0x80808080u, v[i].z ^ 0x80808080u, v[i].w ^ 0x80808080u);
-            }
+            for (int i = 0; i < 4; ++i) v[i] = load_codes<kInt8>(st + 2048 + i * 512);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {  // dims 4 e .. 4 e + 3 of the lane's 16
-                uint32_t x[2][2];
+            for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint4 &v0 = v[2 * i], &v1 = v[2 * i + 1];
-                    const uint32_t w0 = e == 0 ? v0.x : e == 1 ? v0.y : e == 2 ? v0.z : v0.w;
-                    const uint32_t w1 = e == 0 ? v1.x : e == 1 ? v1.y : e == 2 ? v1.z : v1.w;
-                    x[i][0] = __byte_perm(w0, w1, 0x5140);  // tokens t, t + 1 of dims 0 and 1
-                    x[i][1] = __byte_perm(w0, w1, 0x7362);
+                for (int d = 0; d < 2; ++d) {  // dims 16 (lane / 4) + 4 e + 2 d and the next: rows lane / 4 and + 8 of the tile
+                    const uint32_t x = __byte_perm(word(v[0], e), word(v[1], e), d ? 0x7362 : 0x5140);
+                    const uint32_t y = __byte_perm(word(v[2], e), word(v[3], e), d ? 0x7362 : 0x5140);
+                    const uint32_t a[4] = {codes_f16<kInt8, false>(x), codes_f16<kInt8, true>(x), codes_f16<kInt8, false>(y), codes_f16<kInt8, true>(y)};
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) mma_f16(acc[j][2 * e + d], a, w0[j], w1[j]);
                 }
-#pragma unroll
-                for (int d = 0; d < 2; ++d) {
-                    mma_f16(acc[4 * e + 2 * d], a[0], a[1], a[2], a[3], codes_f16<kInt8, false>(x[0][d]), codes_f16<kInt8, false>(x[1][d]));
-                    mma_f16(acc[4 * e + 2 * d + 1], a[0], a[1], a[2], a[3], codes_f16<kInt8, true>(x[0][d]), codes_f16<kInt8, true>(x[1][d]));
-                }
-            }
+            stage = stage == 2 ? 0 : stage + 1;
+            next = next == 2 ? 0 : next + 1;
         }
         cp_async_wait<0>();
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        }
 
         // join the warps: every warp's result at the common maximum
-        if ((lane & 3) == 0) {
-            s_m[warp * 16 + (lane >> 2)] = m[0];
-            s_m[warp * 16 + (lane >> 2) + 8] = m[1];
-            s_l[warp * 16 + (lane >> 2)] = l[0];
-            s_l[warp * 16 + (lane >> 2) + 8] = l[1];
-        }
-        __syncthreads();  // also: every warp is done with its ring
-        float* wacc = reinterpret_cast<float*>(sm);  // [kWarps][16][128], 16-byte chunks XORed with the row
-        float mall[2];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            mall[r] = -INFINITY;
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) mall[r] = fmaxf(mall[r], s_m[w * 16 + (lane >> 2) + 8 * r]);
-            const float f = l[r] != 0.f ? ex2(m[r] - mall[r]) * vref : 0.f;
-            const int row = (lane >> 2) + 8 * r;
+            for (int r = 0; r < 2; ++r) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e)  // dims 32 (lane % 4) + 16 e + 0 .. 15
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int ch = 8 * (lane & 3) + 4 * e + j;
-                    *reinterpret_cast<float4*>(wacc + (warp * 16 + row) * 128 + (ch ^ (row & 7)) * 4) =
-                        make_float4(acc[4 * j][2 * r + e] * f, acc[4 * j + 1][2 * r + e] * f, acc[4 * j + 2][2 * r + e] * f,
-                                    acc[4 * j + 3][2 * r + e] * f);
+                for (int off = 4; off < 32; off <<= 1) l[j][r] += __shfl_xor_sync(0xffffffffu, l[j][r], off);
+                if (lane < 4) {
+                    s_m[warp * kRows + 8 * j + 2 * lane + r] = m[j][r];
+                    s_l[warp * kRows + 8 * j + 2 * lane + r] = l[j][r];
                 }
-        }
+            }
+        __syncthreads();  // also: every warp is done with its ring
+        float* wacc = reinterpret_cast<float*>(att_sm);  // [kWarps][kRows][128], 16-byte chunks XORed with the row
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = 8 * j + 2 * (lane & 3) + r;
+                float mall = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) mall = fmaxf(mall, s_m[w * kRows + row]);
+                const float f = l[j][r] != 0.f ? ex2(m[j][r] - mall) * vref : 0.f;  // a NaN stays one
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    *reinterpret_cast<float4*>(wacc + (warp * kRows + row) * 128 + ((4 * (lane >> 2) + e) ^ (row & 7)) * 4) =
+                        make_float4(acc[j][2 * e][r] * f, acc[j][2 * e][2 + r] * f, acc[j][2 * e + 1][r] * f, acc[j][2 * e + 1][2 + r] * f);
+            }
         __syncthreads();
-        {
-            const int row = tid >> 4;
+        const bool whole = at == seg_begin && stop == seg_end;
+#pragma unroll 1
+        for (int row = tid >> 5; row < min(kRows, R - row0); row += kThreads / 32) {  // a warp a row, four dims a lane
             float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w * 16 + row]);
+            for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w * kRows + row]);
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float mw = s_m[w * 16 + row];
-                const float lw = s_l[w * 16 + row];
-                if (lw != 0.f) ll += lw * ex2(mw - mm);  // a NaN stays one
+                const float lw = s_l[w * kRows + row];
+                if (lw != 0.f) ll += lw * ex2(s_m[w * kRows + row] - mm);
+                const float4 x = *reinterpret_cast<const float4*>(wacc + (w * kRows + row) * 128 + (lane ^ (row & 7)) * 4);
+                o = make_float4(o.x + x.x, o.y + x.y, o.z + x.z, o.w + x.w);
             }
-            float o[8] = {};
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int ch = 2 * (tid & 15) + e;
-                    const float4 x = *reinterpret_cast<const float4*>(wacc + (w * 16 + row) * 128 + (ch ^ (row & 7)) * 4);
-                    o[4 * e] += x.x;
-                    o[4 * e + 1] += x.y;
-                    o[4 * e + 2] += x.z;
-                    o[4 * e + 3] += x.w;
-                }
-            const bool whole = at == seg_begin && stop == seg_end;
-            const int r = row0 + row;
-            if (r < R) {
-                if (whole) {
-                    const float inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
-                    uint32_t u[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) u[e] = pack_bf16x2(o[2 * e] * inv, o[2 * e + 1] * inv);
-                    *reinterpret_cast<uint4*>(p.out + (((size_t)b * p.Q + r / G) * p.Hq + h * G + r % G) * kD + 8 * (tid & 15)) =
-                        make_uint4(u[0], u[1], u[2], u[3]);
-                } else {
-                    const size_t slot = (2 * (size_t)blockIdx.x + (at == seg_begin ? 1 : 0)) * 16 + row;
-                    float4* d = reinterpret_cast<float4*>(p.acc + slot * 128 + 8 * (tid & 15));
-                    d[0] = make_float4(o[0], o[1], o[2], o[3]);
-                    d[1] = make_float4(o[4], o[5], o[6], o[7]);
-                    if ((tid & 15) == 0) {
-                        p.ml[slot * 2] = mm;
-                        p.ml[slot * 2 + 1] = ll;
-                    }
-                }
-            }
-            if (!whole && at == seg_begin && tid == 0) {
-                // the CTA that holds the segment's last block
-                const long long last = (seg_end * ctas - 1) / total;
-                piece = make_int2(b * segs + seg, (int)(last - blockIdx.x));
+            if (whole) {
+                const int r = row0 + row, i = r / G;
+                const float inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
+                *reinterpret_cast<uint2*>(p.out + (((size_t)b * p.Q + i) * p.Hq + h * G + r - i * G) * kD + 4 * lane) =
+                    make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+            } else {
+                const size_t slot = (2 * (size_t)blockIdx.x + (at == seg_begin ? 1 : 0)) * kRows + row;
+                *reinterpret_cast<float4*>(p.acc + slot * 128 + 4 * lane) = o;
+                if (lane == 0) *reinterpret_cast<float2*>(p.ml + slot * 2) = make_float2(mm, ll);
             }
         }
+        if (!whole && at == seg_begin)  // the pieces that follow
+            piece = make_int2(b * segs + seg, cta_of(seg_end - 1, line.total, line.ctas) - (int)blockIdx.x);
         at = stop;
         __syncthreads();
     }
@@ -435,7 +431,7 @@ __global__ void __launch_bounds__(att::kThreads, 2) gdn_cache_attend_kernel(Cach
 }
 
 // Joins a segment that several CTAs of the line hold: CTA x takes the one that CTA x began, row y of its tile.
-__global__ void __launch_bounds__(128) gdn_cache_join_kernel(CacheAttendArgs p) {
+__global__ void __launch_bounds__(128) gdn_cache_join_kernel(CacheAttendArgs p, int rows) {
     __shared__ float4 s_o[4][32];
     __shared__ float s_l[4];
     pdl_wait();
@@ -448,11 +444,11 @@ __global__ void __launch_bounds__(128) gdn_cache_join_kernel(CacheAttendArgs p) 
     }
     const int4 pc = p.piece[blockIdx.x];
     if (pc.x < 0) return;
-    const int G = p.Hq / p.c.Hkv, R = p.Q * G, tiles = (R + 15) / 16, segs = p.c.Hkv * tiles;
-    const int b = pc.x / segs, seg = pc.x % segs, h = seg / tiles, r = (seg % tiles) * 16 + blockIdx.y;
+    const int G = p.Hq / p.c.Hkv, R = p.Q * G, tiles = (R + rows - 1) / rows, segs = p.c.Hkv * tiles;
+    const int b = pc.x / segs, seg = pc.x % segs, h = seg / tiles, r = (seg % tiles) * rows + blockIdx.y;
     if (r >= R) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    auto slot = [&](int i) { return ((size_t)(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0))) * 16 + blockIdx.y; };
+    auto slot = [&](int i) { return ((size_t)(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0))) * rows + blockIdx.y; };
     float m = -INFINITY;
     for (int i = lane; i <= pc.y; i += 32) m = fmaxf(m, p.ml[slot(i) * 2]);
 #pragma unroll
@@ -484,18 +480,24 @@ __global__ void __launch_bounds__(128) gdn_cache_join_kernel(CacheAttendArgs p) 
     }
 }
 
-template <bool kInt8>
+template <bool kInt8, int NT>
 static int launch_attend(const CacheAttendArgs& p, cudaStream_t stream) {
-    if (cudaFuncSetAttribute(gdn_cache_attend_kernel<kInt8>, cudaFuncAttributeMaxDynamicSharedMemorySize, att::kSmem) != cudaSuccess)
+    constexpr int kRows = 8 * NT, kSmem = att::Smem<NT>::kSize;
+    const unsigned ctas = NT < 4 ? kAttendCtas : kAttendCtas / 2;  // what fits on the SMs together
+    if (cudaFuncSetAttribute(gdn_cache_attend_kernel<kInt8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
         return -1;
-    if (launch_pdl(gdn_cache_attend_kernel<kInt8>, dim3(kAttendCtas), dim3(att::kThreads), att::kSmem, stream, p) != cudaSuccess)
-        return -1;
+    if (launch_pdl(gdn_cache_attend_kernel<kInt8, NT>, dim3(ctas), dim3(att::kThreads), kSmem, stream, p) != cudaSuccess) return -1;
     const int rows = p.Q * (p.Hq / p.c.Hkv);
-    return launch_pdl(gdn_cache_join_kernel, dim3(kAttendCtas, (unsigned)(rows < 16 ? rows : 16)), dim3(128), 0, stream, p) == cudaSuccess ? 0 : -1;
+    return launch_pdl(gdn_cache_join_kernel, dim3(ctas, (unsigned)(rows < kRows ? rows : kRows)), dim3(128), 0, stream, p, kRows) == cudaSuccess ? 0 : -1;
 }
 
+// Column tiles of 8 rows: as many as a kv head's q rows need, at most 4 (the accumulators fill the registers).
+int attend_tiles(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+
 int launch_cache_attend(const CacheAttendArgs& p, cudaStream_t stream) {
-    return p.c.int8 ? launch_attend<true>(p, stream) : launch_attend<false>(p, stream);
+    const int nt = attend_tiles(p.Q * (p.Hq / p.c.Hkv));
+    if (p.c.int8) return nt == 1 ? launch_attend<true, 1>(p, stream) : nt == 2 ? launch_attend<true, 2>(p, stream) : launch_attend<true, 4>(p, stream);
+    return nt == 1 ? launch_attend<false, 1>(p, stream) : nt == 2 ? launch_attend<false, 2>(p, stream) : launch_attend<false, 4>(p, stream);
 }
 
 }  // namespace gdn

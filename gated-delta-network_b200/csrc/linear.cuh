@@ -91,10 +91,11 @@ struct CacheAttendArgs {
     uint16_t* out;         // [B, Q, Hq, 128] bf16
     int* status;           // workspace
     int4* piece;           // workspace: [kAttendCtas] {segment that CTA c begins and others end, pieces that follow, status}
-    float* ml;             // workspace: [kAttendCtas][2][16][2] running maximum (base 2) and sum of a piece
-    float* acc;            // workspace: [kAttendCtas][2][16][128]
+    float* ml;             // workspace: [CTAs][2][rows of a tile][2] reference (base 2) and sum of a piece
+    float* acc;            // workspace: [CTAs][2][rows of a tile][128]
 };
-constexpr int kAttendCtas = 296;  // 2 per SM
+constexpr int kAttendCtas = 296;  // 2 per SM with tiles of up to 16 rows; half as many with tiles of 32
+int attend_tiles(int rows);
 
 int launch_cache_append(const CacheAppendArgs& p, cudaStream_t stream);
 int launch_cache_attend(const CacheAttendArgs& p, cudaStream_t stream);
