@@ -368,7 +368,7 @@ int gdn_cache_attend(const void* q, const void* k_cache, const void* v_cache, co
         const long long rows = (long long)Q * (Hq / Hkv);
         if (rows > (1 << 20)) return GDN_ERR_SIZE;
         const long long tile = 8 * gdn::attend_tiles((int)rows), segs = Hkv * ((rows + tile - 1) / tile);
-        if (B * segs * std::max<long long>(1, ((long long)max_pages * page_size + 31) / 32) > 0x7fffffffll) return GDN_ERR_SIZE;
+        if (B * segs * (((long long)max_pages * page_size + 31) / 32 + 17) > 0x7fffffffll) return GDN_ERR_SIZE;
     }
     if (B == 0 || Q == 0) return GDN_OK;
     if (!q || !out) return GDN_ERR_NULL;

@@ -34,6 +34,8 @@ constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kBlock = 32;                       // tokens of the unit that is divided over the CTAs
 constexpr int kStages = 3;
 constexpr int kStageBytes = 4096;                // a warp's 16 tokens of k and v: 8 x 16 bytes a lane
+constexpr int kOwn = 16;                         // places of a segment on the line besides its blocks
+constexpr int kKeep = 16;                        // segments of at most this many blocks are not cut
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 4.f;                    // scores may exceed the reference by this (base 2)
 // Shared memory for tiles of 8 NT rows: the ring, whose place the warps' results take; q as B fragments
@@ -89,42 +91,56 @@ __device__ __forceinline__ int seq_blocks(const CacheArgs& c, int b) {
     return max(1, (visible_length(c, b) + att::kBlock - 1) / att::kBlock);
 }
 
-// Total blocks of the line, the number of CTAs that share it, and where this CTA's stretch begins: its place, the
-// sequence there and the place of that sequence's first block.  By one warp, every lane with an equal part of the
-// sequences.  (Places are ints: the entry point refuses more.)
-struct Stretch {
-    int total, ctas, first, end, b, begin;
+// The line of segments: each has its blocks and kOwn places more, for what a piece costs before and after its tokens
+// (the q fragments, the first pages, the warps' join).  A CTA's stretch goes from one mark to another.  (Places are
+// ints: the entry point refuses more.)
+struct AttMark {
+    int b, seg, block, before;  // block of segment `seg` of sequence b; places in front of the sequence
 };
+struct Stretch {
+    AttMark at, end;
+    int total, ctas;
+};
+// By one warp, every lane with an equal part of the sequences.
 __device__ __forceinline__ void find_stretch(const CacheArgs& c, int segs, Stretch* out) {
+    using namespace att;
     const int lane = threadIdx.x & 31, part = (c.B + 31) / 32, b0 = min(c.B, lane * part), b1 = min(c.B, b0 + part);
-    int x = 0, mine = 0;
+    int mine = 0;
 #pragma unroll 4
-    for (int b = b0; b < b1; ++b) mine += seq_blocks(c, b);
-    x = mine;
+    for (int b = b0; b < b1; ++b) mine += seq_blocks(c, b) + kOwn;
+    int x = mine;
 #pragma unroll 1
     for (int off = 1; off < 32; off <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, off);
         if (lane >= off) x += y;
     }
     const int total = __shfl_sync(0xffffffffu, x, 31) * segs;
-    // at least a block for each warp, so that short caches are not cut into more pieces than they are worth
-    const int ctas = min((int)gridDim.x, (total + att::kWarps - 1) / att::kWarps), per = total / ctas, more = total - per * ctas;
-    const int k = blockIdx.x, first = min(total, k * per + min(k, more));
-    int lo = (x - mine) * segs;
-    if (first >= lo && first < lo + mine * segs) {
-        int b = b0, n = seq_blocks(c, b) * segs;
-        while (first >= lo + n) {
-            lo += n;
-            n = seq_blocks(c, ++b) * segs;
-        }
-        out->b = b;
-        out->begin = lo;
-    }
+    const int ctas = max(1, min((int)gridDim.x, total / (kOwn + kWarps))), per = total / ctas, more = total - per * ctas;
     if (lane == 0) {
         out->total = total;
         out->ctas = ctas;
-        out->first = first;
-        out->end = min(total, (k + 1) * per + min(k + 1, more));
+    }
+    const int first = (x - mine) * segs;
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+        const int k = blockIdx.x + i, want = min(total, k * per + min(k, more));
+        AttMark* m = i ? &out->end : &out->at;
+        if (lane == 0 && want == total) *m = AttMark{c.B, 0, 0, total};
+        int lo = first;
+        if (want < lo || want >= lo + mine * segs) continue;
+        int b = b0, w = seq_blocks(c, b) + kOwn;
+        while (want >= lo + w * segs) {
+            lo += w * segs;
+            w = seq_blocks(c, ++b) + kOwn;
+        }
+        AttMark r{b, (want - lo) / w, 0, lo};
+        const int place = want - lo - r.seg * w - kOwn;
+        if (w - kOwn > kKeep) {
+            r.block = max(0, place);
+        } else if (2 * place >= w - kOwn && ++r.seg == segs) {  // a short segment is not cut: to its nearer end
+            r = AttMark{b + 1, 0, 0, lo + w * segs};
+        }
+        *m = r;
     }
 }
 // The CTA whose stretch holds place x.
@@ -155,21 +171,14 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_atten
     __syncthreads();
     const Stretch line = s_line;
     int2 piece = make_int2(-1, 0);  // the segment that begins here and ends elsewhere (thread 0)
-    int b = line.b, begin = line.begin;
 
 #pragma unroll 1
-    for (int at = line.first; at < line.end;) {
-        const int nb = seq_blocks(c, b);
-        if (at >= begin + nb * segs) {
-            begin += nb * segs;
-            ++b;
-            continue;
-        }
-        const int seg = (at - begin) / nb, h = seg / tiles, row0 = (seg - h * tiles) * kRows;
-        const int seg_begin = begin + seg * nb, seg_end = seg_begin + nb, stop = min(seg_end, line.end);
-        const int len = visible_length(c, b);
+    for (AttMark at = line.at; at.b < line.end.b || (at.b == line.end.b && (at.seg < line.end.seg || (at.seg == line.end.seg && at.block < line.end.block)));) {
+        const int b = at.b, seg = at.seg, h = seg / tiles, row0 = (seg - h * tiles) * kRows;
+        const int len = visible_length(c, b), nb = max(1, (len + kBlock - 1) / kBlock);
+        const int stop = b == line.end.b && seg == line.end.seg ? line.end.block : nb;
         if (tid == 0 && cache_length(c, b) > len) s_status = kErrBadSeqlens;
-        const int tok0 = (at - seg_begin) * kBlock, tok1 = min(len, (stop - seg_begin) * kBlock);
+        const int tok0 = at.block * kBlock, tok1 = min(len, stop * kBlock);
         const int steps = tok1 > tok0 ? (tok1 - tok0 + 15) / 16 : 0;
 
         unsigned char* ring = att_sm + warp * kStages * kStageBytes + lane * 16;
@@ -397,7 +406,7 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_atten
                         make_float4(acc[j][2 * e][r] * f, acc[j][2 * e][2 + r] * f, acc[j][2 * e + 1][r] * f, acc[j][2 * e + 1][2 + r] * f);
             }
         __syncthreads();
-        const bool whole = at == seg_begin && stop == seg_end;
+        const bool begins = at.block == 0, whole = begins && stop == nb;
 #pragma unroll 1
         for (int row = tid >> 5; row < min(kRows, R - row0); row += kThreads / 32) {  // a warp a row, four dims a lane
             float mm = -INFINITY, ll = 0.f;
@@ -417,14 +426,19 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_atten
                 *reinterpret_cast<uint2*>(p.out + (((size_t)b * p.Q + i) * p.Hq + h * G + r - i * G) * kD + 4 * lane) =
                     make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
             } else {
-                const size_t slot = (2 * (size_t)blockIdx.x + (at == seg_begin ? 1 : 0)) * kRows + row;
+                const size_t slot = (2 * (size_t)blockIdx.x + (begins ? 1 : 0)) * kRows + row;
                 *reinterpret_cast<float4*>(p.acc + slot * 128 + 4 * lane) = o;
                 if (lane == 0) *reinterpret_cast<float2*>(p.ml + slot * 2) = make_float2(mm, ll);
             }
         }
-        if (!whole && at == seg_begin)  // the pieces that follow
-            piece = make_int2(b * segs + seg, cta_of(seg_end - 1, line.total, line.ctas) - (int)blockIdx.x);
-        at = stop;
+        if (!whole && begins)  // the pieces that follow
+            piece = make_int2(b * segs + seg, cta_of(at.before + seg * (nb + kOwn) + kOwn + nb - 1, line.total, line.ctas) - (int)blockIdx.x);
+        at.block = 0;
+        if (++at.seg == segs) {
+            at.seg = 0;
+            at.before += (nb + kOwn) * segs;
+            ++at.b;
+        }
         __syncthreads();
     }
     if (tid == 0) p.piece[blockIdx.x] = make_int4(piece.x, piece.y, s_status, 0);
