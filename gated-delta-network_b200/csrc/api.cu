@@ -377,6 +377,7 @@ int gdn_cache_attend(const void* q, const void* k_cache, const void* v_cache, co
         return GDN_ERR_WORKSPACE;
     rc = check_device();
     if (rc != GDN_OK) return rc;
+    if (((long long)num_pages * Hkv) * page_size > 0x7fffffffll) return GDN_ERR_SIZE;  // rows are int coordinates
     if (num_pages == 0) p.c.max_pages = 0;  // an empty cache: every row sees nothing
     unsigned char* ws = static_cast<unsigned char*>(workspace);
     p.q = static_cast<const uint16_t*>(q);

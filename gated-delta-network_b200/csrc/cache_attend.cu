@@ -16,9 +16,10 @@
 //  * The value scale enters the weights: p v_scale / r with r the largest value scale so far, kept like the maximum,
 //    so the accumulator never sees the scales' range.
 //  * Both contractions may permute their index, so a thread takes 16 consecutive bytes of a row and no fragment
-//    needs a shuffle or a transposing load: key step s of lane l holds dims 16 (l % 4) + 4 s .. and the same of q;
-//    value lane l holds dims 16 (l / 4) .. of the four tokens whose weights it owns (after one 8 x 8 transpose). Every
-//    thread reads back only the shared memory it filled itself (cp.async), so the ring needs no barrier.
+//    needs a shuffle or a transposing load: key step s of lane l holds dims 32 (l % 4) + 4 s .. and the same of q;
+//    value lane l holds dims 16 (l / 4) .. of the four tokens whose weights it owns (after one 8 x 8 transpose).
+//  * 16 tokens of k or v of a head are 2 KB in a row, one TMA copy; every warp has a ring of three such pairs of its
+//    own.  (16-byte cp.async into the same ring stopped at 4.6 TB/s with nothing saturated.)
 //  * Tokens are cut evenly over the CTAs whatever the lengths: all (sequence, head, row tile) segments in 32-token
 //    blocks on one line, an equal stretch of it per CTA. A stretch's first and last segment may continue in a
 //    neighbour; those pieces go to the workspace, and a second launch joins them.
@@ -26,6 +27,7 @@
 
 #include "linear.cuh"
 #include "prefill_kernels.cuh"
+#include "sm100.cuh"
 
 namespace gdn {
 
@@ -33,23 +35,23 @@ namespace att {
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kBlock = 32;                       // tokens of the unit that is divided over the CTAs
 constexpr int kStages = 3;
-constexpr int kStageBytes = 4096;                // a warp's 16 tokens of k and v: 8 x 16 bytes a lane
+constexpr int kStageBytes = 4096;                // a warp's 16 tokens of k and of v, rows of 128 bytes, SWIZZLE_128B
 constexpr int kOwn = 16;                         // places of a segment on the line besides its blocks
 constexpr int kKeep = 16;                        // segments of at most this many blocks are not cut
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 4.f;                    // scores may exceed the reference by this (base 2)
 // Shared memory for tiles of 8 NT rows: the ring, whose place the warps' results take; q as B fragments
-// [NT][8 steps][32 lanes][8 bytes]; f32 [8 NT] row factors; f32 [kWarps][8 NT] references, then sums.
+// [NT][8 steps][32 lanes][8 bytes]; f32 [8 NT] row factors; f32 [kWarps][8 NT] references, then sums; the ring's barriers.
 template <int NT>
 struct Smem {
     static constexpr int kRing = kWarps * kStages * kStageBytes, kJoin = kWarps * 8 * NT * 128 * 4;
     static constexpr int kOffQ = kRing > kJoin ? kRing : kJoin, kOffF = kOffQ + NT * 2048, kOffM = kOffF + NT * 32;
-    static constexpr int kSize = kOffM + 2 * kWarps * 8 * NT * 4;
+    static constexpr int kOffBar = kOffM + 2 * kWarps * 8 * NT * 4, kSize = kOffBar + kWarps * kStages * 8;
 };
 }  // namespace att
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -61,7 +63,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 // The two codes in the low (kHigh: high) half of w as fp16, exactly.  int8: w holds code + 128.
@@ -149,12 +151,17 @@ __device__ __forceinline__ int cta_of(int x, int total, int ctas) {
     return x < big ? x / (per + 1) : more + (x - big) / per;
 }
 
+struct AttendMaps {
+    CUtensorMap k, v;  // (128 bytes, rows of all pages) u8, box 128 x 16, SWIZZLE_128B
+};
+
 template <bool kInt8, int NT>
-__global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_attend_kernel(CacheAttendArgs p) {
+__global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
+    gdn_cache_attend_kernel(CacheAttendArgs p, const __grid_constant__ AttendMaps maps) {
     using namespace att;
     using S = Smem<NT>;
     constexpr int kRows = 8 * NT;
-    extern __shared__ __align__(128) unsigned char att_sm[];
+    extern __shared__ __align__(1024) unsigned char att_sm[];
     __shared__ Stretch s_line;
     __shared__ int s_status;
     const CacheArgs& c = p.c;
@@ -162,7 +169,12 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_atten
     float* s_f = reinterpret_cast<float*>(att_sm + S::kOffF);
     float* s_m = reinterpret_cast<float*>(att_sm + S::kOffM);
     float* s_l = s_m + kWarps * kRows;
-    if (tid == 0) s_status = 0;
+    if (tid == 0) s_status = (smem_u32(att_sm) & 1023u) ? kErrScanTmaTimeout : 0;  // (the swizzled tiles need the alignment)
+    uint64_t* bars = reinterpret_cast<uint64_t*>(att_sm + S::kOffBar) + warp * kStages;
+    if (lane == 0) {
+        for (int i = 0; i < kStages; ++i) mbar_init(bars + i, 1);
+        mbar_fence_init();
+    }
     pdl_wait();
     pdl_trigger();
 
@@ -171,6 +183,8 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_atten
     __syncthreads();
     const Stretch line = s_line;
     int2 piece = make_int2(-1, 0);  // the segment that begins here and ends elsewhere (thread 0)
+    int place = 0;                  // ring place of the next step to read
+    uint32_t phases = 0;            // and the phases of the ring's barriers
 
 #pragma unroll 1
     for (AttMark at = line.at; at.b < line.end.b || (at.b == line.end.b && (at.seg < line.end.seg || (at.seg == line.end.seg && at.block < line.end.block)));) {
@@ -181,32 +195,34 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_atten
         const int tok0 = at.block * kBlock, tok1 = min(len, stop * kBlock);
         const int steps = tok1 > tok0 ? (tok1 - tok0 + 15) / 16 : 0;
 
-        unsigned char* ring = att_sm + warp * kStages * kStageBytes + lane * 16;
+        unsigned char* ring = att_sm + warp * kStages * kStageBytes;
         const int mine = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;  // steps warp, warp + 8, ..
         const int* trow = c.table + (size_t)b * c.max_pages;
         const int t_first = tok0 + 16 * warp;
         auto page_of = [&](int n) { return n < mine ? trow[(t_first + 16 * kWarps * n) >> c.page_shift] : 0; };
-        auto issue = [&](int n, int stage, int page) {
-            if (n < mine) {
-                const int t = t_first + 16 * kWarps * n;
-                const bool ok = (unsigned)page < (unsigned)c.pages;
-                const size_t off = ((((size_t)(ok ? page : 0) * c.Hkv + h) << c.page_shift) + (t & ((1 << c.page_shift) - 1))) * kD;
-                const unsigned char* kp = static_cast<const unsigned char*>(c.k_cache) + off + (lane >> 2) * kD + (lane & 3) * 16;
-                const unsigned char* vp = static_cast<const unsigned char*>(c.v_cache) + off + (lane & 3) * 2 * kD + (lane >> 2) * 16;
-                unsigned char* st = ring + stage * kStageBytes;
-                const int left = ok ? tok1 - t : 0;  // rows behind the end arrive as zeros
-#pragma unroll
-                for (int i = 0; i < 4; ++i)  // token lane / 4 (+ 8), 16-byte chunk lane % 4 (+ 4)
-                    cp_async16(st + i * 512, kp + 8 * (i >> 1) * kD + 64 * (i & 1), (lane >> 2) + 8 * (i >> 1) < left);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)  // tokens 2 (lane % 4) + {0, 1} (+ 8), chunk lane / 4
-                    cp_async16(st + 2048 + i * 512, vp + ((i & 1) + 8 * (i >> 1)) * kD, 2 * (lane & 3) + (i & 1) + 8 * (i >> 1) < left);
+        auto issue = [&](int n, int at_, int page) {
+            if (n < mine && lane == 0) {
+                uint64_t* bar = bars + at_;
+                if ((unsigned)page < (unsigned)c.pages) {
+                    const int y = ((page * c.Hkv + h) << c.page_shift) + ((t_first + 16 * kWarps * n) & ((1 << c.page_shift) - 1));
+                    mbar_arrive_expect_tx(bar, kStageBytes);
+                    tma_load_2d(ring + at_ * kStageBytes, &maps.k, 0, y, bar);
+                    tma_load_2d(ring + at_ * kStageBytes + 2048, &maps.v, 0, y, bar);
+                } else {
+                    mbar_arrive(bar);  // no such page: its tokens are hidden
+                }
             }
-            cp_async_commit();
         };
-        int pg0 = page_of(0), pg1 = page_of(1), pg2 = page_of(2);  // pages of the steps in the ring and of the next
-        issue(0, 0, pg0);
-        issue(1, 1, pg1);
+        auto after = [](int at_) { return at_ + 1 == kStages ? 0 : at_ + 1; };
+        auto arrived = [&](int at_) {
+            if (!mbar_wait(bars + at_, (phases >> at_) & 1u, nullptr, 0)) s_status = kErrScanTmaTimeout;
+            phases ^= 1u << at_;
+        };
+        int pg0 = page_of(0), pg1 = page_of(1), pg2 = page_of(2);  // pages of the steps in the ring
+        issue(0, place, pg0);
+        issue(1, after(place), pg1);
+        issue(2, after(after(place)), pg2);
+        int pg3 = page_of(3);
         auto scale_at = [&](int page) { return (size_t)((unsigned)page < (unsigned)c.pages ? page : 0) * c.Hkv + h; };
         float ks = 0.f, vs = 0.f;
         if (mine > 0) {
@@ -234,8 +250,8 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_atten
             const int ex = min(max((int)(__float_as_uint(top) >> 23), 2), 252);
             const float inv = __uint_as_float((uint32_t)(254 - ex) << 23);
             if (x == 0) s_f[r] = __uint_as_float((uint32_t)ex << 23) * (p.scale * kLog2e);
-            // dims 8 x .. 8 x + 7: 16-byte chunk x / 2, steps 2 (x % 2) and the next; the second half of the dims is steps 4-7
-            const int xl = (x >> 1) & 3, s0 = 2 * (x & 1) + 4 * (x >> 3);
+            // dims 8 x .. 8 x + 7: lane x / 4, whose 32 dims are steps 0-7 four by four
+            const int xl = x >> 2, s0 = 2 * (x & 3);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const __half2 lo = __floats2half2_rn(f[4 * e] * inv, f[4 * e + 1] * inv);
@@ -271,28 +287,18 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_atten
             for (int e = 0; e < 8; ++e) qf[NT == 1 ? e : 0] = *reinterpret_cast<const uint2*>(att_sm + S::kOffQ + e * 256 + lane * 8);
         }
 
-        int stage = 0, next = 2;
-#pragma unroll 1
-        for (int n = 0; n < mine; ++n) {
-            issue(n + 2, next, pg2);
-            const bool ok = (unsigned)pg0 < (unsigned)c.pages;
-            if (!ok) s_status = kErrBadPage;
-            const float ks0 = ks, vs0 = ok ? vs : 0.f;
-            pg0 = pg1;
-            pg1 = pg2;
-            pg2 = page_of(n + 3);
-            if (n + 1 < mine) {
-                ks = c.k_scale[scale_at(pg0)];
-                vs = c.v_scale[scale_at(pg0)];
-            }
-            cp_async_wait<2>();
-            const unsigned char* st = ring + stage * kStageBytes;
-            const int t = t_first + 16 * kWarps * n;
-
-            float s[NT][4] = {};  // tokens lane / 4 and + 8, rows 2 (lane % 4) and the next: [token + 8][row]
+        // scores of a step, still without their factors: tokens lane / 4 and + 8, rows 2 (lane % 4) and the next ([token + 8][row])
+        const uint32_t k_off = (lane >> 2) * 128 + (((2 * (lane & 3)) ^ (lane >> 2)) << 4);
+        const uint32_t v_off = 2048 + (2 * (lane & 3)) * 128 + (((lane >> 2) ^ (2 * (lane & 3))) << 4);
+        auto scores = [&](const unsigned char* st, float (&s)[NT][4]) {
+            float s2[NT][4];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {  // dims 0-63, 64-127
-                const uint4 k0 = load_codes<kInt8>(st + half * 512), k1 = load_codes<kInt8>(st + (2 + half) * 512);
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[j][e] = s2[j][e] = 0.f;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {  // 16-byte chunk 2 (lane % 4) + half of the tokens lane / 4 and + 8
+                const uint4 k0 = load_codes<kInt8>(st + (k_off ^ (half << 4))), k1 = load_codes<kInt8>(st + 1024 + (k_off ^ (half << 4)));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t w0 = word(k0, e), w1 = word(k1, e);
@@ -301,10 +307,33 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_atten
                     for (int j = 0; j < NT; ++j) {
                         const uint2 q = NT == 1 ? qf[NT == 1 ? 4 * half + e : 0]
                                                 : *reinterpret_cast<const uint2*>(att_sm + S::kOffQ + j * 2048 + (4 * half + e) * 256 + lane * 8);
-                        mma_f16(s[j], a, q.x, q.y);
+                        mma_f16(half ? s2[j] : s[j], a, q.x, q.y);
                     }
                 }
             }
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[j][e] += s2[j][e];
+        };
+        // The scores of a step are formed beside the softmax and the second product of the one before: a warp has two
+        // chains to work on.  (Those behind the last step are formed from whatever the ring holds, and not used.)
+        float s[NT][4];
+        if (mine > 0) arrived(place);
+        scores(ring + place * kStageBytes, s);
+#pragma unroll 1
+        for (int n = 0; n < mine; ++n) {
+            const bool ok = (unsigned)pg0 < (unsigned)c.pages;
+            if (!ok) s_status = kErrBadPage;
+            const float ks0 = ks, vs0 = ok ? vs : 0.f;
+            pg0 = pg1;
+            pg1 = pg2;
+            pg2 = pg3;
+            if (n + 1 < mine) {
+                ks = c.k_scale[scale_at(pg0)];
+                vs = c.v_scale[scale_at(pg0)];
+            }
+            const int t = t_first + 16 * kWarps * n;
             // scores in base 2; hidden ones are -infinity
             bool over = false;
 #pragma unroll
@@ -346,6 +375,10 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_atten
                     }
             }
             const float mv = vref > 0.f ? vs0 / vref : 0.f;
+            const int next = after(place);
+            if (n + 1 < mine) arrived(next);
+            float sn[NT][4];
+            scores(ring + next * kStageBytes, sn);
             uint32_t w0[NT], w1[NT];  // weights as B fragments: tokens 2 (lane % 4) + {0, 1} (+ 8), row lane / 4
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -361,7 +394,17 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_atten
             }
             uint4 v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = load_codes<kInt8>(st + 2048 + i * 512);
+            for (int i = 0; i < 4; ++i)  // tokens 2 (lane % 4) + {0, 1} (+ 8), chunk lane / 4
+                v[i] = load_codes<kInt8>(ring + place * kStageBytes + 1024 * (i >> 1) + ((v_off + 128 * (i & 1)) ^ ((i & 1) << 4)));
+            if (!ok || t + 16 > tok1) {  // slots behind the sequence's end hold anything: a weight of 0 does not undo a NaN
+                const uint32_t none = kInt8 ? 0x80808080u : 0u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!ok || t + 2 * (lane & 3) + (i & 1) + 8 * (i >> 1) >= tok1) v[i] = make_uint4(none, none, none, none);
+            }
+            __syncwarp();  // the step's place is read: the next one may land there
+            issue(n + 3, place, pg2);
+            pg3 = page_of(n + 4);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -372,10 +415,12 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_atten
 #pragma unroll
                     for (int j = 0; j < NT; ++j) mma_f16(acc[j][2 * e + d], a, w0[j], w1[j]);
                 }
-            stage = stage == 2 ? 0 : stage + 1;
-            next = next == 2 ? 0 : next + 1;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[j][e] = sn[j][e];
+            place = next;
         }
-        cp_async_wait<0>();
 
         // join the warps: every warp's result at the common maximum
 #pragma unroll
@@ -433,6 +478,7 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1) gdn_cache_atten
         }
         if (!whole && begins)  // the pieces that follow
             piece = make_int2(b * segs + seg, cta_of(at.before + seg * (nb + kOwn) + kOwn + nb - 1, line.total, line.ctas) - (int)blockIdx.x);
+        fence_async_smem();  // what was written in the ring's place comes before the next copies
         at.block = 0;
         if (++at.seg == segs) {
             at.seg = 0;
@@ -500,7 +546,12 @@ static int launch_attend(const CacheAttendArgs& p, cudaStream_t stream) {
     const unsigned ctas = NT < 4 ? kAttendCtas : kAttendCtas / 2;  // what fits on the SMs together
     if (cudaFuncSetAttribute(gdn_cache_attend_kernel<kInt8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
         return -1;
-    if (launch_pdl(gdn_cache_attend_kernel<kInt8, NT>, dim3(ctas), dim3(att::kThreads), kSmem, stream, p) != cudaSuccess) return -1;
+    AttendMaps maps{};
+    if (p.c.max_pages > 0) {
+        const uint64_t rows = ((uint64_t)p.c.pages * p.c.Hkv) << p.c.page_shift;
+        if (!map_u8_rows(&maps.k, p.c.k_cache, rows) || !map_u8_rows(&maps.v, p.c.v_cache, rows)) return -3;
+    }
+    if (launch_pdl(gdn_cache_attend_kernel<kInt8, NT>, dim3(ctas), dim3(att::kThreads), kSmem, stream, p, maps) != cudaSuccess) return -1;
     const int rows = p.Q * (p.Hq / p.c.Hkv);
     return launch_pdl(gdn_cache_join_kernel, dim3(ctas, (unsigned)(rows < kRows ? rows : kRows)), dim3(128), 0, stream, p, kRows) == cudaSuccess ? 0 : -1;
 }

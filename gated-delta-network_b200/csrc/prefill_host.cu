@@ -140,6 +140,18 @@ bool map_bf16_rows(CUtensorMap* m, const void* base, int heads, int T) {
                  1, 64, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+bool map_u8_rows(CUtensorMap* m, const void* base, uint64_t rows) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[2] = {128, rows};
+    const cuuint64_t strides[1] = {128};
+    const cuuint32_t box[2] = {128, 16};
+    const cuuint32_t estr[2] = {1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool build_prefill_maps(const PrefillArgs& p, PrefillMaps* m) {
     const uint64_t T = (uint64_t)p.T, R = (uint64_t)p.S * kChunk;
     const auto BF = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;

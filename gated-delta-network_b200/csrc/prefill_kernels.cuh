@@ -120,6 +120,8 @@ __device__ __forceinline__ int clamp_chunks(const PrefillArgs& p, int slot0, int
 
 // Map of [T][heads][128] bf16 rows: one box = 64 columns x 1 head x 64 tokens, SWIZZLE_128B.
 bool map_bf16_rows(CUtensorMap* m, const void* base, int heads, int T);
+// Map of rows of 128 bytes: one box = 16 rows, SWIZZLE_128B.
+bool map_u8_rows(CUtensorMap* m, const void* base, uint64_t rows);
 bool build_prefill_maps(const PrefillArgs& p, PrefillMaps* m);
 
 // Workspace element offset of column group cg (8 state columns) of chunk slot `slot`, v-head hv,
