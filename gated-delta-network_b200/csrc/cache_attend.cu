@@ -544,8 +544,8 @@ template <bool kInt8, int NT>
 static int launch_attend(const CacheAttendArgs& p, cudaStream_t stream) {
     constexpr int kRows = 8 * NT, kSmem = att::Smem<NT>::kSize;
     const unsigned ctas = NT < 4 ? kAttendCtas : kAttendCtas / 2;  // what fits on the SMs together
-    if (cudaFuncSetAttribute(gdn_cache_attend_kernel<kInt8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
-        return -1;
+    static SmemLimit limit;
+    if (!limit.raise(gdn_cache_attend_kernel<kInt8, NT>, kSmem)) return -1;
     AttendMaps maps{};
     if (p.c.max_pages > 0) {
         const uint64_t rows = ((uint64_t)p.c.pages * p.c.Hkv) << p.c.page_shift;

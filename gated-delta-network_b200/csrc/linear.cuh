@@ -97,6 +97,20 @@ struct CacheAttendArgs {
 constexpr int kAttendCtas = 296;  // 2 per SM with tiles of up to 16 rows; half as many with tiles of 32
 int attend_tiles(int rows);
 
+// Raise a kernel's shared-memory limit, once per device and kernel: `done` is that kernel's.  (Two threads may both set
+// it; they set the same.)
+struct SmemLimit {
+    bool done[64] = {};
+    template <typename K>
+    bool raise(K* kernel, int bytes) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+        if (done[dev]) return true;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+        return done[dev] = true;
+    }
+};
+
 int launch_cache_append(const CacheAppendArgs& p, cudaStream_t stream);
 int launch_cache_attend(const CacheAttendArgs& p, cudaStream_t stream);
 int launch_linear_decode(const LinearDecodeArgs& p, cudaStream_t stream);

@@ -973,9 +973,8 @@ int launch_linear_prefill(const LinearPrefillArgs& p, cudaStream_t stream) {
     if (p.T > 0 && !(map_bf16_rows(&maps.q, p.q, p.H, p.T) && map_bf16_rows(&maps.k, p.k, p.H, p.T) &&
                      map_bf16_rows(&maps.v, p.v, p.HV, p.T) && map_bf16_rows(&maps.o, p.out, p.HV, p.T)))
         return -3;
-    if (cudaFuncSetAttribute(gdn_linear_prefill_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
-        cudaFuncSetAttribute(gdn_linear_prefill_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
-        return -1;
+    static SmemLimit out, seg;
+    if (!out.raise(gdn_linear_prefill_kernel<true>, kSmem) || !seg.raise(gdn_linear_prefill_kernel<false>, kSmem)) return -1;
     const dim3 grid((unsigned)p.ctas);
     if (p.cut) {
         if (launch_pdl(gdn_linear_prefill_kernel<false>, grid, dim3(kThreads), kSmem, stream, p, maps) != cudaSuccess) return -1;

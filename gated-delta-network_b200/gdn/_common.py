@@ -77,6 +77,17 @@ def on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
+_get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def call(device: torch.device, fn, *args) -> int:
+    """fn(*args) with `device` current; no context object when it already is."""
+    if _get_device() == device.index:
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
+
+
 def out_ok(t, device: torch.device, dtype: torch.dtype, numel: int) -> bool:
     return (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == device.index and t.dtype is dtype
             and t.is_contiguous() and t.numel() == numel)
@@ -86,13 +97,13 @@ def decay_rows(log_decay, rows: int, HV: int, device: torch.device):
     """(fp32 log decays on `device`, 1 if they hold a row for each token else 0): [HV] or [rows, (1,) HV]."""
     if not isinstance(log_decay, torch.Tensor):
         raise TypeError("log_decay must be a torch.Tensor")
-    shape = tuple(log_decay.shape)
-    if shape == (HV,):
+    shape = log_decay.shape
+    if len(shape) == 1 and shape[0] == HV:
         per_token = 0
     elif len(shape) in (2, 3) and shape[0] == rows and shape[-1] == HV and log_decay.numel() == rows * HV:
         per_token = 1
     else:
-        raise ValueError(f"log_decay must hold [{HV}] or [{rows}, {HV}] values (got {shape})")
+        raise ValueError(f"log_decay must hold [{HV}] or [{rows}, {HV}] values (got {tuple(shape)})")
     return as_dev(log_decay, torch.float32, device), per_token
 
 
@@ -123,20 +134,23 @@ PAGE_SIZES = (16, 32, 64, 128)
 
 def cache_tensors(k_cache, v_cache, k_scale, v_scale, device: torch.device):
     """Checks of a paged 8-bit cache, which is used in place; returns (code, pages, Hkv, page size)."""
+    shape, dtype = k_cache.shape, k_cache.dtype
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != device.index or t.dtype not in CODES
-                or t.dim() != 4 or t.shape[3] != HEAD_DIM or not t.is_contiguous() or t.data_ptr() % 16):
+                or t.dim() != 4 or t.shape[3] != HEAD_DIM or not t.is_contiguous() or t.data_ptr() & 15):
             raise ValueError(f"{name} must be a contiguous, 16-byte aligned int8 or float8_e4m3fn CUDA tensor "
                              f"[pages, heads, page_size, {HEAD_DIM}]")
-    if k_cache.shape != v_cache.shape or k_cache.dtype is not v_cache.dtype:
+    if v_cache.shape != shape or v_cache.dtype is not dtype:
         raise ValueError("k_cache and v_cache must have the same shape and type")
-    pages, Hkv, P, _ = k_cache.shape
+    pages, Hkv, P, _ = shape
     if P not in PAGE_SIZES:
         raise ValueError(f"page size must be one of {PAGE_SIZES} (got {P})")
+    want = shape[:2]
     for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if not out_ok(t, device, torch.float32, pages * Hkv) or tuple(t.shape) != (pages, Hkv):
+        if (not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or not t.is_cuda
+                or t.get_device() != device.index or t.shape != want or not t.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous fp32 CUDA tensor [{pages}, {Hkv}]")
-    return CODES[k_cache.dtype], pages, Hkv, P
+    return CODES[dtype], pages, Hkv, P
 
 
 def cache_rows(block_table, seq_lens, B: int, device: torch.device):
@@ -145,7 +159,7 @@ def cache_rows(block_table, seq_lens, B: int, device: torch.device):
         raise ValueError(f"block_table must be a tensor [{B}, max_pages]")
     if block_table.dtype not in (torch.int32, torch.int64):
         raise ValueError("block_table must be int32 or int64")
-    if not isinstance(seq_lens, torch.Tensor) or tuple(seq_lens.shape) != (B,):
+    if not isinstance(seq_lens, torch.Tensor) or seq_lens.dim() != 1 or seq_lens.shape[0] != B:
         raise ValueError(f"seq_lens must be a tensor [{B}]")
     if seq_lens.dtype not in (torch.int32, torch.int64):
         raise ValueError("seq_lens must be int32 or int64")

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._common import HEAD_DIM, as_dev, cache_rows, cache_tensors, cu_on_device, cuda_device, on_device, ptr, stream_handle
+from ._common import HEAD_DIM, as_dev, cache_rows, cache_tensors, call, cu_on_device, cuda_device, stream_handle
 
 
 def kernel(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens):
@@ -29,15 +29,15 @@ def kernel(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_s
     """
     dev = cuda_device(k, "k")
     code, pages, Hkv, P = cache_tensors(k_cache, v_cache, k_scale, v_scale, dev)
-    if k.dim() != 3 or tuple(k.shape[1:]) != (Hkv, HEAD_DIM) or not isinstance(v, torch.Tensor) or v.shape != k.shape:
+    ks = k.shape
+    if len(ks) != 3 or ks[1] != Hkv or ks[2] != HEAD_DIM or not isinstance(v, torch.Tensor) or v.shape != ks:
         raise ValueError(f"k and v must be [T, {Hkv}, {HEAD_DIM}] tensors of one shape")
     cu, cu64, B = cu_on_device(cu_seqlens, dev)
     table, lens, len64, max_pages = cache_rows(block_table, seq_lens, B, dev)
     k_ = as_dev(k, torch.bfloat16, dev)
     v_ = as_dev(v, torch.bfloat16, dev)
-    lib = _lib.load()
-    with on_device(dev):
-        rc = lib.gdn_cache_append(ptr(k_), ptr(v_), ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), code,
-                                  ptr(table), ptr(lens), len64, ptr(cu), cu64, pages, P, max_pages, B, k.shape[0], Hkv,
-                                  HEAD_DIM, stream_handle(dev), 0)
-    _lib.check("gdn_cache_append", rc)
+    rc = call(dev, _lib.load().gdn_cache_append, k_.data_ptr(), v_.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+              k_scale.data_ptr(), v_scale.data_ptr(), code, table.data_ptr(), lens.data_ptr(), len64, cu.data_ptr(), cu64,
+              pages, P, max_pages, B, k.shape[0], Hkv, HEAD_DIM, stream_handle(dev), 0)
+    if rc:
+        _lib.check("gdn_cache_append", rc)

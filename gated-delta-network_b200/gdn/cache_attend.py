@@ -11,38 +11,54 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._common import (HEAD_DIM, as_dev, cache_rows, cache_tensors, cuda_device, on_device, out_ok, ptr, resolve_scale,
+from ._common import (HEAD_DIM, as_dev, cache_rows, cache_tensors, call, cuda_device, out_ok, resolve_scale,
                       stream_handle, workspace_for)
 from .prefill import read_status  # noqa: F401  (the status word is the workspace's first int here too)
 
 
+_need = 0  # the library's answer, which does not change
+
+
 def workspace_bytes() -> int:
-    return int(_lib.load().gdn_cache_attend_workspace_bytes())
+    global _need
+    if not _need:
+        _need = int(_lib.load().gdn_cache_attend_workspace_bytes())
+    return _need
+
+
+def _launch(dev, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, output, workspace):
+    """`output` None: allocated here and returned."""
+    code, pages, Hkv, P = cache_tensors(k_cache, v_cache, k_scale, v_scale, dev)
+    qs = q.shape
+    if len(qs) != 4 or qs[3] != HEAD_DIM:
+        raise ValueError(f"q must be [B, Q, Hq, {HEAD_DIM}] (got {tuple(qs)})")
+    B, Q, Hq, _ = qs
+    if Hkv < 1 or Hq < Hkv or Hq % Hkv:
+        raise ValueError(f"q heads must be a multiple of the cache's heads (got {Hq} and {Hkv})")
+    table, lens, len64, max_pages = cache_rows(block_table, seq_lens, B, dev)
+    s = scale if type(scale) is float and scale != 0.0 else resolve_scale(scale)
+    q_ = as_dev(q, torch.bfloat16, dev)
+    if output is None:
+        output = torch.empty(qs, dtype=torch.bfloat16, device=dev)
+    elif not out_ok(output, dev, torch.bfloat16, q.numel()) or output.data_ptr() % 16:
+        raise ValueError(f"output must be a contiguous, 16-byte aligned bf16 CUDA tensor with {q.numel()} elements")
+    lib = _lib.load()
+    need = _need or workspace_bytes()
+    ws = workspace_for(workspace, need, dev)
+    rc = call(dev, lib.gdn_cache_attend, q_.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+              v_scale.data_ptr(), code, table.data_ptr(), lens.data_ptr(), len64, pages, P, max_pages, B, Q, Hq, Hkv, HEAD_DIM,
+              s, output.data_ptr(), ws.data_ptr(), need, stream_handle(dev), 0)
+    if rc:
+        _lib.check("gdn_cache_attend", rc)
+    return output
 
 
 def kernel(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, output, *, workspace=None):
     """Destination-passing form of ``run``: writes ``output`` [B, Q, Hq, 128] bf16.  ``workspace``: a CUDA buffer of
     at least ``workspace_bytes()`` bytes, 256-byte aligned, for callers that keep one."""
-    dev = cuda_device(q, "q")
-    code, pages, Hkv, P = cache_tensors(k_cache, v_cache, k_scale, v_scale, dev)
-    if q.dim() != 4 or q.shape[3] != HEAD_DIM:
-        raise ValueError(f"q must be [B, Q, Hq, {HEAD_DIM}] (got {tuple(q.shape)})")
-    B, Q, Hq, _ = q.shape
-    if Hkv < 1 or Hq < Hkv or Hq % Hkv:
-        raise ValueError(f"q heads must be a multiple of the cache's heads (got {Hq} and {Hkv})")
-    table, lens, len64, max_pages = cache_rows(block_table, seq_lens, B, dev)
-    s = resolve_scale(scale)
-    q_ = as_dev(q, torch.bfloat16, dev)
-    if not out_ok(output, dev, torch.bfloat16, q.numel()) or output.data_ptr() % 16:
-        raise ValueError(f"output must be a contiguous, 16-byte aligned bf16 CUDA tensor with {q.numel()} elements")
-    lib = _lib.load()
-    need = workspace_bytes()
-    ws = workspace_for(workspace, need, dev)
-    with on_device(dev):
-        rc = lib.gdn_cache_attend(ptr(q_), ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), code, ptr(table),
-                                  ptr(lens), len64, pages, P, max_pages, B, Q, Hq, Hkv, HEAD_DIM, s, ptr(output),
-                                  ptr(ws), need, stream_handle(dev), 0)
-    _lib.check("gdn_cache_attend", rc)
+    if output is None:
+        raise ValueError("output must be given")
+    _launch(cuda_device(q, "q"), q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, output, workspace)
 
 
 def run(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale):
@@ -54,7 +70,4 @@ def run(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale):
     the Q tokens included.  Row i sees the positions below seq_len - Q + 1 + i; a row that sees none (a padded row
     with seq_lens 0, say) is zero.  scale float, 0-d tensor, or None/0 (1/sqrt(128)).
     """
-    dev = cuda_device(q, "q")
-    output = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
-    kernel(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, output)
-    return output
+    return _launch(cuda_device(q, "q"), q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, None, None)

@@ -10,8 +10,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._common import (HEAD_DIM, NUM_QK_HEADS, NUM_V_HEADS, as_dev, check_heads, cu_on_device, cuda_device, decay_rows,
-                      on_device, out_ok, ptr, resolve_scale, stream_handle, workspace_for)
+from ._common import (HEAD_DIM, NUM_QK_HEADS, NUM_V_HEADS, as_dev, call, check_heads, cu_on_device, cuda_device,
+                      decay_rows, out_ok, ptr, resolve_scale, stream_handle, workspace_for)
 from .prefill import read_status  # noqa: F401  (the status word is the workspace's first int here too)
 
 
@@ -21,37 +21,42 @@ def workspace_bytes(num_seqs: int, total_tokens: int, num_qk_heads: int = NUM_QK
                                                               int(num_v_heads), HEAD_DIM, HEAD_DIM))
 
 
-def _launch(q, k, v, state, log_decay, cu_seqlens, scale, output, new_state, workspace=None, flags=0):
-    dev = cuda_device(q, "q")
-    if q.dim() != 3 or v.dim() != 3 or k.shape != q.shape or v.shape[0] != q.shape[0]:
-        raise ValueError(f"q, k must be [T, H, 128] and v [T, HV, 128] (got {tuple(q.shape)}, {tuple(k.shape)}, "
-                         f"{tuple(v.shape)})")
-    T, H, K = q.shape
-    HV, V = v.shape[1], v.shape[2]
-    check_heads(H, k.shape[1], HV, K, V, prefill=True)
+def _launch(dev, q, k, v, state, log_decay, cu_seqlens, scale, output, new_state, workspace, flags):
+    """`output` / `new_state` None: allocated here and returned."""
+    qs, vs = q.shape, v.shape
+    if len(qs) != 3 or len(vs) != 3 or k.shape != qs or vs[0] != qs[0]:
+        raise ValueError(f"q, k must be [T, H, 128] and v [T, HV, 128] (got {tuple(qs)}, {tuple(k.shape)}, {tuple(vs)})")
+    T, H, K = qs
+    HV, V = vs[1], vs[2]
+    check_heads(H, H, HV, K, V, prefill=True)
     cu, cu64, N = cu_on_device(cu_seqlens, dev)
-    s = resolve_scale(scale)
+    s = scale if type(scale) is float and scale != 0.0 else resolve_scale(scale)
     q_ = as_dev(q, torch.bfloat16, dev)
     k_ = as_dev(k, torch.bfloat16, dev)
     v_ = as_dev(v, torch.bfloat16, dev)
     d_, per_token = decay_rows(log_decay, T, HV, dev)
     st = None
     if state is not None:
-        if tuple(state.shape) != (N, HV, V, K):
+        if state.shape != (N, HV, V, K):
             raise ValueError(f"state must be [N, {HV}, 128, 128], got {tuple(state.shape)}")
         st = as_dev(state, torch.float32, dev)
-    if not out_ok(output, dev, torch.bfloat16, T * HV * V) or output.data_ptr() % 16:
-        raise ValueError(f"output must be a contiguous, 16-byte aligned bf16 CUDA tensor with {T * HV * V} elements")
-    if not out_ok(new_state, dev, torch.float32, N * HV * V * K) or new_state.data_ptr() % 16:
-        raise ValueError(f"new_state must be a contiguous, 16-byte aligned fp32 CUDA tensor with {N * HV * V * K} elements")
+    if output is None:
+        output = torch.empty(vs, dtype=torch.bfloat16, device=dev)
+        new_state = torch.empty((N, HV, V, K), dtype=torch.float32, device=dev)
+    else:
+        if not out_ok(output, dev, torch.bfloat16, T * HV * V) or output.data_ptr() % 16:
+            raise ValueError(f"output must be a contiguous, 16-byte aligned bf16 CUDA tensor with {T * HV * V} elements")
+        if not out_ok(new_state, dev, torch.float32, N * HV * V * K) or new_state.data_ptr() % 16:
+            raise ValueError(f"new_state must be a contiguous, 16-byte aligned fp32 CUDA tensor with {N * HV * V * K} elements")
     lib = _lib.load()
-    need = workspace_bytes(N, T, H, HV)
+    need = lib.gdn_linear_prefill_workspace_bytes(N, T, H, HV, K, V)
     ws = workspace_for(workspace, need, dev)
-    with on_device(dev):
-        rc = lib.gdn_linear_prefill_fwd(ptr(q_), ptr(k_), ptr(v_), ptr(st), ptr(d_), per_token, ptr(cu), cu64, N, T, s,
-                                        ptr(output), ptr(new_state), ptr(ws), need, H, HV, K, V, stream_handle(dev),
-                                        flags)
-    _lib.check("gdn_linear_prefill_fwd", rc)
+    rc = call(dev, lib.gdn_linear_prefill_fwd, q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), ptr(st), d_.data_ptr(), per_token,
+              cu.data_ptr(), cu64, N, T, s, output.data_ptr(), new_state.data_ptr(), ws.data_ptr(), need, H, HV, K, V,
+              stream_handle(dev), flags)
+    if rc:
+        _lib.check("gdn_linear_prefill_fwd", rc)
+    return output, new_state
 
 
 def run(q, k, v, state, log_decay, cu_seqlens, scale):
@@ -63,18 +68,14 @@ def run(q, k, v, state, log_decay, cu_seqlens, scale):
     int32/int64; scale float, 0-d tensor, or None/0 (1/sqrt(128)).  A zero-length sequence keeps its state;
     tokens outside every sequence get a zero output.
     """
-    dev = cuda_device(q, "q")
-    if v.dim() != 3:
-        raise ValueError(f"v must be [T, HV, 128] (got {tuple(v.shape)})")
-    T, HV, N = q.shape[0], v.shape[1], cu_seqlens.shape[0] - 1
-    output = torch.empty((T, HV, HEAD_DIM), dtype=torch.bfloat16, device=dev)
-    new_state = torch.empty((max(N, 0), HV, HEAD_DIM, HEAD_DIM), dtype=torch.float32, device=dev)
-    _launch(q, k, v, state, log_decay, cu_seqlens, scale, output, new_state, flags=_lib.GDN_FLAG_ZERO_UNOWNED)
-    return output, new_state
+    return _launch(cuda_device(q, "q"), q, k, v, state, log_decay, cu_seqlens, scale, None, None, None,
+                   _lib.GDN_FLAG_ZERO_UNOWNED)
 
 
 def kernel(q, k, v, state, log_decay, cu_seqlens, scale, output, new_state, *, workspace=None):
     """Destination-passing prefill: writes ``new_state`` (which may be ``state`` itself) and the rows of
     ``output`` that belong to a sequence; the others are left as they were.  ``workspace``: a CUDA buffer of at
     least ``workspace_bytes(N, T, H, HV)`` bytes, 256-byte aligned, for callers that keep one."""
-    _launch(q, k, v, state, log_decay, cu_seqlens, scale, output, new_state, workspace=workspace)
+    if output is None or new_state is None:
+        raise ValueError("output and new_state must be given")
+    _launch(cuda_device(q, "q"), q, k, v, state, log_decay, cu_seqlens, scale, output, new_state, workspace, 0)
