@@ -925,29 +925,41 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
 __global__ void __launch_bounds__(256) gdn_linear_chain_kernel(LinearPrefillArgs p) {
     pdl_wait();
     pdl_trigger();
-    const int4 kind = p.kind[blockIdx.x];
-    if (kind.x != 1) return;
-    // the stretches that the segment goes through from here: a run of 2s
+    // the stretches that the segment goes through from here: a run of 2s, of which the first 31 come with the 1
     const int lane = threadIdx.x & 31;
-    int end = blockIdx.x + 1;
-    while (true) {
-        const unsigned through = __ballot_sync(0xffffffffu, end + lane < p.ctas && p.kind[min(end + lane, p.ctas - 1)].x == 2);
-        end += __ffs(~through) ? __ffs(~through) - 1 : 32;
-        if (through != 0xffffffffu) break;
+    const int4 mine = p.kind[min((int)blockIdx.x + lane, p.ctas - 1)];
+    if (__shfl_sync(0xffffffffu, mine.x, 0) != 1) return;
+    const int n = __shfl_sync(0xffffffffu, mine.y, 0), hv = __shfl_sync(0xffffffffu, mine.z, 0);
+    unsigned stops = __ballot_sync(0xffffffffu, lane > 0 && ((int)blockIdx.x + lane >= p.ctas || mine.x != 2));
+    int end = blockIdx.x + 32;
+    while (!stops) {
+        stops = __ballot_sync(0xffffffffu, end + lane >= p.ctas || p.kind[min(end + lane, p.ctas - 1)].x != 2);
+        end += 32;
     }
+    end += __ffs(stops) - 1 - 32;
     const size_t el = blockIdx.y * 1024 + threadIdx.x * 4;
     float4 h = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (p.state) {
-        h = *reinterpret_cast<const float4*>(p.state + ((size_t)kind.y * p.HV + kind.z) * kD * kD + el);
-        *reinterpret_cast<float4*>(p.seg + (size_t)(p.ctas + blockIdx.x) * kD * kD + el) = h;
-    }
-#pragma unroll 8
-    for (int c = blockIdx.x; c < end; ++c) {
-        const float gm = p.gamma[c];
-        float4* d = reinterpret_cast<float4*>(p.seg + (size_t)c * kD * kD + el);
-        const float4 y = *d;
-        h = make_float4(fmaf(gm, h.x, y.x), fmaf(gm, h.y, y.y), fmaf(gm, h.z, y.z), fmaf(gm, h.w, y.w));
-        *d = h;
+    if (p.state) h = *reinterpret_cast<const float4*>(p.state + ((size_t)n * p.HV + hv) * kD * kD + el);
+    // twelve stretches at a time: their loads do not wait for one another, nor for the stores before them
+    constexpr int kBatch = 12;
+#pragma unroll 1
+    for (int c = blockIdx.x; c < end; c += kBatch) {
+        float4 y[kBatch];
+        float gm[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int k = min(c + i, end - 1);
+            y[i] = __ldcg(reinterpret_cast<const float4*>(p.seg + (size_t)k * kD * kD + el));
+            gm[i] = __ldcg(p.gamma + k);
+        }
+        if (c == (int)blockIdx.x && p.state) *reinterpret_cast<float4*>(p.seg + (size_t)(p.ctas + c) * kD * kD + el) = h;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (c + i < end) {
+                h = make_float4(fmaf(gm[i], h.x, y[i].x), fmaf(gm[i], h.y, y[i].y), fmaf(gm[i], h.z, y[i].z), fmaf(gm[i], h.w, y[i].w));
+                *reinterpret_cast<float4*>(p.seg + (size_t)(c + i) * kD * kD + el) = h;
+            }
+        }
     }
 }
 
