@@ -586,24 +586,25 @@ __device__ __forceinline__ bool role_v(const LinearPrefillArgs& p, const LinCtx&
                 fence_async_smem();
                 named_bar_sync(1, 256);
             }
-            if (g > 0) LIN_WAIT(lin_bars()->u_full, g - 1);  // the parts of the chunk before are consumed
-            tc_fence_after();
-#pragma unroll 1
+            uint32_t part[3][16];
+#pragma unroll
             for (int i = 0; i < 4; ++i) {  // 16 V x 16 tokens, transposed
-                uint32_t raw[4], part[3][4];
+                uint32_t raw[4];
                 ldsm_x4_t(raw[0], raw[1], raw[2], raw[3], st + from + 2048 * i);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {  // {0, 1}: tokens 16 i + .., {2, 3}: 8 later; odd ones are 8 V further
                     float2 y = mul2(bf2_to_f2(raw[j]), *reinterpret_cast<const float2*>(er + 16 * i + 8 * (j >> 1)));
 #pragma unroll
                     for (int k = 0; k < 3; ++k) {
-                        part[k][j] = pack_bf16x2(y.x, y.y);
-                        if (k < 2) y = sub2(y, bf2_to_f2(part[k][j]));
+                        part[k][4 * i + j] = pack_bf16x2(y.x, y.y);
+                        if (k < 2) y = sub2(y, bf2_to_f2(part[k][4 * i + j]));
                     }
                 }
-#pragma unroll
-                for (int k = 0; k < 3; ++k) tmem_st_16x128b_x2(tl + 32 * k + 8 * i, part[k]);
             }
+            if (g > 0) LIN_WAIT(lin_bars()->u_full, g - 1);  // the parts of the chunk before are consumed
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < 3; ++k) tmem_st_16x128b_x8(tl + 32 * k, part[k]);
             tmem_st_wait();
             tc_fence_before();
             mbar_arrive(&lin_bars()->u_ready);
