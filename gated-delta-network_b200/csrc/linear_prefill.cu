@@ -40,7 +40,7 @@ constexpr uint32_t kStage = 49152;
 constexpr uint32_t kOffP = kStages * kStage;     // P [2][64 i][64 j] bf16
 constexpr uint32_t kOffO = kOffP + 2 * 8192;     // output staging [2][2 atoms][64 tokens][64 V] bf16, SWIZZLE_128B
 constexpr uint32_t kOffG = kOffO + 2 * 16384;    // gates, kGates slots of f32: [64] G | [64] factors of OI | [64] of v | [64] e^{G_b - G}, b the
-                                                 // last of the token's block of 16 | state: factor, unit at the end, decay, whether to multiply
+                                                 // last of the token's block of 16 | state: factor, unit at the end, log of the decay, whether to multiply
 constexpr uint32_t kGateFloats = 264;
 constexpr uint32_t kOffBar = kOffG + kGates * kGateFloats * 4;
 constexpr uint32_t kOffRange = kOffBar + 512;
@@ -388,11 +388,11 @@ __device__ __forceinline__ bool role_gates(const LinearPrefillArgs& p, const Lin
             *reinterpret_cast<float2*>(gt + 128 + 2 * lane) =
                 scale ? make_float2(lin_ex2(after + a1), lin_ex2(after)) : make_float2(lin_ex2(-(g0 + X)), lin_ex2(-(pre + X)));
             *reinterpret_cast<float2*>(gt + 192 + 2 * lane) = make_float2(lin_ex2(gb - g0), lin_ex2(gb - pre));
-            if (lane == 0) gt[256] = scale ? lin_ex2(X + total) : 1.f;  // what the state is multiplied by
+            if (lane == 0) gt[256] = scale ? exp2f(X + total) : 1.f;  // what the state is multiplied by
             X = scale ? 0.f : X + total;
             if (lane == 0) {
-                gt[257] = lin_ex2(X);      // of the state at the chunk's end
-                gt[258] = lin_ex2(total);  // the chunk's decay
+                gt[257] = exp2f(X);        // of the state at the chunk's end
+                gt[258] = total;           // the chunk's decay, as its logarithm
                 gt[259] = scale ? 1.f : 0.f;
             }
             __syncwarp();
@@ -725,14 +725,14 @@ __device__ __forceinline__ bool role_s(const LinearPrefillArgs& p, const LinCtx&
                 reinterpret_cast<float4*>(dst)[j] = src ? reinterpret_cast<const float4*>(src)[j] : make_float4(0.f, 0.f, 0.f, 0.f);
             continue;
         }
-        float gamma = 1.f, unit = 1.f;
+        float gamma = 0.f, unit = 1.f;  // gamma: logarithm of the piece's decay, so that its rounding is not a product's
 #pragma unroll 1
         for (int c = pc.ca; c < pc.cb; ++c, ++g) {
             const float* gt = lin_gates(g);
             LIN_WAIT(lin_bars()->g_full[g % kGates], g / kGates);
             const float factor = gt[256];
             unit = gt[257];
-            gamma *= gt[258];
+            gamma += gt[258];
             const bool begins = c == pc.ca, write = gt[259] != 0.f;
             if (g > 0) {
                 // the state is complete (or, at a segment's start, was read) and OI has read its copy
@@ -817,7 +817,7 @@ __device__ __forceinline__ bool role_s(const LinearPrefillArgs& p, const LinCtx&
                     *reinterpret_cast<float2*>(row + 8 * (j >> 1) + 8 * kD * (j & 1)) =
                         make_float2(unit * __uint_as_float(d[2 * j]), unit * __uint_as_float(d[2 * j + 1]));
             }
-            if (!kOut && r == 0) p.gamma[blockIdx.x] = gamma;
+            if (!kOut && r == 0) p.gamma[blockIdx.x] = exp2f(gamma);
         }
     }
     return true;
@@ -967,7 +967,7 @@ __global__ void __launch_bounds__(256) gdn_linear_chain_kernel(LinearPrefillArgs
 LinearPrefillLayout linear_prefill_layout(int N, int T, int HV) {
     LinearPrefillLayout L{};
     const long long share = ((long long)T / lin::C + 3ll * N) * HV / kLinearCtas;  // places of a CTA
-    L.keep = (int)std::max<long long>(8, std::min<long long>(3 * share / 10, 1 << 20));
+    L.keep = (int)std::min<long long>(16 + share / 2, 1 << 20);
     L.cut = T > (long long)lin::C * L.keep ? 1 : 0;
     L.min_share = L.cut ? 4 : 1;
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
