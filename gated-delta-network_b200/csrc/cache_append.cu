@@ -7,9 +7,9 @@
 // max |x| is over finite values; infinities become the largest code, a NaN the code NaN (e4m3) or 0 (int8).
 //
 // Bound by HBM for prompts (768 bytes a token and head, each row read and written once) and by latency for decode steps.
-// Prompts: one CTA per (page a sequence touches, head, key or value), its rows in registers between the maximum and the
-// encoding.  Steps of a few tokens: one warp each instead, eight of them a CTA, so that the search for the sequence and
-// the loads it leads to are in flight together.
+// A warp holds its rows of a (page a sequence touches, head, key or value) in registers between the maximum and the
+// encoding.  What a CTA waits for in turn (the lengths, the rows and the table, the page's scale) sets the rate, so many
+// bytes have to be in flight: 16 rows a warp, 128 bytes a thread.
 // The quotients would cost more than the traffic: a code is taken from x (1 / s), and from the quotient where the two
 // could round to different codes.
 #include <cuda_fp16.h>
@@ -19,25 +19,34 @@
 
 namespace gdn {
 
+struct Sequence {
+    int b, t0, t1, len;  // its new tokens, its length behind them
+};
 // The sequence whose touched pages hold slot u: the last one with cu[b] / P + 2 b <= u.  n tokens touch at most
 // floor(n / P) + 2 pages, so these bases need no prefix sum.  32 probes a round, all lanes of every warp together.
-__device__ __forceinline__ int find_sequence(const CacheAppendArgs& p, int u) {
+__device__ __forceinline__ Sequence find_sequence(const CacheAppendArgs& p, int u) {
     int lo = 0, n = p.c.B;  // candidates lo .. lo + n - 1; lo always qualifies
     const int lane = threadIdx.x & 31;
-    while (n > 1) {
+    while (true) {
         const int step = (n + 31) / 32, at = lo + lane * step;
-        bool yes = false;
-        if (lane * step < n) {
-            int s, e;
-            seq_bounds(p.cu, p.cu64, at, p.T, s, e);
-            yes = (s >> p.c.page_shift) + 2 * at <= u;
+        const bool any = lane * step < n;
+        Sequence x{at, 0, 0, 0};
+        if (any) {
+            seq_bounds(p.cu, p.cu64, at, p.T, x.t0, x.t1);
+            x.len = cache_length(p.c, at);
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, yes);
+        const unsigned hit = __ballot_sync(0xffffffffu, any && (x.t0 >> p.c.page_shift) + 2 * at <= u);
         const int last = hit ? 31 - __clz(hit) : 0;
+        if (step == 1) {
+            x.b = lo + last;
+            x.t0 = __shfl_sync(0xffffffffu, x.t0, last);
+            x.t1 = __shfl_sync(0xffffffffu, x.t1, last);
+            x.len = __shfl_sync(0xffffffffu, x.len, last);
+            return x;
+        }
         n = min(step, n - last * step);
         lo += last * step;
     }
-    return lo;
 }
 
 // Largest magnitude of 8 bf16 values so far, per half; NaN does not count, infinity is dealt with by finite_max.
@@ -74,30 +83,29 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(y) : "f"(d), "f"(c));
     return (uint32_t)x | ((uint32_t)y << 16);
 }
-// Eight bf16 values to codes of scale s; r = 1 / s rounded, or 0 to have every code from its quotient.
+// Eight bf16 values to codes, by r = 1 / s rounded; false where a quotient might have another code.
 template <bool kInt8>
-__device__ __forceinline__ uint2 encode8(uint4 w, float s, float r) {
+__device__ __forceinline__ bool encode8(uint4 w, float r, uint2& codes) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    bool odd = r == 0.f;  // every code from its quotient
-    if (kInt8) {          // infinity or NaN among them
+    bool differ = false;
+    if (kInt8) {  // infinity or NaN among them
         __nv_bfloat162 top = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u[0]));
 #pragma unroll
         for (int e = 1; e < 4; ++e) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u[e])));
         const uint32_t bits = *reinterpret_cast<const uint32_t*>(&top);
-        odd |= (bits & 0x7f80u) == 0x7f80u || (bits & 0x7f800000u) == 0x7f800000u;
+        differ = (bits & 0x7f80u) == 0x7f80u || (bits & 0x7f800000u) == 0x7f800000u;
     }
     uint32_t o[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const float2 x = make_float2(__uint_as_float(u[2 * e] << 16), __uint_as_float(u[2 * e] & 0xffff0000u));
         const float2 y = make_float2(__uint_as_float(u[2 * e + 1] << 16), __uint_as_float(u[2 * e + 1] & 0xffff0000u));
-        bool differ;
         if (kInt8) {
             // x (1 / s) is within 127 2^-22 < 2^-15 of x / s: another code only where it is that near to a half
             const float2 r2 = make_float2(r, r), big = make_float2(12582912.f, 12582912.f);  // + 1.5 2^23: the rounded integer in the low bits
             const float2 qx = mul2(x, r2), qy = mul2(y, r2), nx = add2(qx, big), ny = add2(qy, big);
             const float2 dx = sub2(qx, sub2(nx, big)), dy = sub2(qy, sub2(ny, big));
-            differ = fmaxf(fmaxf(fabsf(dx.x), fabsf(dx.y)), fmaxf(fabsf(dy.x), fabsf(dy.y))) > 0.5f - 0x1p-14f;
+            differ |= fmaxf(fmaxf(fabsf(dx.x), fabsf(dx.y)), fmaxf(fabsf(dy.x), fabsf(dy.y))) > 0.5f - 0x1p-14f;
             o[e] = __byte_perm(__byte_perm(__float_as_uint(nx.x), __float_as_uint(nx.y), 0x0040),
                                __byte_perm(__float_as_uint(ny.x), __float_as_uint(ny.y), 0x0040), 0x5410);
         } else {
@@ -105,12 +113,20 @@ __device__ __forceinline__ uint2 encode8(uint4 w, float s, float r) {
             const float2 lo = make_float2(r * (1.f - 0x1p-21f), r * (1.f - 0x1p-21f)), hi = make_float2(r * (1.f + 0x1p-21f), r * (1.f + 0x1p-21f));
             const float2 a = mul2(x, lo), b = mul2(y, lo), c = mul2(x, hi), d = mul2(y, hi);
             o[e] = encode4<false, false>(a.x, a.y, b.x, b.y);
-            differ = o[e] != encode4<false, false>(c.x, c.y, d.x, d.y);
+            differ |= o[e] != encode4<false, false>(c.x, c.y, d.x, d.y);
         }
-        if (differ || odd)  // (s = 0: zeros, or values whose scale is below fp32)
-            o[e] = s > 0.f ? encode4<kInt8, true>(__fdiv_rn(x.x, s), __fdiv_rn(x.y, s), __fdiv_rn(y.x, s), __fdiv_rn(y.y, s)) : 0u;
     }
-    return make_uint2(o[0], o[1]);
+    codes = make_uint2(o[0], o[1]);
+    return !differ;
+}
+// The same from the quotients.  (s = 0: zeros, or values whose scale is below fp32.)
+template <bool kInt8>
+__device__ __forceinline__ uint2 encode8_exactly(uint4 w, float s) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __fdiv_rn(__uint_as_float(e & 1 ? u[e >> 1] & 0xffff0000u : u[e >> 1] << 16), s);
+    return s > 0.f ? make_uint2(encode4<kInt8, true>(x[0], x[1], x[2], x[3]), encode4<kInt8, true>(x[4], x[5], x[6], x[7])) : make_uint2(0, 0);
 }
 template <bool kInt8>
 __device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
@@ -148,137 +164,140 @@ __device__ __forceinline__ float reciprocal(float s) { return s > 0x1p-100f && s
 
 // What one page of one sequence gets from the call.
 struct AppendPage {
-    int page, rows, held;  // page < 0: nothing; new rows, and older tokens in front of them
+    int page, rows, held;  // the page's number as the table has it; new rows, and older tokens in front of them
     size_t token;          // first new row in k and v
 };
 __device__ __forceinline__ AppendPage find_page(const CacheAppendArgs& p, int unit) {
     const CacheArgs& c = p.c;
     AppendPage r{-1, 0, 0, 0};
-    const int b = find_sequence(p, unit);
-    int t0, t1;
-    seq_bounds(p.cu, p.cu64, b, p.T, t0, t1);
+    const Sequence q = find_sequence(p, unit);
     // positions of the new tokens; those outside [0, max_pages P) are dropped
-    const int end = cache_length(c, b), start = end - (t1 - t0);
-    const int i = unit - ((t0 >> c.page_shift) + 2 * b) + (max(start, 0) >> c.page_shift);  // page of the sequence
+    const int start = q.len - (q.t1 - q.t0);
+    const int i = unit - ((q.t0 >> c.page_shift) + 2 * q.b) + (max(start, 0) >> c.page_shift);  // page of the sequence
     if (i < 0 || i >= c.max_pages) return r;
-    const int lo = max(max(start, 0), i << c.page_shift), hi = min(end, (i + 1) << c.page_shift);
+    const int lo = max(max(start, 0), i << c.page_shift), hi = min(q.len, (i + 1) << c.page_shift);
     if (lo >= hi) return r;
-    const int page = c.table[(size_t)b * c.max_pages + i];
-    if ((unsigned)page >= (unsigned)c.pages) return r;  // no such page: the rows are dropped
-    r.page = page;
+    r.page = c.table[(size_t)q.b * c.max_pages + i];
     r.rows = hi - lo;
     r.held = lo - (i << c.page_shift);
-    r.token = (size_t)(t0 + lo - start);
+    r.token = (size_t)(q.t0 + lo - start);
     return r;
 }
 
-// R: passes of 16 rows that cover a page.
-template <bool kInt8, int R>
-__global__ void __launch_bounds__(256, R <= 4 ? 5 : 3) gdn_cache_append_kernel(CacheAppendArgs p) {
+// W warps for each (page, head, key or value), 8 / W of these a CTA; a warp takes 2 L new rows, two a load (W = 1: that
+// many at a time).
+template <bool kInt8, int W, int L>
+__global__ void __launch_bounds__(256, L == 8 ? 4 : 5) gdn_cache_append_kernel(CacheAppendArgs p) {
     __shared__ float s_max[8];
     pdl_wait();
     pdl_trigger();
     const CacheArgs& c = p.c;
-    const int tid = threadIdx.x, head = blockIdx.y, row = tid >> 4;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % W;
+    const int pair = blockIdx.y * (8 / W) + warp / W, head = pair >> 1;
     const AppendPage g = find_page(p, blockIdx.x);
-    if (g.page < 0) return;
-    const uint16_t* x = (blockIdx.z ? p.v : p.k) + (g.token * c.Hkv + head) * kD + 8 * (tid & 15);
-    uint8_t* codes = static_cast<uint8_t*>(blockIdx.z ? c.v_cache : c.k_cache) + (((size_t)g.page * c.Hkv + head) << c.page_shift) * kD;
-    float* scale = (blockIdx.z ? c.v_scale : c.k_scale) + (size_t)g.page * c.Hkv + head;
+    if (g.rows == 0) return;  // (the whole CTA, and below)
+    const bool here = head < c.Hkv;
+    const int rows = here ? g.rows : 0, row = lane >> 4;
+    const uint16_t* x = (pair & 1 ? p.v : p.k) + (g.token * c.Hkv + head) * kD + 8 * (lane & 15);
+    auto load = [&](int r) { return __ldg(reinterpret_cast<const uint4*>(x + (size_t)r * c.Hkv * kD)); };
 
-    uint4 w[R];
+    uint4 w[L];
+    auto load_block = [&](int r0) {
+        const uint16_t* at = x + (size_t)(r0 + row) * c.Hkv * kD;
+        const int left = rows - r0 - row;
+#pragma unroll
+        for (int i = 0; i < L; ++i, at += 2 * c.Hkv * kD)
+            w[i] = 2 * i < left ? __ldg(reinterpret_cast<const uint4*>(at)) : make_uint4(0, 0, 0, 0);
+    };
+    int r0 = 2 * L * part;  // W = 1: the last block afterwards
+    load_block(r0);  // with the table's entry still on its way
+    if ((unsigned)g.page >= (unsigned)c.pages) return;  // no such page: the rows are dropped
+    uint8_t* codes = static_cast<uint8_t*>(pair & 1 ? c.v_cache : c.k_cache) + (((size_t)g.page * c.Hkv + head) << c.page_shift) * kD;
+    float* scale = (pair & 1 ? c.v_scale : c.k_scale) + (size_t)g.page * c.Hkv + head;
+    const float old = here && g.held > 0 ? *scale : 0.f;
     __nv_bfloat162 top2 = __float2bfloat162_rn(0.f);
+    while (true) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        w[r] = make_uint4(0, 0, 0, 0);
-        if (16 * r + row < g.rows) w[r] = __ldg(reinterpret_cast<const uint4*>(x + (size_t)(16 * r + row) * c.Hkv * kD));
+        for (int i = 0; i < L; ++i) top2 = abs_max(top2, w[i]);
+        if (W > 1 || r0 + 2 * L >= rows) break;
+        load_block(r0 += 2 * L);
     }
-    const float old = g.held > 0 ? *scale : 0.f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) top2 = abs_max(top2, w[r]);
     float top = fmaxf(__low2float(top2), __high2float(top2));
     if (top == INFINITY) {
         top = 0.f;
 #pragma unroll 1
-        for (int r = 0; r < R; ++r)
-            if (16 * r + row < g.rows) top = fmaxf(top, finite_max(__ldg(reinterpret_cast<const uint4*>(x + (size_t)(16 * r + row) * c.Hkv * kD))));
+        for (int r = 2 * L * part + row; r < min(rows, r0 + 2 * L); r += 2) top = fmaxf(top, finite_max(load(r)));
     }
 #pragma unroll
     for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    if ((tid & 31) == 0) s_max[tid >> 5] = top;
-    __syncthreads();
+    if (W > 1) {
+        if (lane == 0) s_max[warp] = top;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, s_max[w]);
+        for (int i = 0; i < W; ++i) top = fmaxf(top, s_max[warp - part + i]);
+    }
     const float s = fmaxf(old, __fdiv_rn(top, kInt8 ? 127.f : 448.f)), inv = reciprocal(s);
 
-    if (g.held > 0 && s > old)  // older tokens of the page to the new scale, 16 bytes a thread
-        for (int j = tid; j < g.held * 8; j += 256) recode16<kInt8>(reinterpret_cast<uint4*>(codes) + j, old, s);
+    codes += g.held * kD;
+    while (true) {
+        unsigned again = 0;  // rows to encode from their quotients
+        uint8_t* to = codes + (r0 + row) * kD + 8 * (lane & 15);
+        const int left = rows - r0 - row;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-        if (16 * r + row < g.rows)
-            *reinterpret_cast<uint2*>(codes + (size_t)(g.held + 16 * r + row) * kD + 8 * (tid & 15)) = encode8<kInt8>(w[r], s, inv);
-    if (tid == 0) *scale = s;
+        for (int i = 0; i < L; ++i) {
+            uint2 y;
+            if (2 * i < left) {
+                if (!encode8<kInt8>(w[i], inv, y) || inv == 0.f) again |= 1u << i;
+                *reinterpret_cast<uint2*>(to + 2 * i * kD) = y;
+            }
+        }
+#pragma unroll 1
+        while (again) {
+            const int i = __ffs(again) - 1;
+            again &= again - 1;
+            *reinterpret_cast<uint2*>(to + 2 * i * kD) = encode8_exactly<kInt8>(load(r0 + row + 2 * i), s);
+        }
+        if (W > 1 || r0 == 0) break;
+        load_block(r0 -= 2 * L);
+    }
+    codes -= g.held * kD;
+    if (here && g.held > 0 && s > old)  // older tokens of the page to the new scale, 16 bytes a thread
+#pragma unroll 1
+        for (int j = 32 * part + lane; j < g.held * 8; j += 32 * W) recode16<kInt8>(reinterpret_cast<uint4*>(codes) + j, old, s);
+    if (here && part == 0 && lane == 0) *scale = s;
 }
 
-// A warp per (page, head, key or value), two rows a pass; the rows are read again for their codes.
+template <bool kInt8, int W, int L>
+static cudaError_t launch_append(const CacheAppendArgs& p, unsigned units, cudaStream_t stream) {
+    return launch_pdl(gdn_cache_append_kernel<kInt8, W, L>, dim3(units, (unsigned)(2 * p.c.Hkv * W + 7) / 8), dim3(256), 0, stream, p);
+}
 template <bool kInt8>
-__global__ void __launch_bounds__(256) gdn_cache_append_few_kernel(CacheAppendArgs p) {
-    pdl_wait();
-    pdl_trigger();
-    const CacheArgs& c = p.c;
-    const int lane = threadIdx.x & 31, row = lane >> 4, pair = blockIdx.y * 8 + (threadIdx.x >> 5), head = pair >> 1;
-    if (head >= c.Hkv) return;
-    const AppendPage g = find_page(p, blockIdx.x);
-    if (g.page < 0) return;
-    const uint16_t* x = (pair & 1 ? p.v : p.k) + (g.token * c.Hkv + head) * kD + 8 * (lane & 15);
-    uint8_t* codes = static_cast<uint8_t*>(pair & 1 ? c.v_cache : c.k_cache) + (((size_t)g.page * c.Hkv + head) << c.page_shift) * kD;
-    float* scale = (pair & 1 ? c.v_scale : c.k_scale) + (size_t)g.page * c.Hkv + head;
-    const float old = g.held > 0 ? *scale : 0.f;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    float top = 0.f;
-#pragma unroll 1
-    for (int r = 0; r < g.rows; r += 2) {
-        w = make_uint4(0, 0, 0, 0);
-        if (r + row < g.rows) w = __ldg(reinterpret_cast<const uint4*>(x + (size_t)(r + row) * c.Hkv * kD));
-        top = fmaxf(top, finite_max(w));
-    }
-#pragma unroll
-    for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    const float s = fmaxf(old, __fdiv_rn(top, kInt8 ? 127.f : 448.f));
-    if (g.held > 0 && s > old)
-        for (int j = lane; j < g.held * 8; j += 32) recode16<kInt8>(reinterpret_cast<uint4*>(codes) + j, old, s);
-#pragma unroll 1
-    for (int r = 0; r < g.rows; r += 2) {
-        if (r + row < g.rows) {
-            if (g.rows > 2) w = __ldg(reinterpret_cast<const uint4*>(x + (size_t)(r + row) * c.Hkv * kD));
-            *reinterpret_cast<uint2*>(codes + (size_t)(g.held + r + row) * kD + 8 * (lane & 15)) = encode8<kInt8>(w, s, reciprocal(s));
+static cudaError_t launch_append(const CacheAppendArgs& p, cudaStream_t stream) {
+    const unsigned units = (unsigned)((p.T >> p.c.page_shift) + 2 * p.c.B);
+    const long long B = p.c.B;
+    // Few pages: eight warps each, as long as these CTAs are at most some 8 an SM.  8 heads, pages of 16, e4m3: 8
+    // sequences x 16 tokens 3.0 us, with 16 rows a warp 4.2; 16 x 128 7.0 with 16 rows a warp, 9.2 so; 1 to 4 tokens a
+    // sequence are as fast either way, from 32 sequences on faster with a warp a page.
+    if (p.T > 4 * B && (long long)units * 2 * p.c.Hkv <= 8 * 148) {
+        switch (p.c.page_shift) {
+            case 4: return launch_append<kInt8, 8, 1>(p, units, stream);
+            case 5: return launch_append<kInt8, 8, 2>(p, units, stream);
+            case 6: return launch_append<kInt8, 8, 4>(p, units, stream);
+            default: return launch_append<kInt8, 8, 8>(p, units, stream);
         }
     }
-    if (lane == 0) *scale = s;
-}
-
-template <bool kInt8>
-static cudaError_t launch_rows(const CacheAppendArgs& p, dim3 grid, cudaStream_t stream) {
-    switch (p.c.page_shift) {
-        case 4: return launch_pdl(gdn_cache_append_kernel<kInt8, 1>, grid, dim3(256), 0, stream, p);
-        case 5: return launch_pdl(gdn_cache_append_kernel<kInt8, 2>, grid, dim3(256), 0, stream, p);
-        case 6: return launch_pdl(gdn_cache_append_kernel<kInt8, 4>, grid, dim3(256), 0, stream, p);
-        default: return launch_pdl(gdn_cache_append_kernel<kInt8, 8>, grid, dim3(256), 0, stream, p);
+    // One warp a page where sequences get 16 tokens at most on average: 200 x 16 tokens in pages of 64 8.4 us, with a warp
+    // for each 16 rows 9.6; 200 x 32 22.7 with one warp, 20.8 so.
+    switch (p.T <= 16 * B ? 4 : p.c.page_shift) {
+        case 4: return launch_append<kInt8, 1, 8>(p, units, stream);
+        case 5: return launch_append<kInt8, 2, 8>(p, units, stream);
+        case 6: return launch_append<kInt8, 4, 8>(p, units, stream);
+        default: return launch_append<kInt8, 8, 8>(p, units, stream);
     }
 }
 
 int launch_cache_append(const CacheAppendArgs& p, cudaStream_t stream) {
-    const unsigned units = (unsigned)((p.T >> p.c.page_shift) + 2 * p.c.B);
-    cudaError_t e;
-    if (p.T <= 8 * (long long)p.c.B) {  // at most 8 tokens a sequence on average
-        const dim3 grid(units, (unsigned)(2 * p.c.Hkv + 7) / 8);
-        e = p.c.int8 ? launch_pdl(gdn_cache_append_few_kernel<true>, grid, dim3(256), 0, stream, p)
-                     : launch_pdl(gdn_cache_append_few_kernel<false>, grid, dim3(256), 0, stream, p);
-    } else {
-        const dim3 grid(units, (unsigned)p.c.Hkv, 2);
-        e = p.c.int8 ? launch_rows<true>(p, grid, stream) : launch_rows<false>(p, grid, stream);
-    }
-    return e == cudaSuccess ? 0 : -1;
+    return (p.c.int8 ? launch_append<true>(p, stream) : launch_append<false>(p, stream)) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace gdn
