@@ -10,8 +10,8 @@
 // A warp holds its rows of a (page a sequence touches, head, key or value) in registers between the maximum and the
 // encoding.  What a CTA waits for in turn (the lengths, the rows and the table, the page's scale) sets the rate, so many
 // bytes have to be in flight: 16 rows a warp, 128 bytes a thread.
-// The quotients would cost more than the traffic: a code is taken from x (1 / s), and from the quotient where the two
-// could round to different codes.
+// Divisions would cost more than the traffic.  With r = 1 / s rounded and q = x r rounded, q + r (x - q s) in two fused
+// steps is x / s rounded (Markstein, IBM J. Res. Dev. 34, 1990), as long as nothing underflows.
 #include <cuda_fp16.h>
 
 #include "linear.cuh"
@@ -49,11 +49,11 @@ __device__ __forceinline__ Sequence find_sequence(const CacheAppendArgs& p, int 
     }
 }
 
-// Largest magnitude of 8 bf16 values so far, per half; NaN does not count, infinity is dealt with by finite_max.
+// Largest magnitude of 8 bf16 values so far, per half; a NaN stays.
 __device__ __forceinline__ __nv_bfloat162 abs_max(__nv_bfloat162 top, uint4 w) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) top = __hmax2(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u[e])));
+    for (int e = 0; e < 4; ++e) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u[e])));
     return top;
 }
 __device__ __forceinline__ float finite_max(uint4 w) {
@@ -83,50 +83,32 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(y) : "f"(d), "f"(c));
     return (uint32_t)x | ((uint32_t)y << 16);
 }
-// Eight bf16 values to codes, by r = 1 / s rounded; false where a quotient might have another code.
-template <bool kInt8>
-__device__ __forceinline__ bool encode8(uint4 w, float r, uint2& codes) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    bool differ = false;
-    if (kInt8) {  // infinity or NaN among them
-        __nv_bfloat162 top = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u[0]));
-#pragma unroll
-        for (int e = 1; e < 4; ++e) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u[e])));
-        const uint32_t bits = *reinterpret_cast<const uint32_t*>(&top);
-        differ = (bits & 0x7f80u) == 0x7f80u || (bits & 0x7f800000u) == 0x7f800000u;
-    }
-    uint32_t o[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const float2 x = make_float2(__uint_as_float(u[2 * e] << 16), __uint_as_float(u[2 * e] & 0xffff0000u));
-        const float2 y = make_float2(__uint_as_float(u[2 * e + 1] << 16), __uint_as_float(u[2 * e + 1] & 0xffff0000u));
-        if (kInt8) {
-            // x (1 / s) is within 127 2^-22 < 2^-15 of x / s: another code only where it is that near to a half
-            const float2 r2 = make_float2(r, r), big = make_float2(12582912.f, 12582912.f);  // + 1.5 2^23: the rounded integer in the low bits
-            const float2 qx = mul2(x, r2), qy = mul2(y, r2), nx = add2(qx, big), ny = add2(qy, big);
-            const float2 dx = sub2(qx, sub2(nx, big)), dy = sub2(qy, sub2(ny, big));
-            differ |= fmaxf(fmaxf(fabsf(dx.x), fabsf(dx.y)), fmaxf(fabsf(dy.x), fabsf(dy.y))) > 0.5f - 0x1p-14f;
-            o[e] = __byte_perm(__byte_perm(__float_as_uint(nx.x), __float_as_uint(nx.y), 0x0040),
-                               __byte_perm(__float_as_uint(ny.x), __float_as_uint(ny.y), 0x0040), 0x5410);
-        } else {
-            // x (1 / s) is within 2^-22 of x / s, whose code lies between those of r (1 -+ 2^-21)
-            const float2 lo = make_float2(r * (1.f - 0x1p-21f), r * (1.f - 0x1p-21f)), hi = make_float2(r * (1.f + 0x1p-21f), r * (1.f + 0x1p-21f));
-            const float2 a = mul2(x, lo), b = mul2(y, lo), c = mul2(x, hi), d = mul2(y, hi);
-            o[e] = encode4<false, false>(a.x, a.y, b.x, b.y);
-            differ |= o[e] != encode4<false, false>(c.x, c.y, d.x, d.y);
-        }
-    }
-    codes = make_uint2(o[0], o[1]);
-    return !differ;
+// x / s rounded, for finite x and r = 1 / s rounded, 2^-60 < s < 2^60.  (Quotients below 2^-30 may be off; their codes are 0.)
+// Formed negated, which keeps the sign of a zero.
+__device__ __forceinline__ float2 quotients(float2 x, float s, float r) {
+    const float2 minus = make_float2(-r, -r), q = mul2(x, minus), y = fma2(fma2(q, make_float2(s, s), x), minus, q);
+    return make_float2(-y.x, -y.y);
 }
-// The same from the quotients.  (s = 0: zeros, or values whose scale is below fp32.)
+__device__ __forceinline__ float reciprocal(float s) { return s > 0x1p-60f && s < 0x1p60f ? __frcp_rn(s) : 0.f; }
+// Eight bf16 values to codes.  r: reciprocal(s), or 0 where there is none or not all values are finite.
+// (s = 0: zeros, or values whose scale is below fp32.)
 template <bool kInt8>
-__device__ __forceinline__ uint2 encode8_exactly(uint4 w, float s) {
+__device__ __forceinline__ uint2 encode8(uint4 w, float s, float r) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    float x[8];
+    float2 x[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = __fdiv_rn(__uint_as_float(e & 1 ? u[e >> 1] & 0xffff0000u : u[e >> 1] << 16), s);
-    return s > 0.f ? make_uint2(encode4<kInt8, true>(x[0], x[1], x[2], x[3]), encode4<kInt8, true>(x[4], x[5], x[6], x[7])) : make_uint2(0, 0);
+    for (int e = 0; e < 4; ++e) x[e] = make_float2(__uint_as_float(u[e] << 16), __uint_as_float(u[e] & 0xffff0000u));
+    if (r != 0.f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = quotients(x[e], s, r);
+        return make_uint2(encode4<kInt8, false>(x[0].x, x[0].y, x[1].x, x[1].y), encode4<kInt8, false>(x[2].x, x[2].y, x[3].x, x[3].y));
+    }
+    uint2 y = make_uint2(0, 0);
+    if (s > 0.f) {
+        y.x = encode4<kInt8, true>(__fdiv_rn(x[0].x, s), __fdiv_rn(x[0].y, s), __fdiv_rn(x[1].x, s), __fdiv_rn(x[1].y, s));
+        y.y = encode4<kInt8, true>(__fdiv_rn(x[2].x, s), __fdiv_rn(x[2].y, s), __fdiv_rn(x[3].x, s), __fdiv_rn(x[3].y, s));
+    }
+    return y;
 }
 template <bool kInt8>
 __device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
@@ -144,23 +126,27 @@ __device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
         }
     }
 }
-// 16 codes of scale `old` to scale s.
+// 16 codes of scale `old` to scale s > old.
 template <bool kInt8>
-__device__ __forceinline__ void recode16(uint4* at, float old, float s) {
+__device__ __forceinline__ void recode16(uint4* at, float old, float s, float r) {
     const uint4 y = *at;
     uint32_t u[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         float f[4];
         decode4<kInt8>(u[e], f);
-#pragma unroll
-        for (int d = 0; d < 4; ++d) f[d] = __fdiv_rn(__fmul_rn(f[d], old), s);
-        u[e] = encode4<kInt8, true>(f[0], f[1], f[2], f[3]);
+        float2 a = mul2(make_float2(f[0], f[1]), make_float2(old, old)), b = mul2(make_float2(f[2], f[3]), make_float2(old, old));
+        if (r != 0.f) {
+            a = quotients(a, s, r);
+            b = quotients(b, s, r);
+        } else {
+            a = make_float2(__fdiv_rn(a.x, s), __fdiv_rn(a.y, s));
+            b = make_float2(__fdiv_rn(b.x, s), __fdiv_rn(b.y, s));
+        }
+        u[e] = encode4<kInt8, true>(a.x, a.y, b.x, b.y);
     }
     *at = make_uint4(u[0], u[1], u[2], u[3]);
 }
-// 1 / s for encode8, or 0 where it or its products may leave fp32's normal range.
-__device__ __forceinline__ float reciprocal(float s) { return s > 0x1p-100f && s < 0x1p100f ? __frcp_rn(s) : 0.f; }
 
 // What one page of one sequence gets from the call.
 struct AppendPage {
@@ -223,7 +209,8 @@ __global__ void __launch_bounds__(256, L == 8 ? 4 : 5) gdn_cache_append_kernel(C
         load_block(r0 += 2 * L);
     }
     float top = fmaxf(__low2float(top2), __high2float(top2));
-    if (top == INFINITY) {
+    const bool odd = !(__low2float(top2) < INFINITY && __high2float(top2) < INFINITY);  // infinities or NaN among them
+    if (odd) {
         top = 0.f;
 #pragma unroll 1
         for (int r = 2 * L * part + row; r < min(rows, r0 + 2 * L); r += 2) top = fmaxf(top, finite_max(load(r)));
@@ -236,26 +223,19 @@ __global__ void __launch_bounds__(256, L == 8 ? 4 : 5) gdn_cache_append_kernel(C
 #pragma unroll
         for (int i = 0; i < W; ++i) top = fmaxf(top, s_max[warp - part + i]);
     }
-    const float s = fmaxf(old, __fdiv_rn(top, kInt8 ? 127.f : 448.f)), inv = reciprocal(s);
+    const float s = fmaxf(old, __fdiv_rn(top, kInt8 ? 127.f : 448.f)), inv = odd ? 0.f : reciprocal(s);
 
     codes += g.held * kD;
     while (true) {
-        unsigned again = 0;  // rows to encode from their quotients
         uint8_t* to = codes + (r0 + row) * kD + 8 * (lane & 15);
         const int left = rows - r0 - row;
+        if (inv != 0.f) {
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            uint2 y;
-            if (2 * i < left) {
-                if (!encode8<kInt8>(w[i], inv, y) || inv == 0.f) again |= 1u << i;
-                *reinterpret_cast<uint2*>(to + 2 * i * kD) = y;
-            }
-        }
+            for (int i = 0; i < L; ++i)
+                if (2 * i < left) *reinterpret_cast<uint2*>(to + 2 * i * kD) = encode8<kInt8>(w[i], s, inv);
+        } else {
 #pragma unroll 1
-        while (again) {
-            const int i = __ffs(again) - 1;
-            again &= again - 1;
-            *reinterpret_cast<uint2*>(to + 2 * i * kD) = encode8_exactly<kInt8>(load(r0 + row + 2 * i), s);
+            for (int i = 0; 2 * i < min(left, 2 * L); ++i) *reinterpret_cast<uint2*>(to + 2 * i * kD) = encode8<kInt8>(load(r0 + row + 2 * i), s, 0.f);
         }
         if (W > 1 || r0 == 0) break;
         load_block(r0 -= 2 * L);
@@ -263,7 +243,7 @@ __global__ void __launch_bounds__(256, L == 8 ? 4 : 5) gdn_cache_append_kernel(C
     codes -= g.held * kD;
     if (here && g.held > 0 && s > old)  // older tokens of the page to the new scale, 16 bytes a thread
 #pragma unroll 1
-        for (int j = 32 * part + lane; j < g.held * 8; j += 32 * W) recode16<kInt8>(reinterpret_cast<uint4*>(codes) + j, old, s);
+        for (int j = 32 * part + lane; j < g.held * 8; j += 32 * W) recode16<kInt8>(reinterpret_cast<uint4*>(codes) + j, old, s, reciprocal(s));
     if (here && part == 0 && lane == 0) *scale = s;
 }
 
@@ -286,9 +266,9 @@ static cudaError_t launch_append(const CacheAppendArgs& p, cudaStream_t stream) 
             default: return launch_append<kInt8, 8, 8>(p, units, stream);
         }
     }
-    // One warp a page where sequences get 16 tokens at most on average: 200 x 16 tokens in pages of 64 8.4 us, with a warp
-    // for each 16 rows 9.6; 200 x 32 22.7 with one warp, 20.8 so.
-    switch (p.T <= 16 * B ? 4 : p.c.page_shift) {
+    // One warp a page where sequences get 32 tokens at most on average: 200 x 1 token in pages of 64 4.9 us, with a warp
+    // for each 16 rows 11.4; 200 x 32 13.7 and 20.7, 64 x 32 10.7 and 9.5, 200 x 64 29 both ways.
+    switch (p.T <= 32 * B ? 4 : p.c.page_shift) {
         case 4: return launch_append<kInt8, 1, 8>(p, units, stream);
         case 5: return launch_append<kInt8, 2, 8>(p, units, stream);
         case 6: return launch_append<kInt8, 4, 8>(p, units, stream);
