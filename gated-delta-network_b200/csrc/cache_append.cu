@@ -9,7 +9,8 @@
 // Bound by HBM for prompts (768 bytes a token and head, each row read and written once) and by latency for decode steps.
 // A warp holds its rows of a (page a sequence touches, head, key or value) in registers between the maximum and the
 // encoding.  What a CTA waits for in turn (the lengths, the rows and the table, the page's scale) sets the rate, so many
-// bytes have to be in flight: 16 rows a warp, 128 bytes a thread.
+// bytes have to be in flight: 16 rows a warp, 128 bytes a thread.  12 prompts of 10 to 8192 tokens, 8 heads, pages of 64:
+// 22.1 us (5.0 TB/s); 200 x 1 token: 4.8 us.
 // Divisions would cost more than the traffic.  With r = 1 / s rounded and q = x r rounded, q + r (x - q s) in two fused
 // steps is x / s rounded (Markstein, IBM J. Res. Dev. 34, 1990), as long as nothing underflows.
 #include <cuda_fp16.h>
@@ -170,10 +171,10 @@ __device__ __forceinline__ AppendPage find_page(const CacheAppendArgs& p, int un
     return r;
 }
 
-// W warps for each (page, head, key or value), 8 / W of these a CTA; a warp takes 2 L new rows, two a load (W = 1: that
-// many at a time).
-template <bool kInt8, int W, int L>
-__global__ void __launch_bounds__(256, L == 8 ? 4 : 5) gdn_cache_append_kernel(CacheAppendArgs p) {
+// W warps for each (page, head, key or value), 8 / W of these a CTA; a warp takes 16 new rows, two a load (W = 1: 16 at a
+// time).
+template <bool kInt8, int W>
+__global__ void __launch_bounds__(256, 4) gdn_cache_append_kernel(CacheAppendArgs p) {
     __shared__ float s_max[8];
     pdl_wait();
     pdl_trigger();
@@ -187,6 +188,7 @@ __global__ void __launch_bounds__(256, L == 8 ? 4 : 5) gdn_cache_append_kernel(C
     const uint16_t* x = (pair & 1 ? p.v : p.k) + (g.token * c.Hkv + head) * kD + 8 * (lane & 15);
     auto load = [&](int r) { return __ldg(reinterpret_cast<const uint4*>(x + (size_t)r * c.Hkv * kD)); };
 
+    constexpr int L = 8;
     uint4 w[L];
     auto load_block = [&](int r0) {
         const uint16_t* at = x + (size_t)(r0 + row) * c.Hkv * kD;
@@ -247,32 +249,21 @@ __global__ void __launch_bounds__(256, L == 8 ? 4 : 5) gdn_cache_append_kernel(C
     if (here && part == 0 && lane == 0) *scale = s;
 }
 
-template <bool kInt8, int W, int L>
-static cudaError_t launch_append(const CacheAppendArgs& p, unsigned units, cudaStream_t stream) {
-    return launch_pdl(gdn_cache_append_kernel<kInt8, W, L>, dim3(units, (unsigned)(2 * p.c.Hkv * W + 7) / 8), dim3(256), 0, stream, p);
+template <bool kInt8, int W>
+static cudaError_t launch_append(const CacheAppendArgs& p, cudaStream_t stream) {
+    const dim3 grid((unsigned)((p.T >> p.c.page_shift) + 2 * p.c.B), (unsigned)(2 * p.c.Hkv * W + 7) / 8);
+    return launch_pdl(gdn_cache_append_kernel<kInt8, W>, grid, dim3(256), 0, stream, p);
 }
+// A warp for each 16 rows of a page, or one for all of them where sequences get 32 tokens at most on average.  8 heads,
+// pages of 64, us with one warp a page and with four: 200 x 1 token 4.8 and 11.5, 200 x 32 10.4 and 17.9, 64 x 32 8.0 and
+// 7.8, 4 x 32 4.3 and 3.0, 64 x 64 12.4 and 9.4.  (CTAs cost as much as rows here, and half of a short call's get none.)
 template <bool kInt8>
 static cudaError_t launch_append(const CacheAppendArgs& p, cudaStream_t stream) {
-    const unsigned units = (unsigned)((p.T >> p.c.page_shift) + 2 * p.c.B);
-    const long long B = p.c.B;
-    // Few pages: eight warps each, as long as these CTAs are at most some 8 an SM.  8 heads, pages of 16, e4m3: 8
-    // sequences x 16 tokens 3.0 us, with 16 rows a warp 4.2; 16 x 128 7.0 with 16 rows a warp, 9.2 so; 1 to 4 tokens a
-    // sequence are as fast either way, from 32 sequences on faster with a warp a page.
-    if (p.T > 4 * B && (long long)units * 2 * p.c.Hkv <= 8 * 148) {
-        switch (p.c.page_shift) {
-            case 4: return launch_append<kInt8, 8, 1>(p, units, stream);
-            case 5: return launch_append<kInt8, 8, 2>(p, units, stream);
-            case 6: return launch_append<kInt8, 8, 4>(p, units, stream);
-            default: return launch_append<kInt8, 8, 8>(p, units, stream);
-        }
-    }
-    // One warp a page where sequences get 32 tokens at most on average: 200 x 1 token in pages of 64 4.9 us, with a warp
-    // for each 16 rows 11.4; 200 x 32 13.7 and 20.7, 64 x 32 10.7 and 9.5, 200 x 64 29 both ways.
-    switch (p.T <= 32 * B ? 4 : p.c.page_shift) {
-        case 4: return launch_append<kInt8, 1, 8>(p, units, stream);
-        case 5: return launch_append<kInt8, 2, 8>(p, units, stream);
-        case 6: return launch_append<kInt8, 4, 8>(p, units, stream);
-        default: return launch_append<kInt8, 8, 8>(p, units, stream);
+    switch (p.T <= 32 * (long long)p.c.B ? 4 : p.c.page_shift) {
+        case 4: return launch_append<kInt8, 1>(p, stream);
+        case 5: return launch_append<kInt8, 2>(p, stream);
+        case 6: return launch_append<kInt8, 4>(p, stream);
+        default: return launch_append<kInt8, 8>(p, stream);
     }
 }
 
