@@ -267,6 +267,7 @@ int gdn_linear_prefill_fwd(const void* q, const void* k, const void* v, const fl
     p.new_state = new_state;
     p.ctas = gdn::kLinearCtas;
     p.min_share = lay.min_share;
+    p.whole = lay.whole;
     p.keep = lay.keep;
     p.cut = lay.cut;
     p.kind = reinterpret_cast<int4*>(ws + lay.off_kind);

@@ -36,7 +36,8 @@ struct LinearPrefillArgs {
     float* new_state;      // [N, HV, 128, 128] (may alias state)
     int ctas;              // stretches of the line of chunks, one per SM
     int min_share;         // chunks of a stretch, at least
-    int keep;              // segments of at most this many chunks are not cut
+    int whole;             // no segment is cut if the longest one has at most this many chunks,
+    int keep;              // else those of at most this many are not
     int cut;               // a sequence can be longer than that: build and chain segment states
     int* status;           // workspace: first error code of a bounded wait
     int4* kind;            // workspace: [ctas] what the stretch's last segment does, its sequence and v-head
@@ -47,7 +48,7 @@ struct LinearPrefillArgs {
 constexpr int kLinearCtas = 148;
 
 struct LinearPrefillLayout {
-    int min_share, keep, cut;
+    int min_share, whole, keep, cut;
     size_t off_status, off_kind, off_gamma, off_seg, total;
 };
 LinearPrefillLayout linear_prefill_layout(int N, int T, int HV);

@@ -4,23 +4,30 @@
 // C = 64 tokens with G_i = a_1 + .. + a_i and the state S_0 at its start:
 //   o_i = scale (e^{G_i} S_0 q_i + sum_{j <= i} e^{G_i - G_j} (q_i . k_j) v_j)
 //   S_C = e^{G_C} S_0 + sum_j (e^{G_C - G_j} v_j) k_j^T
-// Four tcgen05 products a chunk, the V dimension as the 128 rows:
-//   QK  [Q; K] (128 x 128, K-major) x K (64 tokens)            -> rows 0-63: q_i . k_j
-//   U   Vd^T (128 V x 64 tokens, A from TMEM) x K (128 K)      -> what the chunk adds to the state
+// Four tcgen05 products a chunk:
+//   QK  Q (64 tokens) x K (64 tokens)                          -> q_i . k_j
+//   U   Vd^T (128 V x 64 tokens, A from TMEM) x K (128 K)      -> added to the state where it lies in TMEM
 //   OA  V^T (128 V x 64 tokens, MN-major from the v tile) x P  -> P = decayed, causal QK in bf16
 //   OI  S_0 (128 V x 128 K, A from TMEM) x Q (64 tokens)       -> S_0 q_i, scaled by e^{G_i} in the epilogue
-// The state stays in fp32 registers (one V row a thread); its bf16 copy for OI and P round to 2^-8, as the output
-// does.  The decayed v is cut into three bf16 parts that keep all 24 bits, so the state is as exact as an fp32 sum.
+// The state stays in TMEM in fp32, in a unit 2^X that takes the decays, so that it is multiplied only where X would leave
+// [-8, 8] or a segment ends: mostly, U adds to it and a bf16 copy for OI is all that is read.  That copy and P round to
+// 2^-8, as the output does (the q, k and v they meet are bf16 too).  The decayed v is cut into three bf16 parts that keep
+// all 24 bits: the state is off by 4e-7 after 2 chunks and 1e-6 in the long run (the tensor core's sums drop bits that an
+// fp32 sum would round; two parts gave 3e-6).
 //
-// Bound by HBM (1 KB a token and head), then by shared-memory bandwidth: operands that a thread forms anyway (S_0,
-// Vd) go to TMEM, which takes 128 KB a chunk off it.  Every product and every group of warps works on a
-// chunk of its own: TMA and gates run ahead, the P and V warps prepare chunk c + 1 while the tensor core works on c
-// and the output warps write c - 1; only h <- e^{G_C} h + U and the product OI form a chain over chunks.
+// Bound by HBM for many sequences (1 KB a token and head), but not reached: S -> OI and U -> S form a chain over the
+// chunks, some 2750 clocks each for one CTA an SM.  Operands that a thread forms anyway (S_0, Vd) go to TMEM, which takes
+// 128 KB a chunk off the shared-memory bandwidth.  Every product and every group of warps works on a chunk of its own: TMA
+// and gates run ahead, the P and V warps prepare chunk c + 1 while the tensor core works on c and the output warps write
+// c - 1.  Loops stay rolled: unrolled, the roles together missed the instruction cache and warps waited 2.9 clocks an
+// instruction for it, 0.5 now.  4 q/k and 8 v heads: 64 x 4096 tokens 432 to 460 us (3.6 to 3.9 TB/s, 0.30 PFLOP/s), 16 of
+// 6 to 8192 93, 1 x 8192 46, 1 x 100 10.7.  Not better: 1024 threads with a second group of warps for P; OI in tf32 from
+// the fp32 state without the bf16 copy (64 x 4096 443 -> 485).
 //
 // Tokens are cut evenly over the CTAs whatever the lengths: all (sequence, v-head) segments lie on one line in
 // chunks, and a CTA takes an equal stretch of it.  The state at a stretch's start comes from two launches before:
 // what every unfinished segment adds to the state in its CTA (U alone; it does not read the state), and a chain over
-// those sums.  Stretches end at segment ends where segments are short, so such calls need one launch.
+// those sums.  Where no segment is long, stretches end at segment ends and one launch does it all.
 #include <algorithm>
 
 #include "linear.cuh"
@@ -86,7 +93,7 @@ __device__ __forceinline__ int lin_chunks(int s, int e) { return max(0, (e - s +
 // point refuses calls of 2^31 chunks.)
 __device__ __forceinline__ void find_range(const LinearPrefillArgs& p, Mark* at) {
     const int lane = threadIdx.x & 31, part = (p.N + 31) / 32, n0 = min(p.N, lane * part), n1 = min(p.N, n0 + part);
-    int x = 0, lo = 0, total = 0, per = 0, more = 0;
+    int x = 0, lo = 0, total = 0, per = 0, more = 0, keep = 0;
 #pragma unroll 1
     for (int round = 0; round < 2; ++round) {  // the sum of the lane's lengths, then the marks among them
         int s = n0 < n1 ? cu_at(p, n0) : 0;
@@ -95,14 +102,17 @@ __device__ __forceinline__ void find_range(const LinearPrefillArgs& p, Mark* at)
             const int e = cu_at(p, n + 1), nc = lin_chunks(s, e), w = nc + 2;
             s = e;
             x += w;
-            if (round == 0) continue;
+            if (round == 0) {
+                keep = max(keep, nc);
+                continue;
+            }
 #pragma unroll 1
             for (int i = 0; i < 2; ++i) {
                 const int c = blockIdx.x + i, off = min(total, c * per + min(c, more)) - lo;
                 if (off < 0 || off >= w * p.HV) continue;
                 Mark m{n, off / w, 0};
                 const int place = off - m.hv * w - 2;
-                if (nc > p.keep) {
+                if (nc > keep) {
                     m.chunk = max(0, place);
                 } else if (2 * place >= nc) {  // a short segment is not cut: to its nearer end
                     if (++m.hv == p.HV) m = Mark{n + 1, 0, 0};
@@ -118,6 +128,8 @@ __device__ __forceinline__ void find_range(const LinearPrefillArgs& p, Mark* at)
                 const int y = __shfl_up_sync(0xffffffffu, x, off);
                 if (lane >= off) x += y;
             }
+            keep = __reduce_max_sync(0xffffffffu, keep);
+            if (keep > p.whole) keep = p.keep;
             lo = (x - mine) * p.HV;
             total = __shfl_sync(0xffffffffu, x, 31) * p.HV;
             const int ctas = max(1, min(p.ctas, total / p.min_share)), c = blockIdx.x + lane;
@@ -964,11 +976,18 @@ __global__ void __launch_bounds__(256) gdn_linear_chain_kernel(LinearPrefillArgs
     }
 }
 
+// A segment that is cut costs its chunks twice, in part, and the call three launches instead of one; one that is not may
+// make a CTA's stretch that much longer.  So none is cut while the longest is shorter than an equal share and 16 chunks
+// (us without and with cuts, 8 heads: 12 x 2048 tokens 66 and 101, 20 x 2048 119 and 138, 1 x 1000 31 and 30, 60 of 100 to
+// 4000 184 and 203; 30 of 200 to 6000 205 and 180).  Beyond that, short ones stay whole: with 16 or 0.3 shares instead of
+// 8 or 0.3 shares 8 of 64 to 4096 54 instead of 57, with 16 and half a share 64.  A stretch is at least 4 chunks long
+// where there are cuts: 1 x 2500 31 us, with 1 chunk 32.5, with 8 40.
 LinearPrefillLayout linear_prefill_layout(int N, int T, int HV) {
     LinearPrefillLayout L{};
     const long long share = ((long long)T / lin::C + 3ll * N) * HV / kLinearCtas;  // places of a CTA
-    L.keep = (int)std::min<long long>(16 + share / 2, 1 << 20);
-    L.cut = T > (long long)lin::C * L.keep ? 1 : 0;
+    L.whole = (int)std::min<long long>(16 + share, 1 << 24);
+    L.keep = (int)std::max<long long>(16, std::min<long long>(3 * share / 10, 1 << 24));
+    L.cut = T > (long long)lin::C * L.whole ? 1 : 0;
     L.min_share = L.cut ? 4 : 1;
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     const size_t slots = L.cut ? kLinearCtas : 0;

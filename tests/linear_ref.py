@@ -38,7 +38,7 @@ def check(out, new_state, ref, chunked):
 
     Output: one rounding to bf16 at the end, and in the chunked form one of the state copy or of the decayed
     products before it, each u = 2^-8 of the terms' magnitudes (2 u covers both and the fp32 sums).  State: fp32
-    sums, and in the chunked form the decayed v as two bf16 parts, u^2 = 2^-16 of the magnitudes; 2^-15 covers that,
+    sums, and in the chunked form the decayed v as bf16 parts, two of which are u^2 = 2^-16 off; 2^-15 covers that,
     the fp32 sums of up to 64 terms and of the chunks, and the decays (a prefix sum of at most 20 where the decay
     matters, so 20 * 2^-23 relative).
     """
