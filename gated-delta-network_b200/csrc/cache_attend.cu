@@ -19,10 +19,14 @@
 //    needs a shuffle or a transposing load: key step s of lane l holds dims 32 (l % 4) + 4 s .. and the same of q;
 //    value lane l holds dims 16 (l / 4) .. of the four tokens whose weights it owns (after one 8 x 8 transpose).
 //  * 16 tokens of k or v of a head are 2 KB in a row, one TMA copy; every warp has a ring of three such pairs of its
-//    own.  (16-byte cp.async into the same ring stopped at 4.6 TB/s with nothing saturated.)
+//    own.  (16-byte cp.async into the same ring stopped at 4.6 TB/s with nothing saturated; two stages and three CTAs
+//    an SM instead of two were slower, 150 us where this takes 95.)
 //  * Tokens are cut evenly over the CTAs whatever the lengths: all (sequence, head, row tile) segments in 32-token
 //    blocks on one line, an equal stretch of it per CTA. A stretch's first and last segment may continue in a
 //    neighbour; those pieces go to the workspace, and a second launch joins them.
+// 8 kv heads, e4m3: 64 x 4096 tokens with 4 rows a head 95 us (5.65 TB/s); 16 rows (64 x 2048) 78 us and 32 rows 121 us,
+// where the products and conversions bound it; 1 x 1000 tokens 13 us, most of it the two launches and what a CTA waits
+// for in turn.
 #include <cuda_fp16.h>
 
 #include "linear.cuh"
@@ -36,8 +40,9 @@ constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kBlock = 32;                       // tokens of the unit that is divided over the CTAs
 constexpr int kStages = 3;
 constexpr int kStageBytes = 4096;                // a warp's 16 tokens of k and of v, rows of 128 bytes, SWIZZLE_128B
-constexpr int kOwn = 16;                         // places of a segment on the line besides its blocks
-constexpr int kKeep = 16;                        // segments of at most this many blocks are not cut
+// Places of a segment on the line besides its blocks (24 of 17 to 6000 tokens, 16 rows: 37 us; with 4 places 45), and the
+// blocks up to which one is not cut (32 x 512 tokens: 15 us, cut 18; that ragged batch would take 34 with every cut).
+constexpr int kOwn = 16, kKeep = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 4.f;                    // scores may exceed the reference by this (base 2)
 // Shared memory for tiles of 8 NT rows: the ring, whose place the warps' results take; q as B fragments
@@ -497,10 +502,17 @@ __global__ void __launch_bounds__(128) gdn_cache_join_kernel(CacheAttendArgs p, 
     pdl_wait();
     pdl_trigger();
     if (blockIdx.x == 0 && blockIdx.y == 0) {  // the call's status: any of the CTAs'
-        int st = 0;
-        for (int i = threadIdx.x; i < (int)gridDim.x; i += 128) st = max(st, p.piece[i].z);
-        const int page = __syncthreads_or(st == kErrBadPage), any = __syncthreads_or(st != 0);
-        if (threadIdx.x == 0) *p.status = page ? kErrBadPage : any ? kErrBadSeqlens : 0;
+        bool late = false, page = false, length = false;
+        for (int i = threadIdx.x; i < (int)gridDim.x; i += 128) {
+            const int st = p.piece[i].z;
+            late |= st == kErrScanTmaTimeout;
+            page |= st == kErrBadPage;
+            length |= st == kErrBadSeqlens;
+        }
+        late = __syncthreads_or(late);
+        page = __syncthreads_or(page);
+        length = __syncthreads_or(length);
+        if (threadIdx.x == 0) *p.status = late ? kErrScanTmaTimeout : page ? kErrBadPage : length ? kErrBadSeqlens : 0;
     }
     const int4 pc = p.piece[blockIdx.x];
     if (pc.x < 0) return;
@@ -556,7 +568,9 @@ static int launch_attend(const CacheAttendArgs& p, cudaStream_t stream) {
     return launch_pdl(gdn_cache_join_kernel, dim3(ctas, (unsigned)(rows < kRows ? rows : kRows)), dim3(128), 0, stream, p, kRows) == cudaSuccess ? 0 : -1;
 }
 
-// Column tiles of 8 rows: as many as a kv head's q rows need, at most 4 (the accumulators fill the registers).
+// Column tiles of 8 rows: as many as a kv head's q rows need, at most 4 (the accumulators fill the registers).  64 x 2048
+// tokens with 16 rows: 100 us in tiles of 8, 78 of 16, 112 of 32; with 32 rows 182 of 8, 121 of 32; 64 x 4096 with 4 rows
+// 95 of 8, 185 of 32.
 int attend_tiles(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
 int launch_cache_attend(const CacheAttendArgs& p, cudaStream_t stream) {
