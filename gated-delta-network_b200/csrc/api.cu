@@ -286,7 +286,7 @@ namespace {
 int cache_args(void* k_cache, void* v_cache, float* k_scale, float* v_scale, int code, const int* block_table,
                const void* seq_lens, int len_is_int64, int num_pages, int page_size, int max_pages, int B, int Hkv, int D,
                gdn::CacheArgs* c) {
-    if (D != GDN_HEAD_DIM || Hkv < 1 || Hkv > 65535) return GDN_ERR_SHAPE;
+    if (D != GDN_HEAD_DIM || Hkv < 1 || Hkv > 32767) return GDN_ERR_SHAPE;  // (2 Hkv blocks in a grid's y)
     if (code != GDN_CODE_INT8 && code != GDN_CODE_E4M3) return GDN_ERR_SIZE;
     int shift = 4;
     while (shift < 7 && (1 << shift) != page_size) ++shift;

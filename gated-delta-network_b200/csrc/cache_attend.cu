@@ -14,7 +14,7 @@
 //  * The maximum is a reference that moves only when a score exceeds it by 4 (base 2), so most steps need no
 //    reduction and no rescaling; weights stay below 2^4 in fp16, their sum is fp32 and of the unrounded ones.
 //  * The value scale enters the weights: p v_scale / r with r the largest value scale so far, kept like the maximum,
-//    so the accumulator never sees the scales' range.
+//    so the accumulator never sees the scales' range.  Weights round to 2^-11, or to 2^-25 r where they are below 2^-14.
 //  * Both contractions may permute their index, so a thread takes 16 consecutive bytes of a row and no fragment
 //    needs a shuffle or a transposing load: key step s of lane l holds dims 32 (l % 4) + 4 s .. and the same of q;
 //    value lane l holds dims 16 (l / 4) .. of the four tokens whose weights it owns (after one 8 x 8 transpose).

@@ -134,12 +134,12 @@ PAGE_SIZES = (16, 32, 64, 128)
 
 def cache_tensors(k_cache, v_cache, k_scale, v_scale, device: torch.device):
     """Checks of a paged 8-bit cache, which is used in place; returns (code, pages, Hkv, page size)."""
-    shape, dtype = k_cache.shape, k_cache.dtype
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != device.index or t.dtype not in CODES
                 or t.dim() != 4 or t.shape[3] != HEAD_DIM or not t.is_contiguous() or t.data_ptr() & 15):
             raise ValueError(f"{name} must be a contiguous, 16-byte aligned int8 or float8_e4m3fn CUDA tensor "
                              f"[pages, heads, page_size, {HEAD_DIM}]")
+    shape, dtype = k_cache.shape, k_cache.dtype
     if v_cache.shape != shape or v_cache.dtype is not dtype:
         raise ValueError("k_cache and v_cache must have the same shape and type")
     pages, Hkv, P, _ = shape

@@ -187,6 +187,39 @@ def test_append_of_zeros_and_tiny_values():
         assert torch.equal(ks.cpu().nan_to_num(-1), torch.from_numpy(want[1]).nan_to_num(-1))
 
 
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("size", [2.0 ** -100, 2.0 ** -62, 2.0 ** -55, 1.0, 2.0 ** 64, 2.0 ** 120])
+def test_codes_are_those_of_the_quotients(code, size):
+    """Values at and beside the halves between codes, zeros of both signs, over the range of fp32's scales."""
+    g = torch.Generator().manual_seed(3)
+    T, m = 48, 127 if code == "int8" else 448
+    x = torch.randn((T, 1, 128), generator=g)
+    top = x.abs().amax()
+    x[:, :, 1::4] = top / 2 ** torch.randint(0, 14, (T, 1, 32), generator=g)
+    x[:, :, 2::4] = top * (torch.randint(-m, m, (T, 1, 32), generator=g) + 0.5) / m
+    x[::3, :, 3] = 0.0
+    x[1::3, :, 3] = -0.0
+    x = (x * size).to(torch.bfloat16)
+    table, pages = ref.tables([T], 16)
+    kc, vc, ks, vs = ref.empty_cache(pages, 1, 16, code)
+    for n, part in ((7, x[:7]), (10, x[7:10]), (T, x[10:])):  # the last part grows a page's scale
+        d = (part * (1.0 if n == T else 0.25)).cuda()
+        cu = [0, part.shape[0]]
+        want = [ref.append(y, c, s, table, [n], cu, code) for y, c, s in ((d, kc, ks), (-d, vc, vs))]
+        gdn.cache_append.kernel(d, -d, kc, vc, ks, vs, table, _i32([n]), _i32(cu))
+        for (raw, sc), c, s in zip(want, (kc, vc), (ks, vs)):
+            assert torch.equal(s.cpu().nan_to_num(-1), torch.from_numpy(sc).nan_to_num(-1))
+            assert torch.equal(c.view(torch.uint8).cpu(), torch.from_numpy(raw))
+
+
+@pytest.mark.parametrize("lens", [[1] * 2500, [40, 0, 200] * 30, [33] * 40])
+def test_append_to_many_sequences(lens):
+    """Searches of several rounds; one warp a page, whose rows need several turns, and a warp for each 16 rows."""
+    f = Filled(lens, 3, 64, "e4m3", more=[0] * len(lens))
+    q = f.q(1, 3)
+    f.check(q, gdn.cache_attend.run(q, *f.args(), f.seq, SCALE))
+
+
 def test_padded_rows_and_bad_pages_drop_their_rows():
     """seq_lens 0 with a row given, a table too short, pages outside the cache: dropped, the rest is as ever."""
     table, pages = ref.tables([40, 40, 40, 40], 16)

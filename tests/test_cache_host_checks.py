@@ -28,7 +28,7 @@ def _attend(lib, code=0, pages=4, P=16, max_pages=2, B=1, Q=1, Hq=4, Hkv=2, D=12
 
 @pytest.mark.parametrize("call", [_append, _attend])
 def test_cache_status_codes(lib, call):
-    assert call(lib, D=64) == 2 and call(lib, Hkv=0) == 2
+    assert call(lib, D=64) == 2 and call(lib, Hkv=0) == 2 and call(lib, Hkv=32768) == 2
     for kw in (dict(code=2), dict(P=8), dict(P=48), dict(P=256), dict(pages=-1), dict(max_pages=-1), dict(B=-1), dict(len64=2),
                dict(flags=1), dict(max_pages=1 << 28)):
         assert call(lib, **kw) == 4, kw

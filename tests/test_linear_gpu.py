@@ -226,3 +226,31 @@ def test_refusals():
     with pytest.raises(ValueError, match="must be \\["):
         Dc.run(q, k, v, st, a, SCALE)
     assert _lib.load().gdn_version() >= 100
+
+
+@pytest.mark.parametrize("lens", [[700] * 17, [1100] * 3, [64, 1500] * 4, [1] * 3000, [0] * 50 + [2100]])
+def test_many_and_equal_segments(lens):
+    """Batches whose segments all stay whole beside ones that are cut, and searches over many sequences."""
+    x = ref.inputs(lens, 1, 2, seed=len(lens))
+    out, ns = _run(x)
+    ref.check(out, ns, ref.reference(*x, SCALE), chunked=True)
+
+
+def test_one_graph_for_other_lengths():
+    """cu_seqlens may change between replays: one long sequence, two, and a short one beside a long one."""
+    x = ref.inputs([3000, 0], seed=11)
+    q, k, v, st, a, cu = x
+    c, out, ns = _cu(cu), torch.empty_like(v), torch.empty_like(st)
+    ws = torch.empty(gdn.linear_prefill.workspace_bytes(2, 3000, q.shape[1], v.shape[1]), dtype=torch.uint8, device="cuda")
+    call = lambda: gdn.linear_prefill.kernel(q, k, v, st, a, c, SCALE, out, ns, workspace=ws)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for ends in ([0, 1500, 3000], [0, 3000, 3000], [0, 100, 3000], [0, 500, 1000]):
+        c.copy_(_cu(ends))
+        graph.replay()
+        want = ref.reference(q, k, v, st, a, ends, SCALE)
+        ref.check(out[:ends[-1]], ns, [w[:ends[-1]] if i in (0, 2) else w for i, w in enumerate(want)], chunked=True)
+        assert gdn.linear_prefill.read_status(ws) == 0
