@@ -39,7 +39,7 @@ def _launch(dev, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, s
     s = scale if type(scale) is float and scale != 0.0 else resolve_scale(scale)
     q_ = as_dev(q, torch.bfloat16, dev)
     if output is None:
-        output = torch.empty(qs, dtype=torch.bfloat16, device=dev)
+        output = torch.empty_like(q_)
     elif not out_ok(output, dev, torch.bfloat16, q.numel()) or output.data_ptr() % 16:
         raise ValueError(f"output must be a contiguous, 16-byte aligned bf16 CUDA tensor with {q.numel()} elements")
     lib = _lib.load()

@@ -41,8 +41,8 @@ def _launch(dev, q, k, v, state, log_decay, cu_seqlens, scale, output, new_state
             raise ValueError(f"state must be [N, {HV}, 128, 128], got {tuple(state.shape)}")
         st = as_dev(state, torch.float32, dev)
     if output is None:
-        output = torch.empty(vs, dtype=torch.bfloat16, device=dev)
-        new_state = torch.empty((N, HV, V, K), dtype=torch.float32, device=dev)
+        output = torch.empty_like(v_)
+        new_state = torch.empty((N, HV, V, K), dtype=torch.float32, device=dev) if st is None else torch.empty_like(st)
     else:
         if not out_ok(output, dev, torch.bfloat16, T * HV * V) or output.data_ptr() % 16:
             raise ValueError(f"output must be a contiguous, 16-byte aligned bf16 CUDA tensor with {T * HV * V} elements")
