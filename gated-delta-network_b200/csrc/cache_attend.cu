@@ -25,7 +25,7 @@
 //    blocks on one line, an equal stretch of it per CTA. A stretch's first and last segment may continue in a
 //    neighbour; those pieces go to the workspace, and a second launch joins them.
 // 8 kv heads, e4m3: 64 x 4096 tokens with 4 rows a head 95 us (5.65 TB/s); 16 rows (64 x 2048) 78 us and 32 rows 121 us,
-// where the products and conversions bound it; 1 x 1000 tokens 13 us, most of it the two launches and what a CTA waits
+// where the products and conversions bound it; 1 x 1000 tokens 9.8 us, most of it the two launches and what a CTA waits
 // for in turn.
 #include <cuda_fp16.h>
 
@@ -40,9 +40,9 @@ constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kBlock = 32;                       // tokens of the unit that is divided over the CTAs
 constexpr int kStages = 3;
 constexpr int kStageBytes = 4096;                // a warp's 16 tokens of k and of v, rows of 128 bytes, SWIZZLE_128B
-// Places of a segment on the line besides its blocks (24 of 17 to 6000 tokens, 16 rows: 37 us; with 4 places 45), and the
-// blocks up to which one is not cut (32 x 512 tokens: 15 us, cut 18; that ragged batch would take 34 with every cut).
-constexpr int kOwn = 16, kKeep = 16;
+// Places of a segment on the line besides its blocks (24 of 17 to 6000 tokens, 16 rows: 33 us; with 8 places 36.5, with 16
+// 37), and the blocks up to which one is not cut (8 and 32 x 512 tokens: 11.5 and 15 us, cut 14.5 and 18).
+constexpr int kOwn = 12, kKeep = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 4.f;                    // scores may exceed the reference by this (base 2)
 // Shared memory for tiles of 8 NT rows: the ring, whose place the warps' results take; q as B fragments
@@ -122,7 +122,8 @@ __device__ __forceinline__ void find_stretch(const CacheArgs& c, int segs, Stret
         if (lane >= off) x += y;
     }
     const int total = __shfl_sync(0xffffffffu, x, 31) * segs;
-    const int ctas = max(1, min((int)gridDim.x, total / (kOwn + kWarps))), per = total / ctas, more = total - per * ctas;
+    // Stretches of 24 places at least, or of 8 while there are at most 64: 1 x 1000 tokens 9.8 us, with 24 there too 13.0.
+    const int ctas = max(1, min((int)gridDim.x, max(total / 24, min(total / 8, 64)))), per = total / ctas, more = total - per * ctas;
     if (lane == 0) {
         out->total = total;
         out->ctas = ctas;
