@@ -40,9 +40,10 @@ constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kBlock = 32;                       // tokens of the unit that is divided over the CTAs
 constexpr int kStages = 3;
 constexpr int kStageBytes = 4096;                // a warp's 16 tokens of k and of v, rows of 128 bytes, SWIZZLE_128B
-// Places of a segment on the line besides its blocks (24 of 17 to 6000 tokens, 16 rows: 33 us; with 8 places 36.5, with 16
-// 37), and the blocks up to which one is not cut (8 and 32 x 512 tokens: 11.5 and 15 us, cut 14.5 and 18).
-constexpr int kOwn = 12, kKeep = 16;
+// Places of a segment on the line besides its blocks (40 of 100 to 30000 tokens, 32 rows: 60 us, with 12 places 68, with 24
+// 57; 128 of 17 to 4000, 4 rows: 60, with 4 places 86, with 24 67).  The blocks up to which one is not cut (64 of 50 to 2000
+// tokens, 16 rows: 42 us, with 16 blocks 44), or if none is longer (8 and 32 x 512 tokens: 11.5 and 15 us, cut 14.5 and 18).
+constexpr int kOwn = 16, kKeep = 8, kWhole = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 4.f;                    // scores may exceed the reference by this (base 2)
 // Shared memory for tiles of 8 NT rows: the ring, whose place the warps' results take; q as B fragments
@@ -112,9 +113,14 @@ struct Stretch {
 __device__ __forceinline__ void find_stretch(const CacheArgs& c, int segs, Stretch* out) {
     using namespace att;
     const int lane = threadIdx.x & 31, part = (c.B + 31) / 32, b0 = min(c.B, lane * part), b1 = min(c.B, b0 + part);
-    int mine = 0;
+    int mine = 0, longest = 0;
 #pragma unroll 4
-    for (int b = b0; b < b1; ++b) mine += seq_blocks(c, b) + kOwn;
+    for (int b = b0; b < b1; ++b) {
+        const int nb = seq_blocks(c, b);
+        mine += nb + kOwn;
+        longest = max(longest, nb);
+    }
+    const int keep = __reduce_max_sync(0xffffffffu, longest) <= kWhole ? kWhole : kKeep;
     int x = mine;
 #pragma unroll 1
     for (int off = 1; off < 32; off <<= 1) {
@@ -143,7 +149,7 @@ __device__ __forceinline__ void find_stretch(const CacheArgs& c, int segs, Stret
         }
         AttMark r{b, (want - lo) / w, 0, lo};
         const int place = want - lo - r.seg * w - kOwn;
-        if (w - kOwn > kKeep) {
+        if (w - kOwn > keep) {
             r.block = max(0, place);
         } else if (2 * place >= w - kOwn && ++r.seg == segs) {  // a short segment is not cut: to its nearer end
             r = AttMark{b + 1, 0, 0, lo + w * segs};
