@@ -57,7 +57,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColQK = 0, kColI = 64, kColA = 128, kColS = 192, kColB = 320, kColV = 384;
 static_assert(kSmem <= 227 * 1024, "shared memory");
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718f;
 // Log decays are clamped here: e^-110 is below every fp32 number, and -infinity would turn the differences
 // of prefix sums into NaN.
 constexpr float kMinDecay = -110.f;
@@ -360,7 +360,7 @@ __device__ __forceinline__ bool role_load(const LinearPrefillArgs& p, const Line
 // Warp 2: prefix and suffix sums of every chunk's log decays (base 2 from here on), two tokens a lane.  The state in TMEM
 // is S 2^-X: as long as -8 <= X <= 8 a chunk's decay only moves X (its own tokens enter times 2^-(G_j + X)), so the state
 // is not touched; beyond that it is multiplied by 2^(X + G_C) and X is 0 again.  The exponents stay small, so fp32 holds
-// them to 2^-21.
+// them to 2^-21; what the sums X drop is carried along, since it would add up over the chunks.
 __device__ __forceinline__ bool role_gates(const LinearPrefillArgs& p, const LinCtx& x) {
     using namespace lin;
     const int lane = threadIdx.x & 31;
@@ -370,7 +370,7 @@ __device__ __forceinline__ bool role_gates(const LinearPrefillArgs& p, const Lin
 #pragma unroll 1
     while (w.next(p, pc)) {
         if (pc.e <= pc.s) continue;
-        float X = 0.f;
+        float X = 0.f, rest = 0.f;  // X, and what its sum has rounded away
 #pragma unroll 1
         for (int c = pc.ca; c < pc.cb; ++c, ++g) {
             const int t0 = pc.s + c * C, L = min(C, pc.e - t0);
@@ -398,13 +398,18 @@ __device__ __forceinline__ bool role_gates(const LinearPrefillArgs& p, const Lin
             *reinterpret_cast<float2*>(gt + 64 + 2 * lane) = make_float2(p.scale * lin_ex2(g0 + X), p.scale * lin_ex2(pre + X));
             // 2^(G_C - G_j) from the sum of the later decays: exact where it matters, near the chunk's end
             *reinterpret_cast<float2*>(gt + 128 + 2 * lane) =
-                scale ? make_float2(lin_ex2(after + a1), lin_ex2(after)) : make_float2(lin_ex2(-(g0 + X)), lin_ex2(-(pre + X)));
+                scale ? make_float2(lin_ex2(after + a1), lin_ex2(after))
+                      : make_float2(lin_ex2(-(g0 + X)) * (1.f - kLn2 * rest), lin_ex2(-(pre + X)) * (1.f - kLn2 * rest));
             *reinterpret_cast<float2*>(gt + 192 + 2 * lane) = make_float2(lin_ex2(gb - g0), lin_ex2(gb - pre));
-            if (lane == 0) gt[256] = scale ? exp2f(X + total) : 1.f;  // what the state is multiplied by
-            X = scale ? 0.f : X + total;
+            const float sum = X + total, added = sum - X;
+            rest += (X - (sum - added)) + (total - added);
+            const float unit = exp2f(sum) * (1.f + kLn2 * rest);
+            X = scale ? 0.f : sum;
+            if (scale) rest = 0.f;
             if (lane == 0) {
-                gt[257] = exp2f(X);        // of the state at the chunk's end
-                gt[258] = total;           // the chunk's decay, as its logarithm
+                gt[256] = scale ? unit : 1.f;  // what the state is multiplied by
+                gt[257] = scale ? 1.f : unit;  // of the state at the chunk's end
+                gt[258] = total;               // the chunk's decay, as its logarithm
                 gt[259] = scale ? 1.f : 0.f;
             }
             __syncwarp();
