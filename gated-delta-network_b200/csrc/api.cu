@@ -234,7 +234,13 @@ int gdn_linear_prefill_fwd(const void* q, const void* k, const void* v, const fl
     if (N < 0 || T < 0 || (decay_per_token != 0 && decay_per_token != 1) || (cu_is_int64 != 0 && cu_is_int64 != 1) ||
         (flags & ~GDN_FLAG_ZERO_UNOWNED))
         return GDN_ERR_SIZE;
-    if (N == 0) return GDN_OK;
+    if (N == 0) {  // every token is outside
+        if (T == 0 || !(flags & GDN_FLAG_ZERO_UNOWNED)) return GDN_OK;
+        if (!out) return GDN_ERR_NULL;
+        const int rc = check_device();
+        if (rc != GDN_OK) return rc;
+        return cudaMemsetAsync(out, 0, (size_t)T * HV * V * 2, static_cast<cudaStream_t>(stream)) == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
+    }
     if (!cu_seqlens || !new_state) return GDN_ERR_NULL;
     if (T > 0 && (!q || !k || !v || !log_decay || !out)) return GDN_ERR_NULL;
     if ((T > 0 && (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))) || !aligned16(new_state) ||

@@ -882,10 +882,9 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     }
     pdl_wait();
     pdl_trigger();
-    if (blockIdx.x == 0) {
-        if (tid == 0 && (!kOut || !p.cut)) *p.status = 0;  // the call's first launch
-        if (kOut && p.zero_unowned) zero_rows(p, tid, kThreads);
-    }
+    if (blockIdx.x == 0 && tid == 0 && (!kOut || !p.cut)) *p.status = 0;  // the call's first launch
+    if (kOut && p.zero_unowned && warp >= 2)  // beside find_range
+        zero_rows(p, blockIdx.x * (kThreads - 64) + tid - 64, gridDim.x * (kThreads - 64));
     if (warp == 0) find_range(p, range);
     if (warp == 1) tmem_alloc(&b->tmem, kTmemCols);
     if (kOut) {  // P above its diagonal

@@ -254,3 +254,21 @@ def test_one_graph_for_other_lengths():
         want = ref.reference(q, k, v, st, a, ends, SCALE)
         ref.check(out[:ends[-1]], ns, [w[:ends[-1]] if i in (0, 2) else w for i, w in enumerate(want)], chunked=True)
         assert gdn.linear_prefill.read_status(ws) == 0
+
+
+@pytest.mark.parametrize("lens", [[], [0], [0, 0, 0]])
+def test_no_token_belongs_to_a_sequence(lens):
+    q, k, v, st, a, cu = ref.inputs(lens, tail=9)
+    junk = torch.full((1 << 16,), float("nan"), device="cuda")  # freed memory that is not zero
+    del junk
+    out, ns = _run((q, k, v, st, a, cu))
+    assert out.shape == v.shape and not out.any()
+    assert torch.equal(ns, st)
+
+
+def test_a_long_padded_tail_is_zeroed():
+    x = list(ref.inputs([100, 30], lead=5, tail=5000))
+    want = ref.reference(*x, SCALE)
+    out, ns = _run(x)
+    assert not out[:5].any() and not out[x[5][-1]:].any()
+    ref.check(out, ns, want, chunked=True)
