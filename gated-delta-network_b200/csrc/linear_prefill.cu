@@ -63,9 +63,10 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718f;
 constexpr float kMinDecay = -110.f;
 
 // A wait tells a phase from the one before it only, so whoever waits on a barrier must be needed for its next phase
-// but one: hence the pairs p_full and p_empty, whose sides run up to two chunks apart.
+// but one: hence the pairs p_full and p_empty, whose sides run up to two chunks apart.  v_full goes by the gates' slots:
+// the V warps of chunk g + 8 start when the gates of g + 8 are there, so after the outputs of g + 1 and the OA of g.
 struct Bars {
-    uint64_t full[kStages], empty[kStages], g_full[kGates], g_empty[kGates];
+    uint64_t full[kStages], empty[kStages], g_full[kGates], g_empty[kGates], v_full[kGates];
     uint64_t qk_full, qk_empty, u_ready, u_full, b_ready, i_full, p_full[2], p_empty[2], o_empty, o_full, done[2];
     uint32_t tmem;
 };
@@ -490,6 +491,7 @@ __device__ __forceinline__ bool role_mma(const LinearPrefillArgs& p, const LinCt
         }
         if (g >= 0) {
             LIN_WAIT(lin_bars()->p_full[g & 1], g >> 1);
+            LIN_WAIT(lin_bars()->v_full[g % kGates], g / kGates);  // no foreign rows in v: P is 0 there, but 0 NaN is NaN
             tc_fence_after();
             mma_ss<false>(one, x.tmem + kColA, d_v + st, pb, idesc_oa);
 #pragma unroll
@@ -594,7 +596,7 @@ __device__ __forceinline__ bool role_v(const LinearPrefillArgs& p, const LinCtx&
             unsigned char* st = lin_sm + s * kStage;
             if (L < C) {
                 // Rows behind the segment's end hold another sequence's tokens, or zeros.  They become zero in v and
-                // k, so whatever they hold cannot reach a product.
+                // k before OA (v_full) and U (u_ready) read them; QK may read either, its columns there are dropped.
                 for (int i = tid; i < (C - L) * 16; i += 256) {
                     const uint32_t off = (uint32_t)(L + (i >> 4)) * 128 + (i & 7) * 16;
                     *reinterpret_cast<uint4*>(st + kOffV + ((i >> 3) & 1) * 8192 + off) = make_uint4(0, 0, 0, 0);
@@ -603,6 +605,7 @@ __device__ __forceinline__ bool role_v(const LinearPrefillArgs& p, const LinCtx&
                 fence_async_smem();
                 named_bar_sync(1, 256);
             }
+            if (kOut && lane == 0) mbar_arrive(&lin_bars()->v_full[g % kGates]);
             uint32_t part[3][16];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {  // 16 V x 16 tokens, transposed
@@ -863,6 +866,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         for (int s = 0; s < kGates; ++s) {
             mbar_init(&b->g_full[s], 1);
             mbar_init(&b->g_empty[s], 4);
+            mbar_init(&b->v_full[s], 8);
         }
         mbar_init(&b->qk_full, 1);
         mbar_init(&b->qk_empty, 128);

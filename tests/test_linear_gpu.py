@@ -272,3 +272,22 @@ def test_a_long_padded_tail_is_zeroed():
     out, ns = _run(x)
     assert not out[:5].any() and not out[x[5][-1]:].any()
     ref.check(out, ns, want, chunked=True)
+
+
+@pytest.mark.parametrize("with_state", [False, True])
+def test_partial_chunks_beside_rows_that_are_not_finite(with_state):
+    """Every CTA begins with a chunk whose tile also holds a neighbour's tokens, all of them NaN or infinite."""
+    lens = [1 + 7 * i % 63 for i in range(600)]
+    x = list(ref.inputs(lens, 1, 1, seed=12, with_state=with_state, tail=64))
+    q, k, v, st, a, cu = x
+    want = ref.reference(*x, SCALE)
+    foreign = torch.ones(q.shape[0], dtype=torch.bool)
+    for n in range(0, len(lens), 2):
+        foreign[cu[n]:cu[n + 1]] = False
+    for t, junk in ((q, float("nan")), (k, float("inf")), (v, float("nan"))):
+        t[foreign.cuda()] = junk
+    v[cu[1]:cu[2]] = float("inf")
+    keep = (~foreign).cuda()
+    for _ in range(20):
+        out, ns = _run(x)
+        ref.check(out[keep], ns[::2], [want[0][keep], want[1][::2], want[2][keep], want[3][::2]], chunked=True)
