@@ -91,10 +91,12 @@ __device__ __forceinline__ int lin_chunks(int s, int e) { return max(0, (e - s +
 
 // The ends of the stretch of CTA blockIdx.x, by one warp: every lane sums up an equal part of the sequences.  A segment
 // takes its chunks and 2 more places for its state, which is 128 KB to the 48 of a chunk.  (Places are ints: the entry
-// point refuses calls of 2^31 chunks.)
+// point refuses calls that could have 2^31.  Overlapping sequences may claim more than it counted; then every stretch is
+// empty, and the status says so.)
 __device__ __forceinline__ void find_range(const LinearPrefillArgs& p, Mark* at) {
     const int lane = threadIdx.x & 31, part = (p.N + 31) / 32, n0 = min(p.N, lane * part), n1 = min(p.N, n0 + part);
-    int x = 0, lo = 0, total = 0, per = 0, more = 0, keep = 0;
+    long long x = 0;
+    int lo = 0, total = 0, per = 0, more = 0, keep = 0;
 #pragma unroll 1
     for (int round = 0; round < 2; ++round) {  // the sum of the lane's lengths, then the marks among them
         int s = n0 < n1 ? cu_at(p, n0) : 0;
@@ -123,16 +125,22 @@ __device__ __forceinline__ void find_range(const LinearPrefillArgs& p, Mark* at)
             lo += w * p.HV;
         }
         if (round == 0) {
-            const int mine = x;
+            const long long mine = x;
 #pragma unroll 1
             for (int off = 1; off < 32; off <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, off);
+                const long long y = __shfl_up_sync(0xffffffffu, x, off);
                 if (lane >= off) x += y;
+            }
+            const long long places = __shfl_sync(0xffffffffu, x, 31);
+            if (places > p.T / lin::C + 3ll * p.N) {
+                if (lane < 2) at[lane] = Mark{p.N, 0, 0};
+                if (blockIdx.x == 0 && lane == 0) atomicCAS(p.status, 0, kErrBadSeqlens);
+                return;
             }
             keep = __reduce_max_sync(0xffffffffu, keep);
             if (keep > p.whole) keep = p.keep;
-            lo = (x - mine) * p.HV;
-            total = __shfl_sync(0xffffffffu, x, 31) * p.HV;
+            lo = (int)(x - mine) * p.HV;
+            total = (int)places * p.HV;
             const int ctas = max(1, min(p.ctas, total / p.min_share)), c = blockIdx.x + lane;
             per = total / ctas;
             more = total - per * ctas;

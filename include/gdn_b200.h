@@ -213,7 +213,8 @@ int gdn_linear_decode_fwd(const void* q, const void* k, const void* v, const flo
  * state), and output rows of tokens outside every sequence are left as they were unless
  * GDN_FLAG_ZERO_UNOWNED (the only flag) is given.  new_state may be state itself.  The workspace
  * (256-byte aligned, at least gdn_linear_prefill_workspace_bytes) carries nothing between calls; its first
- * int receives 0 or the code of a bounded device-side wait that gave up.
+ * int receives 0 or a GDN_DEVSTATUS_* code: a bounded device-side wait that gave up, or BAD_SEQLENS where
+ * overlapping sequences claim more chunks than T tokens in N sequences can have; then no sequence is computed.
  */
 size_t gdn_linear_prefill_workspace_bytes(int N, int T, int H, int HV, int K, int V);
 int gdn_linear_prefill_fwd(const void* q, const void* k, const void* v, const float* state, const float* log_decay,

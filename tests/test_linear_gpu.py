@@ -291,3 +291,19 @@ def test_partial_chunks_beside_rows_that_are_not_finite(with_state):
     for _ in range(20):
         out, ns = _run(x)
         ref.check(out[keep], ns[::2], [want[0][keep], want[1][::2], want[2][keep], want[3][::2]], chunked=True)
+
+
+@pytest.mark.parametrize("N,T", [(3, 1200), (40, 2000), (65536, 1 << 22)])
+def test_sequences_that_overlap_too_much_are_reported(N, T):
+    """Every other sequence holds all tokens; the last size has 2^31 chunks.  Nothing is computed, in bounds and at once."""
+    q, k, v = (torch.zeros((T, 1, 128), dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    out = torch.full_like(v, 3.0)
+    ns = torch.empty((N, 1, 128, 128), device="cuda")
+    ns[-1] = 3.0
+    cu = torch.arange(N + 1, device="cuda") % 2 * T
+    ws = torch.empty(gdn.linear_prefill.workspace_bytes(N, T, 1, 1), dtype=torch.uint8, device="cuda")
+    gdn.linear_prefill.kernel(q, k, v, None, torch.zeros(1, device="cuda"), cu, SCALE, out, ns, workspace=ws)
+    assert gdn.linear_prefill.read_status(ws) == 5
+    assert (out[::997] == 3).all() and (ns[-1] == 3).all()
+    gdn.linear_prefill.kernel(q, k, v, None, torch.zeros(1, device="cuda"), cu[:2], SCALE, out, ns[:1], workspace=ws)
+    assert gdn.linear_prefill.read_status(ws) == 0 and not out.any() and not ns[0].any()
