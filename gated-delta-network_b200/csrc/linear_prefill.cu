@@ -719,7 +719,6 @@ __device__ __forceinline__ bool role_o(const LinearPrefillArgs& p, const LinearM
             LIN_CHECK();
         }
     }
-    if (r == 0) tma_store_wait_all();
     return true;
 }
 
@@ -939,6 +938,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         ok = role_v<kOut>(p, x);
     } else if (warp < 20) {
         if (kOut) ok = role_o(p, maps, x);
+        if (kOut && warp == 16) tma_store_wait_all();  // its first lane's stores, if a wait gave up too
     } else {
         ok = role_s<kOut>(p, x);
     }
