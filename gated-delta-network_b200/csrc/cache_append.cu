@@ -92,7 +92,7 @@ __device__ __forceinline__ float2 quotients(float2 x, float s, float r) {
 }
 __device__ __forceinline__ float reciprocal(float s) { return s > 0x1p-60f && s < 0x1p60f ? __frcp_rn(s) : 0.f; }
 // Eight bf16 values to codes.  r: reciprocal(s), or 0 where there is none or not all values are finite.
-// (s = 0: zeros, or values whose scale is below fp32.)
+// (s = 0: zeros, or values whose scale is below fp32; infinities and NaN among them keep their codes.)
 template <bool kInt8>
 __device__ __forceinline__ uint2 encode8(uint4 w, float s, float r) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -104,12 +104,13 @@ __device__ __forceinline__ uint2 encode8(uint4 w, float s, float r) {
         for (int e = 0; e < 4; ++e) x[e] = quotients(x[e], s, r);
         return make_uint2(encode4<kInt8, false>(x[0].x, x[0].y, x[1].x, x[1].y), encode4<kInt8, false>(x[2].x, x[2].y, x[3].x, x[3].y));
     }
-    uint2 y = make_uint2(0, 0);
-    if (s > 0.f) {
-        y.x = encode4<kInt8, true>(__fdiv_rn(x[0].x, s), __fdiv_rn(x[0].y, s), __fdiv_rn(x[1].x, s), __fdiv_rn(x[1].y, s));
-        y.y = encode4<kInt8, true>(__fdiv_rn(x[2].x, s), __fdiv_rn(x[2].y, s), __fdiv_rn(x[3].x, s), __fdiv_rn(x[3].y, s));
+    if (!(s > 0.f)) {
+        s = 1.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = make_float2(fabsf(x[e].x) < INFINITY ? 0.f : x[e].x, fabsf(x[e].y) < INFINITY ? 0.f : x[e].y);
     }
-    return y;
+    return make_uint2(encode4<kInt8, true>(__fdiv_rn(x[0].x, s), __fdiv_rn(x[0].y, s), __fdiv_rn(x[1].x, s), __fdiv_rn(x[1].y, s)),
+                      encode4<kInt8, true>(__fdiv_rn(x[2].x, s), __fdiv_rn(x[2].y, s), __fdiv_rn(x[3].x, s), __fdiv_rn(x[3].y, s)));
 }
 template <bool kInt8>
 __device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {

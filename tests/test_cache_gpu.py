@@ -378,3 +378,29 @@ def test_refusals():
         gdn.cache_attend.kernel(q, *f.args(), f.seq, SCALE, torch.empty_like(q), workspace=q)
     with pytest.raises(ValueError, match="k and v"):
         gdn.cache_append.kernel(q[0], q[0], *f.args()[:4], f.table, f.seq, _i32([0, 1]))
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_append_of_infinities_and_nan_among_zeros(code):
+    """The page's scale is 0 then; the codes are those of any other page, and stay when a later token brings a scale."""
+    table, pages = ref.tables([10], 16)
+    kc, vc, ks, vs = ref.empty_cache(pages, 1, 16, code)
+    x = torch.zeros((6, 1, 128), dtype=torch.bfloat16)
+    x[1, 0, 5], x[2, 0, 6], x[4, 0, 9], x[4, 0, 10] = float("inf"), float("-inf"), float("nan"), -0.0
+    big, nan = (127, 0) if code == "int8" else (0x7E, 0x7F)
+    minus = 129 if code == "int8" else 0xFE
+    gdn.cache_append.kernel(x.cuda(), -x.cuda(), kc, vc, ks, vs, table, _i32([6]), _i32([0, 6]))
+    page = table[0, 0].item()
+    for c, s, inf, ninf in ((kc, ks, big, minus), (vc, vs, minus, big)):
+        raw = c.view(torch.uint8)[page, 0, :6].cpu()
+        assert s[page, 0] == 0
+        assert raw[1, 5] == inf and raw[2, 6] == ninf
+        assert (raw[4, 9] & (0x7F if code == "e4m3" else 0xFF)) == nan
+        assert (raw.to(torch.int32) & 0x7F != 0).sum() == (3 if code == "e4m3" else 2)
+    y = torch.ones((1, 1, 128), dtype=torch.bfloat16).cuda()
+    gdn.cache_append.kernel(y, y, kc, vc, ks, vs, table, _i32([7]), _i32([0, 1]))
+    raw = kc.view(torch.uint8)[page, 0, :7].cpu().to(torch.int32) & 0x7F
+    assert ks[page, 0] > 0 and (raw[6] == big).all()
+    assert (raw[4, 9] == 0x7F) if code == "e4m3" else raw[4, 9] == 0
+    raw[4, 9] = 0
+    assert not raw[:6].any()  # an infinity kept no size: 0 times its code
