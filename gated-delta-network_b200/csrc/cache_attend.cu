@@ -15,6 +15,9 @@
 //    reduction and no rescaling; weights stay below 2^4 in fp16, their sum is fp32 and of the unrounded ones.
 //  * The value scale enters the weights: p v_scale / r with r the largest value scale so far, kept like the maximum,
 //    so the accumulator never sees the scales' range.  Weights round to 2^-11, or to 2^-25 r where they are below 2^-14.
+//  * A row is kept from what it does not see: 0 NaN is NaN, so in the steps that only some rows see all of, values that
+//    are not finite (the e4m3 code NaN, or any under such a scale) are left out, and a pass behind the loop, which ordinary
+//    data never takes, gives them to the rows that see them.
 //  * Both contractions may permute their index, so a thread takes 16 consecutive bytes of a row and no fragment
 //    needs a shuffle or a transposing load: key step s of lane l holds dims 32 (l % 4) + 4 s .. and the same of q;
 //    value lane l holds dims 16 (l / 4) .. of the four tokens whose weights it owns (after one 8 x 8 transpose).
@@ -90,6 +93,8 @@ __device__ __forceinline__ uint4 load_codes(const unsigned char* p) {
     if (kInt8) x = make_uint4(x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u);
     return x;
 }
+// Bytes of w that are the e4m3 code NaN, as 0xff.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 __device__ __forceinline__ uint32_t word(const uint4& x, int e) { return e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w; }
 
 __device__ __forceinline__ int visible_length(const CacheArgs& c, int b) {
@@ -331,13 +336,17 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
         // The scores of a step are formed beside the softmax and the second product of the one before: a warp has two
         // chains to work on.  (Those behind the last step are formed from whatever the ring holds, and not used.)
         float s[NT][4];
+        bool odd = false;  // values that are not finite were left out where not every row sees them
         if (mine > 0) arrived(place);
         scores(ring + place * kStageBytes, s);
 #pragma unroll 1
         for (int n = 0; n < mine; ++n) {
             const bool ok = (unsigned)pg0 < (unsigned)c.pages;
             if (!ok) s_status = kErrBadPage;
-            const float ks0 = ks, vs0 = ok ? vs : 0.f;
+            const int t = t_first + 16 * kWarps * n;
+            const bool some = t + 16 > all_see;  // not every row sees all of it
+            const float ks0 = ks;
+            float vs0 = ok ? vs : 0.f;
             pg0 = pg1;
             pg1 = pg2;
             pg2 = pg3;
@@ -345,19 +354,22 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
                 ks = c.k_scale[scale_at(pg0)];
                 vs = c.v_scale[scale_at(pg0)];
             }
-            const int t = t_first + 16 * kWarps * n;
             // scores in base 2; hidden ones are -infinity
             bool over = false;
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[j][e] *= ks0 * rf[j][e & 1];
-            if (t + 16 > all_see || !ok) {
+            if (some || !ok) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (!ok || t + (lane >> 2) + 8 * (e >> 1) >= lim[j][e & 1]) s[j][e] = -INFINITY;
+                if (!(vs0 < INFINITY)) {
+                    vs0 = 0.f;
+                    odd = true;
+                }
             }
 #pragma unroll
             for (int j = 0; j < NT; ++j)
@@ -404,15 +416,25 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
                 w0[j] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&x));
                 w1[j] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&y));
             }
+            // tokens 2 (lane % 4) + {0, 1} (+ 8), chunk lane / 4
+            auto v_at = [&](int i) { return ring + place * kStageBytes + 1024 * (i >> 1) + ((v_off + 128 * (i & 1)) ^ ((i & 1) << 4)); };
+            auto v_token = [&](int i) { return t + 2 * (lane & 3) + (i & 1) + 8 * (i >> 1); };
             uint4 v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)  // tokens 2 (lane % 4) + {0, 1} (+ 8), chunk lane / 4
-                v[i] = load_codes<kInt8>(ring + place * kStageBytes + 1024 * (i >> 1) + ((v_off + 128 * (i & 1)) ^ ((i & 1) << 4)));
+            for (int i = 0; i < 4; ++i) v[i] = load_codes<kInt8>(v_at(i));
             if (!ok || t + 16 > tok1) {  // slots behind the sequence's end hold anything: a weight of 0 does not undo a NaN
                 const uint32_t none = kInt8 ? 0x80808080u : 0u;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (!ok || t + 2 * (lane & 3) + (i & 1) + 8 * (i >> 1) >= tok1) v[i] = make_uint4(none, none, none, none);
+                    if (!ok || v_token(i) >= tok1) v[i] = make_uint4(none, none, none, none);
+            }
+            if (!kInt8 && some) {  // nor that of a token that some rows do not see: those that do get it after the loop
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint4 x = make_uint4(nan_codes(v[i].x), nan_codes(v[i].y), nan_codes(v[i].z), nan_codes(v[i].w));
+                    v[i] = make_uint4(v[i].x & ~x.x, v[i].y & ~x.y, v[i].z & ~x.z, v[i].w & ~x.w);
+                    odd |= (x.x | x.y | x.z | x.w) != 0;
+                }
             }
             __syncwarp();  // the step's place is read: the next one may land there
             issue(n + 3, place, pg2);
@@ -432,6 +454,54 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[j][e] = sn[j][e];
             place = next;
+        }
+
+        if (__any_sync(0xffffffffu, odd)) {
+            // A product of ones, in the places of those values and of the tokens that a row sees, finds the sums that become NaN.
+#pragma unroll 1
+            for (int n = 0; n < mine; ++n) {
+                const int t = t_first + 16 * kWarps * n, page = page_of(n);
+                if (t + 16 <= all_see || (unsigned)page >= (unsigned)c.pages) continue;
+                const bool all = !(c.v_scale[scale_at(page)] < INFINITY);
+                const uint32_t one = kInt8 ? 0x81818181u : 0x38383838u, none = kInt8 ? 0x80808080u : 0u;
+                uint4 v[4];  // the value's place, as in the loop above: one
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int tok = t + 2 * (lane & 3) + (i & 1) + 8 * (i >> 1);
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (!kInt8)
+                        x = *reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(c.v_cache) + 16 * (lane >> 2) +
+                                                            128 * ((((size_t)page * c.Hkv + h) << c.page_shift) + (tok & ((1 << c.page_shift) - 1))));
+                    auto mark = [&](uint32_t w) { return all ? one : kInt8 ? none : one & nan_codes(w); };
+                    v[i] = make_uint4(mark(x.x), mark(x.y), mark(x.z), mark(x.w));
+                }
+                uint32_t w0[NT], w1[NT];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    float e[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) e[i] = t + (lane >> 2) + 8 * (i >> 1) < lim[j][i & 1] ? 1.f : 0.f;
+                    const __half2 x = __floats2half2_rn(e[0], e[1]), y = __floats2half2_rn(e[2], e[3]);
+                    w0[j] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&x));
+                    w1[j] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&y));
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int d = 0; d < 2; ++d) {
+                        const uint32_t x = __byte_perm(word(v[0], e), word(v[1], e), d ? 0x7362 : 0x5140);
+                        const uint32_t y = __byte_perm(word(v[2], e), word(v[3], e), d ? 0x7362 : 0x5140);
+                        const uint32_t a[4] = {codes_f16<kInt8, false>(x), codes_f16<kInt8, true>(x), codes_f16<kInt8, false>(y), codes_f16<kInt8, true>(y)};
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            float hit[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma_f16(hit, a, w0[j], w1[j]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (hit[i] > 0.f) acc[j][2 * e + d][i] = NAN;
+                        }
+                    }
+            }
         }
 
         // join the warps: every warp's result at the common maximum

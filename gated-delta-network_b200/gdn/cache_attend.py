@@ -68,6 +68,7 @@ def run(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale):
     float8_e4m3fn, k_scale, v_scale [pages, Hkv] fp32 (see ``gdn.cache_append``), Hq a multiple of Hkv (q head h
     reads head h // (Hq // Hkv)); block_table [B, max_pages] int32 (int64 is converted); seq_lens [B] int32/int64,
     the Q tokens included.  Row i sees the positions below seq_len - Q + 1 + i; a row that sees none (a padded row
-    with seq_lens 0, say) is zero.  scale float, 0-d tensor, or None/0 (1/sqrt(128)).
+    with seq_lens 0, say) is zero.  What a row does not see cannot reach it, be it NaN; a NaN or infinite value that it
+    sees makes that dim of it NaN or infinite.  scale float, 0-d tensor, or None/0 (1/sqrt(128)).
     """
     return _launch(cuda_device(q, "q"), q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, None, None)

@@ -404,3 +404,48 @@ def test_append_of_infinities_and_nan_among_zeros(code):
     assert (raw[4, 9] == 0x7F) if code == "e4m3" else raw[4, 9] == 0
     raw[4, 9] = 0
     assert not raw[:6].any()  # an infinity kept no size: 0 times its code
+
+
+class Poked(Filled):
+    """A filled cache some of whose codes and value scales are then overwritten; `rows` that see none of them keep their values."""
+
+    def poke(self, b, token, head, dim, raw):
+        P = self.vc.shape[2]
+        self.vc.view(torch.uint8)[self.table[b, token // P].item(), head, token % P, dim] = raw
+
+    def check_apart(self, q, clean, tol, dirty):
+        """NaN (or infinite) exactly where `dirty` is, elsewhere as before the pokes."""
+        out = gdn.cache_attend.run(q, *self.args(), self.seq, SCALE).double()
+        hit = ~torch.isfinite(dirty)
+        assert torch.equal(~torch.isfinite(out), hit)
+        assert hit.any() and (((out - clean).abs() <= tol) | hit).all()
+
+
+@pytest.mark.parametrize("Q,Hq,Hkv", [(2, 2, 2), (4, 8, 2), (3, 5, 1), (16, 8, 1), (33, 2, 1)])
+@pytest.mark.parametrize("P", [16, 64])
+def test_nan_in_v_reaches_only_rows_that_see_it(Q, Hq, Hkv, P):
+    """e4m3 has a code for NaN: a later token's must not reach earlier rows, nor one that sees no token at all."""
+    lens = [Q + 38, 3, 1, 500, 2, Q + 9]
+    f = Poked(lens, Hkv, P, "e4m3", seed=Q, more=[0] * len(lens))
+    q = f.q(Q, Hq)
+    clean, tol = ref.attend(q, *f.args(), f.lens, SCALE)
+    for b, n in enumerate(lens[:-1]):  # the last sequence stays clean
+        f.poke(b, n - 1, Hkv - 1, 5, 0x7F)
+        if n > 2:
+            f.poke(b, n - 2, 0, 77, 0xFF)
+            f.poke(b, n - 2, 0, slice(96, 128), 0x7F)
+    f.poke(3, 100, Hkv - 1, 127, 0x7F)
+    f.check_apart(q, clean, tol, ref.attend(q, *f.args(), f.lens, SCALE)[0])
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("Q", [2, 4, 20])
+def test_value_scale_that_is_not_finite_reaches_only_rows_that_see_its_page(code, bad, Q):
+    lens = [33, 65, 17]  # the last token begins a page
+    f = Poked(lens, 1, 16, code, more=[0] * 3)
+    f.vc.view(torch.uint8)[f.table[0, 2].item(), :, 0] = 0x11
+    q = f.q(Q, 3)
+    clean, tol = ref.attend(q, *f.args(), f.lens, SCALE)
+    f.vs[f.table[0, 2].item()] = bad
+    f.check_apart(q, clean, tol, ref.attend(q, *f.args(), f.lens, SCALE)[0])
