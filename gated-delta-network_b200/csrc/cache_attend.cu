@@ -13,8 +13,10 @@
 //    2^-25 of it), and the page's key scale multiplies the fp32 scores.
 //  * The maximum is a reference that moves only when a score exceeds it by 4 (base 2), so most steps need no
 //    reduction and no rescaling; weights stay below 2^4 in fp16, their sum is fp32 and of the unrounded ones.
-//  * The value scale enters the weights: p v_scale / r with r the largest value scale so far, kept like the maximum,
-//    so the accumulator never sees the scales' range.  Weights round to 2^-11, or to 2^-25 r where they are below 2^-14.
+//  * The value scale enters the weights, p v_scale / r, so the accumulator never sees the scales' range.  r is a power of
+//    two for each row, at most its largest p v_scale so far and some 9 bits below it at worst, and moves like the maximum.
+//    (Of the weights, not of the scales: a page of large values that has no weight must not cost the others their bits.)
+//    Weights round to 2^-11, or to 2^-25 r where they are below 2^-14 r.
 //  * A row is kept from what it does not see: 0 NaN is NaN, so in the steps that only some rows see all of, values that
 //    are not finite (the e4m3 code NaN, or any under such a scale) are left out, and a pass behind the loop, which ordinary
 //    data never takes, gives them to the rows that see them.
@@ -49,6 +51,7 @@ constexpr int kStageBytes = 4096;                // a warp's 16 tokens of k and 
 constexpr int kOwn = 16, kKeep = 8, kWhole = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 4.f;                    // scores may exceed the reference by this (base 2)
+constexpr float kRoom = 16.f;                    // value scales may exceed a row's r times this much
 // Shared memory for tiles of 8 NT rows: the ring, whose place the warps' results take; q as B fragments
 // [NT][8 steps][32 lanes][8 bytes]; f32 [8 NT] row factors; f32 [kWarps][8 NT] references, then sums; the ring's barriers.
 template <int NT>
@@ -93,6 +96,8 @@ __device__ __forceinline__ uint4 load_codes(const unsigned char* p) {
     if (kInt8) x = make_uint4(x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u);
     return x;
 }
+// 1 / x for a power of two.
+__device__ __forceinline__ float power2(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
 // Bytes of w that are the e4m3 code NaN, as 0xff.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 __device__ __forceinline__ uint32_t word(const uint4& x, int e) { return e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w; }
@@ -280,7 +285,8 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
         __syncthreads();
 
         // this thread's q rows of column tile j: row0 + 8 j + 2 (lane % 4) and the next
-        float acc[NT][8][4], m[NT][2], l[NT][2], rf[NT][2], vref = 0.f;
+        float acc[NT][8][4], m[NT][2], l[NT][2], rf[NT][2];
+        float inv[NT][2], vmax = 0.f;  // 1 / r; the largest value scale that none of these r has to move for
         int lim[NT][2];  // positions that the rows see
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -294,6 +300,7 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
                 m[j][r] = -INFINITY;
                 l[j][r] = 0.f;
                 rf[j][r] = s_f[row];
+                inv[j][r] = 0x1p120f;
                 lim[j][r] = len - p.Q + 1 + (row0 + row) / G;
             }
         }
@@ -375,30 +382,32 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) over |= s[j][e] > m[j][e & 1] + kSlack;
-            const float vnew = fmaxf(vref, vs0);
-            if (__any_sync(0xffffffffu, over) || vnew > vref) {
-                const float vr = vnew > 0.f ? vref / vnew : 1.f;
-                vref = vnew;
+            if (__any_sync(0xffffffffu, over || vs0 > vmax)) {
+                vmax = INFINITY;
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        float top = fmaxf(s[j][r], s[j][2 + r]);
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                        top = fmaxf(top, m[j][r]);
+                        float here = fmaxf(s[j][r], s[j][2 + r]);  // the step's maximum
+                        here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, 4));
+                        here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, 8));
+                        here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, 16));
+                        const float top = fmaxf(here, m[j][r]);
                         const float f = m[j][r] == -INFINITY ? 0.f : ex2(m[j][r] - top);
                         m[j][r] = top;
                         l[j][r] *= f;
+                        // r follows the maximum, or the step's largest weight (kept within what r and 1 / r can both hold)
+                        const float old = f * power2(inv[j][r]), now = here == -INFINITY ? 0.f : ex2(here - top) * vs0;
+                        const int ex = min(max((int)(__float_as_uint(fmaxf(old, now)) >> 23), 7), 247);
+                        inv[j][r] = __uint_as_float((uint32_t)(254 - ex) << 23);
+                        vmax = fminf(vmax, kRoom * __uint_as_float((uint32_t)ex << 23));
 #pragma unroll
                         for (int d = 0; d < 8; ++d) {
-                            acc[j][d][r] *= f * vr;
-                            acc[j][d][2 + r] *= f * vr;
+                            acc[j][d][r] *= old * inv[j][r];
+                            acc[j][d][2 + r] *= old * inv[j][r];
                         }
                     }
             }
-            const float mv = vref > 0.f ? vs0 / vref : 0.f;
             const int next = after(place);
             if (n + 1 < mine) arrived(next);
             float sn[NT][4];
@@ -412,7 +421,9 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
                     e[i] = ex2(s[j][i] - (m[j][i & 1] == -INFINITY ? 0.f : m[j][i & 1]));
                     l[j][i & 1] += e[i];
                 }
-                const __half2 x = __floats2half2_rn(e[0] * mv, e[1] * mv), y = __floats2half2_rn(e[2] * mv, e[3] * mv);
+                const float2 in = make_float2(inv[j][0], inv[j][1]), vv = make_float2(vs0, vs0);
+                const float2 e0 = mul2(mul2(make_float2(e[0], e[1]), vv), in), e1 = mul2(mul2(make_float2(e[2], e[3]), vv), in);
+                const __half2 x = __floats2half2_rn(e0.x, e0.y), y = __floats2half2_rn(e1.x, e1.y);
                 w0[j] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&x));
                 w1[j] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&y));
             }
@@ -526,7 +537,7 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
                 float mall = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) mall = fmaxf(mall, s_m[w * kRows + row]);
-                const float f = l[j][r] != 0.f ? ex2(m[j][r] - mall) * vref : 0.f;  // a NaN stays one
+                const float f = l[j][r] != 0.f ? ex2(m[j][r] - mall) * power2(inv[j][r]) : 0.f;  // a NaN stays one
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     *reinterpret_cast<float4*>(wacc + (warp * kRows + row) * 128 + ((4 * (lane >> 2) + e) ^ (row & 7)) * 4) =

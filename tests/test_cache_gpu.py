@@ -449,3 +449,36 @@ def test_value_scale_that_is_not_finite_reaches_only_rows_that_see_its_page(code
     clean, tol = ref.attend(q, *f.args(), f.lens, SCALE)
     f.vs[f.table[0, 2].item()] = bad
     f.check_apart(q, clean, tol, ref.attend(q, *f.args(), f.lens, SCALE)[0])
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("ratio", [2.0 ** -100, 2.0 ** -20, 2.0 ** 12, 2.0 ** 17, 2.0 ** 30, 2.0 ** 45])
+@pytest.mark.parametrize("Q,page", [(1, 0), (1, 150), (3, 7), (8, 255)])
+def test_a_page_of_other_size_and_little_weight(code, ratio, Q, page):
+    """Values `ratio` times as large in one page, whose scores are 2^-60 below the others': it must not cost the others
+    their bits.  The bound is cache_ref's, but weights below fp16's normal range are measured by the row's largest
+    weight times value scale, 2^-25 of it each, instead of the largest value in the cache."""
+    n, P, Hq = 4096, 16, 4
+    table, pages = ref.tables([n], P)
+    kc, vc, ks, vs = ref.empty_cache(pages, 1, P, code)
+    g = torch.Generator().manual_seed(7)
+    k, v = (torch.randn((n, 1, 128), generator=g) for _ in range(2))
+    q = (torch.randn((1, Q, Hq, 128), generator=g) * 0.1 + 1).to(torch.bfloat16).cuda()
+    at = slice(page * P, (page + 1) * P)
+    k[at] = k[at] * 0.1 - 60 * 0.69315 / SCALE / 128
+    v[at] *= ratio
+    gdn.cache_append.kernel(k.to(torch.bfloat16).cuda(), v.to(torch.bfloat16).cuda(), kc, vc, ks, vs, table, _i32([n]), _i32([0, n]))
+    out = gdn.cache_attend.run(q, kc, vc, ks, vs, table, _i32([n]), SCALE).double()
+    idx = table[0].long()
+    K, V = ((c.view(torch.uint8)[idx, 0].view(c.dtype).double() * s[idx, 0].double()[:, None, None]).reshape(-1, 128) for c, s in ((kc, ks), (vc, vs)))
+    size = vs[idx, 0].double().repeat_interleave(P) * (127 if code == "int8" else 448)
+    for i in range(Q):
+        m = n - Q + 1 + i
+        qq = q[0, i].double()
+        s = SCALE * (qq @ K[:m].T)
+        d = SCALE * (2.0 ** -17 * (qq.abs() @ K[:m].abs().T) + 2.0 ** -24 * qq.abs().amax(-1, keepdim=True) * K[:m].abs().sum(-1)) + 2.0 ** -21 * s.abs()
+        w = torch.softmax(s, -1)
+        o = w @ V[:m]
+        tol = 2.0 ** -8 * o.abs() + (2.0 ** -10 + 2 * d.amax(-1, keepdim=True)) * (w @ V[:m].abs()) + m * 2.0 ** -25 * (w * size[:m]).amax(-1, keepdim=True)
+        e = (out[0, i] - o).abs()
+        assert (e <= tol).all(), f"row {i} off by {(e / tol).max().item():.2f} times its bound"
