@@ -49,15 +49,17 @@ constexpr int kStageBytes = 4096;                // a warp's 16 tokens of k and 
 // 57; 128 of 17 to 4000, 4 rows: 60, with 4 places 86, with 24 67).  The blocks up to which one is not cut (64 of 50 to 2000
 // tokens, 16 rows: 42 us, with 16 blocks 44), or if none is longer (8 and 32 x 512 tokens: 11.5 and 15 us, cut 14.5 and 18).
 constexpr int kOwn = 16, kKeep = 8, kWhole = 16;
+constexpr int kTooLong = 1, kNoPage = 2, kLate = 4;  // what a CTA has met; the gravest of all CTAs' becomes the call's status
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 4.f;                    // scores may exceed the reference by this (base 2)
 constexpr float kRoom = 16.f;                    // value scales may exceed a row's r times this much
 // Shared memory for tiles of 8 NT rows: the ring, whose place the warps' results take; q as B fragments
-// [NT][8 steps][32 lanes][8 bytes]; f32 [8 NT] row factors; f32 [kWarps][8 NT] references, then sums; the ring's barriers.
+// [NT][8 steps][32 lanes][8 bytes]; f32 [8 NT] row factors, int [8 NT] positions that the rows see; f32 [kWarps][8 NT]
+// references, then sums; the ring's barriers.
 template <int NT>
 struct Smem {
     static constexpr int kRing = kWarps * kStages * kStageBytes, kJoin = kWarps * 8 * NT * 128 * 4;
-    static constexpr int kOffQ = kRing > kJoin ? kRing : kJoin, kOffF = kOffQ + NT * 2048, kOffM = kOffF + NT * 32;
+    static constexpr int kOffQ = kRing > kJoin ? kRing : kJoin, kOffF = kOffQ + NT * 2048, kOffM = kOffF + NT * 64;
     static constexpr int kOffBar = kOffM + 2 * kWarps * 8 * NT * 4, kSize = kOffBar + kWarps * kStages * 8;
 };
 }  // namespace att
@@ -189,9 +191,10 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
     const CacheArgs& c = p.c;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     float* s_f = reinterpret_cast<float*>(att_sm + S::kOffF);
+    int* s_lim = reinterpret_cast<int*>(s_f + kRows);
     float* s_m = reinterpret_cast<float*>(att_sm + S::kOffM);
     float* s_l = s_m + kWarps * kRows;
-    if (tid == 0) s_status = (smem_u32(att_sm) & 1023u) ? kErrScanTmaTimeout : 0;  // (the swizzled tiles need the alignment)
+    if (tid == 0) s_status = (smem_u32(att_sm) & 1023u) ? kLate : 0;  // (the swizzled tiles need the alignment)
     uint64_t* bars = reinterpret_cast<uint64_t*>(att_sm + S::kOffBar) + warp * kStages;
     if (lane == 0) {
         for (int i = 0; i < kStages; ++i) mbar_init(bars + i, 1);
@@ -206,19 +209,20 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
     const Stretch line = s_line;
     int2 piece = make_int2(-1, 0);  // the segment that begins here and ends elsewhere (thread 0)
     int place = 0;                  // ring place of the next step to read
-    uint32_t phases = 0;            // and the phases of the ring's barriers
+    uint32_t phases = 0;            // and the phases of the ring's barriers; above them kGaveUp
+    constexpr uint32_t kGaveUp = 1u << 31;  // a wait did: the warp takes no more steps
 
 #pragma unroll 1
     for (AttMark at = line.at; at.b < line.end.b || (at.b == line.end.b && (at.seg < line.end.seg || (at.seg == line.end.seg && at.block < line.end.block)));) {
         const int b = at.b, seg = at.seg, h = seg / tiles, row0 = (seg - h * tiles) * kRows;
         const int len = visible_length(c, b), nb = max(1, (len + kBlock - 1) / kBlock);
         const int stop = b == line.end.b && seg == line.end.seg ? line.end.block : nb;
-        if (tid == 0 && cache_length(c, b) > len) s_status = kErrBadSeqlens;
+        if (tid == 0 && cache_length(c, b) > len) atomicOr(&s_status, kTooLong);
         const int tok0 = at.block * kBlock, tok1 = min(len, stop * kBlock);
         const int steps = tok1 > tok0 ? (tok1 - tok0 + 15) / 16 : 0;
 
         unsigned char* ring = att_sm + warp * kStages * kStageBytes;
-        const int mine = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;  // steps warp, warp + 8, ..
+        const int mine = steps > warp && !(phases & kGaveUp) ? (steps - warp + kWarps - 1) / kWarps : 0;  // steps warp, warp + 8, ..
         const int* trow = c.table + (size_t)b * c.max_pages;
         const int t_first = tok0 + 16 * warp;
         auto page_of = [&](int n) { return n < mine ? trow[(t_first + 16 * kWarps * n) >> c.page_shift] : 0; };
@@ -236,10 +240,6 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
             }
         };
         auto after = [](int at_) { return at_ + 1 == kStages ? 0 : at_ + 1; };
-        auto arrived = [&](int at_) {
-            if (!mbar_wait(bars + at_, (phases >> at_) & 1u, nullptr, 0)) s_status = kErrScanTmaTimeout;
-            phases ^= 1u << at_;
-        };
         int pg0 = page_of(0), pg1 = page_of(1), pg2 = page_of(2);  // pages of the steps in the ring
         issue(0, place, pg0);
         issue(1, after(place), pg1);
@@ -271,7 +271,10 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
             // 2^-e with top in [2^e, 2^(e+1)); kept within what 2^e and 2^-e can both hold
             const int ex = min(max((int)(__float_as_uint(top) >> 23), 2), 252);
             const float inv = __uint_as_float((uint32_t)(254 - ex) << 23);
-            if (x == 0) s_f[r] = __uint_as_float((uint32_t)ex << 23) * (p.scale * kLog2e);
+            if (x == 0) {
+                s_f[r] = __uint_as_float((uint32_t)ex << 23) * (p.scale * kLog2e);
+                s_lim[r] = len - p.Q + 1 + i;
+            }
             // dims 8 x .. 8 x + 7: lane x / 4, whose 32 dims are steps 0-7 four by four
             const int xl = x >> 2, s0 = 2 * (x & 3);
 #pragma unroll
@@ -287,7 +290,6 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
         // this thread's q rows of column tile j: row0 + 8 j + 2 (lane % 4) and the next
         float acc[NT][8][4], m[NT][2], l[NT][2], rf[NT][2];
         float inv[NT][2], vmax = 0.f;  // 1 / r; the largest value scale that none of these r has to move for
-        int lim[NT][2];  // positions that the rows see
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -301,7 +303,6 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
                 l[j][r] = 0.f;
                 rf[j][r] = s_f[row];
                 inv[j][r] = 0x1p120f;
-                lim[j][r] = len - p.Q + 1 + (row0 + row) / G;
             }
         }
         const int all_see = len - p.Q + 1 + row0 / G;  // positions that every row of the tile sees
@@ -342,6 +343,10 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
         };
         // The scores of a step are formed beside the softmax and the second product of the one before: a warp has two
         // chains to work on.  (Those behind the last step are formed from whatever the ring holds, and not used.)
+        auto arrived = [&](int at_) {
+            if (!mbar_wait(bars + at_, (phases >> at_) & 1u, nullptr, 0)) vmax = -1.f;  // below every scale: seen at the next step
+            phases ^= 1u << at_;
+        };
         float s[NT][4];
         bool odd = false;  // values that are not finite were left out where not every row sees them
         if (mine > 0) arrived(place);
@@ -349,7 +354,7 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
 #pragma unroll 1
         for (int n = 0; n < mine; ++n) {
             const bool ok = (unsigned)pg0 < (unsigned)c.pages;
-            if (!ok) s_status = kErrBadPage;
+            if (!ok) atomicOr(&s_status, kNoPage);
             const int t = t_first + 16 * kWarps * n;
             const bool some = t + 16 > all_see;  // not every row sees all of it
             const float ks0 = ks;
@@ -372,7 +377,7 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (!ok || t + (lane >> 2) + 8 * (e >> 1) >= lim[j][e & 1]) s[j][e] = -INFINITY;
+                        if (!ok || t + (lane >> 2) + 8 * (e >> 1) >= s_lim[8 * j + 2 * (lane & 3) + (e & 1)]) s[j][e] = -INFINITY;
                 if (!(vs0 < INFINITY)) {
                     vs0 = 0.f;
                     odd = true;
@@ -383,6 +388,15 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) over |= s[j][e] > m[j][e & 1] + kSlack;
             if (__any_sync(0xffffffffu, over || vs0 > vmax)) {
+                if (__any_sync(0xffffffffu, vmax < 0.f)) {
+                    phases |= kGaveUp;
+                    atomicOr(&s_status, kLate);
+                    for (int i = 1; i < kStages && n + i < mine; ++i) {  // let the other copies land (bounded)
+                        const int at_ = (place + i) % kStages;
+                        mbar_wait(bars + at_, (phases >> at_) & 1u, nullptr, 0);
+                    }
+                    break;
+                }
                 vmax = INFINITY;
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
@@ -491,7 +505,7 @@ __global__ void __launch_bounds__(att::kThreads, NT < 4 ? 2 : 1)
                 for (int j = 0; j < NT; ++j) {
                     float e[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) e[i] = t + (lane >> 2) + 8 * (i >> 1) < lim[j][i & 1] ? 1.f : 0.f;
+                    for (int i = 0; i < 4; ++i) e[i] = t + (lane >> 2) + 8 * (i >> 1) < s_lim[8 * j + 2 * (lane & 3) + (i & 1)] ? 1.f : 0.f;
                     const __half2 x = __floats2half2_rn(e[0], e[1]), y = __floats2half2_rn(e[2], e[3]);
                     w0[j] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&x));
                     w1[j] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&y));
@@ -590,16 +604,10 @@ __global__ void __launch_bounds__(128) gdn_cache_join_kernel(CacheAttendArgs p, 
     pdl_wait();
     pdl_trigger();
     if (blockIdx.x == 0 && blockIdx.y == 0) {  // the call's status: any of the CTAs'
-        bool late = false, page = false, length = false;
-        for (int i = threadIdx.x; i < (int)gridDim.x; i += 128) {
-            const int st = p.piece[i].z;
-            late |= st == kErrScanTmaTimeout;
-            page |= st == kErrBadPage;
-            length |= st == kErrBadSeqlens;
-        }
-        late = __syncthreads_or(late);
-        page = __syncthreads_or(page);
-        length = __syncthreads_or(length);
+        int met = 0;
+        for (int i = threadIdx.x; i < (int)gridDim.x; i += 128) met |= p.piece[i].z;
+        const bool late = __syncthreads_or(met & att::kLate), page = __syncthreads_or(met & att::kNoPage);
+        const bool length = __syncthreads_or(met & att::kTooLong);
         if (threadIdx.x == 0) *p.status = late ? kErrScanTmaTimeout : page ? kErrBadPage : length ? kErrBadSeqlens : 0;
     }
     const int4 pc = p.piece[blockIdx.x];

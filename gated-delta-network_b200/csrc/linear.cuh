@@ -91,7 +91,7 @@ struct CacheAttendArgs {
     float scale;
     uint16_t* out;         // [B, Q, Hq, 128] bf16
     int* status;           // workspace
-    int4* piece;           // workspace: [kAttendCtas] {segment that CTA c begins and others end, pieces that follow, status}
+    int4* piece;           // workspace: [kAttendCtas] {segment that CTA c begins and others end, pieces that follow, what it met}
     float* ml;             // workspace: [CTAs][2][rows of a tile][2] reference (base 2) and sum of a piece
     float* acc;            // workspace: [CTAs][2][rows of a tile][128]
 };

@@ -55,7 +55,8 @@ def _launch(dev, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, s
 
 def kernel(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, output, *, workspace=None):
     """Destination-passing form of ``run``: writes ``output`` [B, Q, Hq, 128] bf16.  ``workspace``: a CUDA buffer of
-    at least ``workspace_bytes()`` bytes, 256-byte aligned, for callers that keep one."""
+    at least ``workspace_bytes()`` bytes, 256-byte aligned, for callers that keep one; ``read_status`` of it tells whether
+    the call went well (a call without a sequence or a q row leaves the status as it was)."""
     if output is None:
         raise ValueError("output must be given")
     _launch(cuda_device(q, "q"), q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, output, workspace)

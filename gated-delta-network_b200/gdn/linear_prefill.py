@@ -75,7 +75,8 @@ def run(q, k, v, state, log_decay, cu_seqlens, scale):
 def kernel(q, k, v, state, log_decay, cu_seqlens, scale, output, new_state, *, workspace=None):
     """Destination-passing prefill: writes ``new_state`` (which may be ``state`` itself) and the rows of
     ``output`` that belong to a sequence; the others are left as they were.  ``workspace``: a CUDA buffer of at
-    least ``workspace_bytes(N, T, H, HV)`` bytes, 256-byte aligned, for callers that keep one."""
+    least ``workspace_bytes(N, T, H, HV)`` bytes, 256-byte aligned, for callers that keep one; ``read_status`` of it tells
+    whether the call went well (a call without a sequence leaves the status as it was)."""
     if output is None or new_state is None:
         raise ValueError("output and new_state must be given")
     _launch(cuda_device(q, "q"), q, k, v, state, log_decay, cu_seqlens, scale, output, new_state, workspace, 0)

@@ -215,6 +215,7 @@ int gdn_linear_decode_fwd(const void* q, const void* k, const void* v, const flo
  * (256-byte aligned, at least gdn_linear_prefill_workspace_bytes) carries nothing between calls; its first
  * int receives 0 or a GDN_DEVSTATUS_* code: a bounded device-side wait that gave up, or BAD_SEQLENS where
  * overlapping sequences claim more chunks than T tokens in N sequences can have; then no sequence is computed.
+ * A call without a sequence leaves it as it was.
  */
 size_t gdn_linear_prefill_workspace_bytes(int N, int T, int H, int HV, int K, int V);
 int gdn_linear_prefill_fwd(const void* q, const void* k, const void* v, const float* state, const float* log_decay,
@@ -246,8 +247,9 @@ int gdn_linear_prefill_fwd(const void* q, const void* k, const void* v, const fl
  * step), already appended; Hq is a multiple of Hkv and q head h reads kv head h / (Hq / Hkv).  Row i sees
  * positions j < seq_len - Q + 1 + i; a row that sees none gets zeros.  out [B, Q, Hq, 128] bf16.  The
  * workspace (256-byte aligned, at least gdn_cache_attend_workspace_bytes) carries nothing between calls;
- * calls that can overlap need one each.  Its first int receives 0 or a GDN_DEVSTATUS_* code.
- * flags must be 0.
+ * calls that can overlap need one each.  Its first int receives 0 or a GDN_DEVSTATUS_* code, the gravest
+ * of TMA_TIMEOUT, BAD_PAGE, BAD_SEQLENS; a call without a sequence or a q row launches nothing and leaves it
+ * as it was.  flags must be 0.
  */
 #define GDN_CODE_INT8 0
 #define GDN_CODE_E4M3 1

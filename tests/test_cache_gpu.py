@@ -482,3 +482,17 @@ def test_a_page_of_other_size_and_little_weight(code, ratio, Q, page):
         tol = 2.0 ** -8 * o.abs() + (2.0 ** -10 + 2 * d.amax(-1, keepdim=True)) * (w @ V[:m].abs()) + m * 2.0 ** -25 * (w * size[:m]).amax(-1, keepdim=True)
         e = (out[0, i] - o).abs()
         assert (e <= tol).all(), f"row {i} off by {(e / tol).max().item():.2f} times its bound"
+
+
+def test_the_gravest_status_of_a_block_is_kept():
+    """A bad page, then a sequence longer than its row of the table, wherever the two fall among the blocks."""
+    f = Filled([20] * 700, 1, 16, "int8", more=[0] * 700)
+    q = f.q(1, 2)
+    ws = torch.empty(gdn.cache_attend.workspace_bytes(), dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(q)
+    for b in range(300, 306):
+        table, seq = f.table.clone(), f.seq.clone()
+        table[b, 0] = -1
+        seq[b + 1] = 1000
+        gdn.cache_attend.kernel(q, *f.args()[:4], table, seq, SCALE, out, workspace=ws)
+        assert gdn.cache_attend.read_status(ws) == 6
