@@ -47,8 +47,9 @@ constexpr uint32_t kStage = 49152;
 constexpr uint32_t kOffP = kStages * kStage;     // P [2][64 i][64 j] bf16
 constexpr uint32_t kOffO = kOffP + 2 * 8192;     // output staging [2][2 atoms][64 tokens][64 V] bf16, SWIZZLE_128B
 constexpr uint32_t kOffG = kOffO + 2 * 16384;    // gates, kGates slots of f32: [64] G | [64] factors of OI | [64] of v | [64] e^{G_b - G}, b the
-                                                 // last of the token's block of 16 | state: factor, unit at the end, log of the decay, whether to multiply
-constexpr uint32_t kGateFloats = 264;
+                                                 // last of the token's block of 16 | state: factor, unit at the end, log of the decay, whether to multiply;
+                                                 // of v: int [8] whether 16 V have a value that is not finite | int [128] its first token
+constexpr uint32_t kGateFloats = 400, kOdd = 264, kOddFrom = 272;
 constexpr uint32_t kOffBar = kOffG + kGates * kGateFloats * 4;
 constexpr uint32_t kOffRange = kOffBar + 512;
 constexpr uint32_t kSmem = kOffRange + 256;
@@ -580,6 +581,27 @@ __device__ __forceinline__ bool role_p(const LinearPrefillArgs& p, const LinCtx&
     return true;
 }
 
+// Column v of a staged [2 atoms][64 tokens][64 V] bf16 tile becomes NaN from token `from` on.
+__device__ __noinline__ void void_odd_v(unsigned char* tile, int v, int from) {
+    for (int t = from; t < 64; ++t)
+        *reinterpret_cast<uint16_t*>(tile + (v >> 6) * 8192 + t * 128 + ((((v >> 3) & 7) ^ (t & 7)) << 4) + (v & 7) * 2) = 0x7fff;
+}
+// By a warp: of the 64 tokens and the V columns v0 .. v0 + 15 of a v tile, values that are not finite become 0, and `from`
+// gets the first token of one for each V (64: there is none).
+__device__ __noinline__ void hide_odd_v(unsigned char* tile, int* from, int v0) {
+    const int lane = threadIdx.x & 31, v = v0 + (lane & 15);
+    int first = 64;
+    for (int t = lane >> 4; t < 64; t += 2) {
+        uint16_t* at = reinterpret_cast<uint16_t*>(tile + (v >> 6) * 8192 + t * 128 + ((((v >> 3) & 7) ^ (t & 7)) << 4) + (v & 7) * 2);
+        if ((*at & 0x7f80u) == 0x7f80u) {
+            *at = 0;
+            first = min(first, t);
+        }
+    }
+    first = min(first, __shfl_xor_sync(0xffffffffu, first, 16));
+    from[v] = first;
+}
+
 // Warps 8-15: the decayed v, transposed, as three bf16 parts in TMEM (lane = V index, two tokens a column); 16 V a warp.
 template <bool kOut>
 __device__ __forceinline__ bool role_v(const LinearPrefillArgs& p, const LinCtx& x) {
@@ -613,8 +635,8 @@ __device__ __forceinline__ bool role_v(const LinearPrefillArgs& p, const LinCtx&
                 fence_async_smem();
                 named_bar_sync(1, 256);
             }
-            if (kOut && lane == 0) mbar_arrive(&lin_bars()->v_full[g % kGates]);
             uint32_t part[3][16];
+            float2 zero = make_float2(0.f, 0.f);  // NaN if one of the values is not finite
 #pragma unroll
             for (int i = 0; i < 4; ++i) {  // 16 V x 16 tokens, transposed
                 uint32_t raw[4];
@@ -622,6 +644,7 @@ __device__ __forceinline__ bool role_v(const LinearPrefillArgs& p, const LinCtx&
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {  // {0, 1}: tokens 16 i + .., {2, 3}: 8 later; odd ones are 8 V further
                     float2 y = mul2(bf2_to_f2(raw[j]), *reinterpret_cast<const float2*>(er + 16 * i + 8 * (j >> 1)));
+                    if (kOut) zero = fma2(y, make_float2(0.f, 0.f), zero);
 #pragma unroll
                     for (int k = 0; k < 3; ++k) {
                         part[k][4 * i + j] = pack_bf16x2(y.x, y.y);
@@ -636,6 +659,19 @@ __device__ __forceinline__ bool role_v(const LinearPrefillArgs& p, const LinCtx&
             tmem_st_wait();
             tc_fence_before();
             mbar_arrive(&lin_bars()->u_ready);
+            if (kOut) {
+                const bool odd = __any_sync(0xffffffffu, !(zero.x + zero.y == 0.f));
+                int* note = reinterpret_cast<int*>(lin_gates(g) + kOdd);
+                if (lane == 0) note[2 * quarter + hf] = odd;
+                if (odd) {
+                    // P is 0 for a later token, but 0 NaN is NaN: OA gets 0 in place of such values, and the outputs of that
+                    // V become NaN from its token on (the state does by U).
+                    hide_odd_v(st + kOffV, note + (kOddFrom - kOdd), 32 * quarter + 16 * hf);
+                    fence_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&lin_bars()->v_full[g % kGates]);
+            }
             if (++s == kStages) {
                 s = 0;
                 s_ph ^= 1;
@@ -696,6 +732,13 @@ __device__ __forceinline__ bool role_o(const LinearPrefillArgs& p, const LinearM
             }
             tc_fence_before();
             mbar_arrive(&lin_bars()->o_empty);
+            LIN_WAIT(lin_bars()->v_full[g % kGates], g / kGates);
+            const int* note = reinterpret_cast<const int*>(eg - 64);
+            const int2 odd = *reinterpret_cast<const int2*>(note + kOdd + 2 * quarter);
+            if (odd.x | odd.y) {
+                __syncwarp();
+                if (lane < 16 ? odd.x : odd.y) void_odd_v(lin_sm + kOffO + buf, 32 * quarter + lane, note[kOddFrom + 32 * quarter + lane]);
+            }
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&lin_bars()->g_empty[g % kGates]);

@@ -307,3 +307,23 @@ def test_sequences_that_overlap_too_much_are_reported(N, T):
     assert (out[::997] == 3).all() and (ns[-1] == 3).all()
     gdn.linear_prefill.kernel(q, k, v, None, torch.zeros(1, device="cuda"), cu[:2], SCALE, out, ns[:1], workspace=ws)
     assert gdn.linear_prefill.read_status(ws) == 0 and not out.any() and not ns[0].any()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("lens,tokens", [([64], [0, 63]), ([64], [40]), ([100, 30], [10, 99, 115]), ([2500, 3], [1, 1300, 2400]),
+                                         ([200] * 3, [63, 64, 300, 463, 599])])
+def test_v_that_is_not_finite_reaches_later_tokens_only(bad, lens, tokens):
+    """Its V column of the head, from its token on; the tokens before it in the same chunk keep their values."""
+    x = ref.inputs(lens, 2, 4, seed=13)
+    v = x[2]
+    want = ref.reference(*x, SCALE)
+    for i, t in enumerate(tokens):
+        v[t, i % 4, 37 * i % 128] = bad
+        v[t, i % 4, 127 - i] = bad
+    dirty = ref.reference(*x, SCALE)
+    out, ns = _run(x)
+    for got, bad_ref in ((out, dirty[0]), (ns, dirty[1])):
+        hit = ~torch.isfinite(bad_ref)
+        assert torch.equal(~torch.isfinite(got.double()), hit) and hit.any()
+    fill = lambda got, ref_, hit: torch.where(hit, ref_.to(got.dtype), got)  # noqa: E731
+    ref.check(fill(out, want[0], ~torch.isfinite(dirty[0])), fill(ns, want[1], ~torch.isfinite(dirty[1])), want, chunked=True)
