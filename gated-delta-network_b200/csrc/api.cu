@@ -297,7 +297,8 @@ int cache_args(void* k_cache, void* v_cache, float* k_scale, float* v_scale, int
     int shift = 4;
     while (shift < 7 && (1 << shift) != page_size) ++shift;
     if ((1 << shift) != page_size) return GDN_ERR_SIZE;
-    if (num_pages < 0 || max_pages < 0 || ((long long)max_pages << shift) > 0x7fffffffll || B < 0 ||
+    // positions are ints, and some way behind a sequence's end is counted too
+    if (num_pages < 0 || max_pages < 0 || ((long long)max_pages << shift) > (1ll << 30) || B < 0 ||
         (len_is_int64 != 0 && len_is_int64 != 1))
         return GDN_ERR_SIZE;
     if (B == 0) return GDN_OK;

@@ -231,7 +231,8 @@ int gdn_linear_prefill_fwd(const void* q, const void* k, const void* v, const fl
  *   k_cache, v_cache [num_pages, Hkv, page_size, D=128] codes, int8 (GDN_CODE_INT8) or e4m3 (GDN_CODE_E4M3);
  *                    a value is code * scale.  16-byte aligned.  page_size is 16, 32, 64 or 128.
  *   k_scale, v_scale [num_pages, Hkv]  f32, >= 0
- *   block_table      [B, max_pages]    int32, device: page i of a sequence holds its tokens i * page_size ..
+ *   block_table      [B, max_pages]    int32, device: page i of a sequence holds its tokens i * page_size ..;
+ *                                      at most 2^30 tokens a row
  *   seq_lens         [B]               int32 / int64, device: tokens of each sequence, counting the call's
  *                                      new ones; 0 for an unused row of a padded batch
  *

@@ -65,3 +65,13 @@ def test_python_refuses_cpu_tensors():
         gdn.cache_attend.run(q, c, c, s, s, i[None], i, None)
     with pytest.raises(ValueError, match="CUDA"):
         gdn.cache_append.kernel(q[0, :, :2], q[0, :, :2], c, c, s, s, i[None], i, torch.tensor([0, 1]))
+
+
+@pytest.mark.parametrize("call", [_append, _attend])
+@pytest.mark.parametrize("P", [16, 128])
+def test_rows_of_the_table_hold_at_most_2_30_tokens(lib, call, P):
+    """Above it, positions behind a sequence's end would not be ints."""
+    empty = dict(T=0) if call is _append else dict(Q=0)
+    assert call(lib, P=P, max_pages=(1 << 30) // P, **empty) == 0
+    assert call(lib, P=P, max_pages=(1 << 30) // P + 1, **empty) == 4
+    assert call(lib, P=P, max_pages=((1 << 31) - P) // P, **empty) == 4
