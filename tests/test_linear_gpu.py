@@ -327,3 +327,43 @@ def test_v_that_is_not_finite_reaches_later_tokens_only(bad, lens, tokens):
         assert torch.equal(~torch.isfinite(got.double()), hit) and hit.any()
     fill = lambda got, ref_, hit: torch.where(hit, ref_.to(got.dtype), got)  # noqa: E731
     ref.check(fill(out, want[0], ~torch.isfinite(dirty[0])), fill(ns, want[1], ~torch.isfinite(dirty[1])), want, chunked=True)
+
+
+@pytest.mark.parametrize("what", ["q", "k", "decay", "state"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_is_not_finite_stays_where_it_belongs(what, bad):
+    """q in its token, k and the decay from their token on, a state in its sequence and V rows."""
+    if what == "decay":
+        bad = float("nan")  # log decays are at most 0
+    lens = [130, 64, 300]
+    x = ref.inputs(lens, 2, 4, seed=14)
+    q, k, v, st, a, cu = x
+    want = ref.reference(*x, SCALE)
+    if what == "state":
+        st[1, 2, 17, 3] = bad
+    else:
+        t = {"q": q, "k": k, "decay": a}[what]
+        for i in (40, 150, 194 + 64, 194 + 299):
+            t[(i, 1, 5) if what != "decay" else (i, 1)] = bad
+    dirty = ref.reference(*x, SCALE)
+    out, ns = _run(x)
+    hit = [~torch.isfinite(dirty[0]), ~torch.isfinite(dirty[1])]
+    assert torch.equal(~torch.isfinite(out), hit[0]) and torch.equal(~torch.isfinite(ns), hit[1]) and hit[0].any()
+    ref.check(torch.where(hit[0], want[0].to(out.dtype), out), torch.where(hit[1], want[1].float(), ns), want, chunked=True)
+
+
+@pytest.mark.parametrize("HV", [1, 8])
+def test_the_state_keeps_24_bits_of_a_decayed_v(HV):
+    """Keys of one 1 each: every column of the state holds one decayed v, and no sum hides what it lost.
+
+    The exponents stay below 1, so each of their sums is off by 2^-25 at most: some 30 of them, over two chunks, move a
+    result by 30 * 2^-25 * ln 2 = 6.2e-7; two exponentials of 2^-22 each and four fp32 roundings of 2^-24 add 7.2e-7.
+    That is below 2^-19 = 1.9e-6.  Two bf16 parts of the decayed v would be off by up to 2^-17 = 7.6e-6.
+    """
+    g = torch.Generator().manual_seed(15)
+    k = torch.eye(128)[torch.randperm(128, generator=g)][:, None].to(torch.bfloat16).cuda()
+    v = torch.randn((128, HV, 128), generator=g).to(torch.bfloat16).cuda()
+    a = (-0.005 * torch.rand((128, HV), generator=g)).cuda()
+    want = ref.reference(k, k, v, None, a, [0, 128], SCALE)
+    _, ns = _run((k, k, v, None, a, [0, 128]))
+    assert ((ns.double() - want[1]).abs() <= 2.0 ** -19 * want[1].abs()).all()
