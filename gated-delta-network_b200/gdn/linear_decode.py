@@ -52,7 +52,7 @@ def run(q, k, v, state, log_decay, scale):
 
     q, k [B,1,H,128] bf16; v [B,1,HV,128] bf16, HV a multiple of H (v-head hv reads q/k head
     hv // (HV // H)); state [B,HV,128,128] fp32 (k-last) or None (zeros); log_decay fp32, <= 0, either [HV]
-    (one decay for each head) or [B,1,HV] (one for each sequence and head; -inf forgets the state);
+    (one decay for each head) or [B,1,HV] (one for each sequence and head; -inf forgets a finite state);
     scale float, 0-d tensor, or None/0 (1/sqrt(128)).
     """
     return _launch(cuda_device(q, "q"), q, k, v, state, log_decay, scale, None, None)

@@ -64,7 +64,7 @@ def run(q, k, v, state, log_decay, cu_seqlens, scale):
 
     q, k [T,H,128] bf16; v [T,HV,128] bf16, HV a multiple of H (v-head hv reads q/k head hv // (HV // H));
     state [N,HV,128,128] fp32 or None (zeros); log_decay fp32, <= 0, either [HV] (one decay for each head) or
-    [T,HV] (one for each token and head; -inf forgets the state before the token); cu_seqlens [N+1]
+    [T,HV] (one for each token and head; -inf forgets a finite state before the token); cu_seqlens [N+1]
     int32/int64; scale float, 0-d tensor, or None/0 (1/sqrt(128)).  A value of v that is not finite makes its V
     column of the head NaN from its token on, in the outputs and the state; earlier tokens keep theirs.  A zero-length sequence keeps its state;
     tokens outside every sequence get a zero output.

@@ -197,7 +197,7 @@ int gdn_prefill_fwd_noalloc(const void* q, const void* k, const void* v, const f
  * and without the delta correction,
  *   S <- e^a S + v k^T,   out = scale S q        (S is [V][K], fp32, k-last)
  * with the log decay a <= 0 given for each head (decay_per_token = 0: log_decay [HV]) or for each token and
- * head (decay_per_token = 1: log_decay [B, HV] or [T, HV]), f32.  -infinity forgets the state.  Neither
+ * head (decay_per_token = 1: log_decay [B, HV] or [T, HV]), f32.  -infinity forgets a finite state.  Neither
  * entry point has a counterpart in the reference.
  *
  * gdn_linear_decode_fwd: one token for each of B sequences.  Tensors as for gdn_decode_fwd; new_state may
