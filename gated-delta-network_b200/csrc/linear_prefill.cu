@@ -20,9 +20,9 @@
 // 128 KB a chunk off the shared-memory bandwidth.  Every product and every group of warps works on a chunk of its own: TMA
 // and gates run ahead, the P and V warps prepare chunk c + 1 while the tensor core works on c and the output warps write
 // c - 1.  Loops stay rolled: unrolled, the roles together missed the instruction cache and warps waited 2.9 clocks an
-// instruction for it, 0.5 now.  4 q/k and 8 v heads: 64 x 4096 tokens 440 to 465 us (3.6 to 3.8 TB/s, 0.30 PFLOP/s; 520 to
-// 545 at the power cap, called for a second on end), 16 of 6 to 8192 93, 1 x 8192 46, 1 x 100 10.9.  Not better: 1024 threads with a second group of warps for P; OI in tf32 from
-// the fp32 state without the bf16 copy (64 x 4096 443 -> 485).
+// instruction for it, 0.5 now.  4 q/k and 8 v heads: 64 x 4096 tokens 440 to 465 us (3.6 to 3.8 TB/s, 0.30 PFLOP/s; 520
+// to 545 at the power cap, called for a second on end), 16 of 6 to 8192 93, 1 x 8192 46, 1 x 100 10.9.  Not better: 1024
+// threads with a second group of warps for P; OI in tf32 from the fp32 state without the bf16 copy (64 x 4096 443 -> 485).
 //
 // Tokens are cut evenly over the CTAs whatever the lengths: all (sequence, v-head) segments lie on one line in
 // chunks, and a CTA takes an equal stretch of it.  The state at a stretch's start comes from two launches before:
@@ -735,8 +735,7 @@ __device__ __forceinline__ bool role_o(const LinearPrefillArgs& p, const LinearM
             LIN_WAIT(lin_bars()->v_full[g % kGates], g / kGates);
             const int* note = reinterpret_cast<const int*>(eg - 64);
             const int2 odd = *reinterpret_cast<const int2*>(note + kOdd + 2 * quarter);
-            if (odd.x | odd.y) {
-                __syncwarp();
+            if ((odd.x | odd.y) && __all_sync(0xffffffffu, ok)) {  // (the notes are there)
                 if (lane < 16 ? odd.x : odd.y) void_odd_v(lin_sm + kOffO + buf, 32 * quarter + lane, note[kOddFrom + 32 * quarter + lane]);
             }
             fence_async_smem();
